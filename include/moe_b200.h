@@ -14,7 +14,8 @@
  *     (a cudaStream_t passed as void*).
  *   - Return value: MOE_B200_OK or a negative MOE_B200_ERR_* (see moe_b200_error_string).
  *   - `status` is a device int32 word the kernels set non-zero when they notice a problem while
- *     running (a bounded wait that ran out = 1, an expert id out of range = 2). The host reads it
+ *     running (a bounded wait that ran out = 1, an expert id out of range = 2, run starts that
+ *     decrease or leave the rows = 3). The host reads it
  *     whenever it wants to pay for the synchronisation.
  *   - "slot order": pairs (token, expert) sorted by expert, every expert's run padded to a
  *     multiple of 128 rows; pad slots hold the sentinel n_pairs in sorted_ids and zero rows in
@@ -46,6 +47,11 @@ extern "C" {
 #define MOE_B200_ACT_RELU 2
 #define MOE_B200_ACT_SIGMOID 3
 #define MOE_B200_ACT_TANH 4
+
+/* Element types of the entry points that take more than bf16. */
+#define MOE_B200_BF16 0
+#define MOE_B200_FP16 1
+#define MOE_B200_FP32 2
 
 /* ABI version of this header. */
 int32_t moe_b200_abi_version(void);
@@ -651,6 +657,67 @@ int moe_b200_stack_infer(const void* plan, int32_t n_layers, const void* x, void
                          int32_t n_shared, int32_t top_k, int32_t normalize, int32_t activation,
                          void* scratch, size_t scratch_bytes, int32_t* n_launches, int32_t* status,
                          void* stream);
+
+/* ---- Products grouped by expert over ragged runs --------------------------------------------------
+ * offsets [n_groups + 1]: rows offsets[g] .. offsets[g + 1] belong to group g, back to back, of any
+ * length (also none); n_groups <= 1024. Starts that decrease or leave [0, rows] are taken into range
+ * and reported through status. dtype MOE_B200_BF16 or MOE_B200_FP16; widths and strides are
+ * multiples of 8 elements; fp32 sums, rounded once.
+ *
+ * moe_b200_grouped_mm: y [rows, n_dim] = x[r] @ w[g(r)], x [rows, k_dim] with ld_x elements between
+ * rows. n_inner != 0: w[g] is [k_dim, n_dim] with n contiguous and ld_w elements between k;
+ * 0: w[g] is [n_dim, k_dim] with k contiguous (the gradient of x is the call with dy for x and the
+ * same w read the other way). Rows of no run are zero.
+ * moe_b200_grouped_wgrad: dw[g] [m_dim, n_dim] = sum over g's rows of a[r]^T b[r]; zero without rows.
+ * Summed in a fixed order (bit-reproducible). scratch: 32-byte aligned. */
+int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* w,
+                        int32_t n_groups, int64_t w_group_stride, int64_t ld_w, int32_t n_inner,
+                        int32_t n_dim, const int32_t* offsets, int32_t dtype, void* y, int32_t* status,
+                        void* stream);
+size_t moe_b200_grouped_wgrad_scratch_bytes(int32_t m_dim, int32_t n_dim, int64_t rows,
+                                            int32_t n_groups);
+int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const void* b, int64_t ld_b,
+                           int32_t n_dim, int64_t rows, const int32_t* offsets, int32_t n_groups,
+                           int32_t dtype, void* dw, void* scratch, size_t scratch_bytes, int32_t* status,
+                           void* stream);
+
+/* ---- Weights in 4 bits -----------------------------------------------------------------------------
+ * W[k, n] = (level[k, n] - 8) * scale[k / group, n], level 0 .. 15, group 32 or a multiple of 64; the
+ * last group may be short. Packed once per matrix (nanospeaker_b200/int4.py does it), the outputs in
+ * strips of 16, the inputs in blocks of 64, padded with level 8:
+ *   levels [strips][blocks][32 lanes][4 words]: nibble i of the low / high half of word j of lane
+ *     4 * g + t is input 64 * block + 32 * (j / 2) + 8 * t + 4 * (j % 2) + 2 * (i / 2) + {0, 1},
+ *     output 16 * strip + g + 8 * (i % 2)
+ *   scales [strips][groups][8][2] in the activations' type: outputs g and g + 8
+ * x, y, topk_w: bf16 or fp16 (dtype), k_dim a multiple of 8; fp32 sums.
+ *
+ * moe_b200_int4_mm: y [rows, n_dim] = x [rows, k_dim] @ W.
+ * moe_b200_int4_experts: out[t] = sum_j topk_w[t, j] * expert topk_idx[t, j] of x[t], plus the shared
+ * experts of x[t]; an expert is (act(gate) * up) @ W_out with gate | up = x @ W_in, W_in
+ * [d_model, 2 * d_hidden], d_hidden a multiple of 16. No dispatch comes before it. A pair whose expert
+ * does not exist adds nothing and is reported through status. scratch: 16-byte aligned. Bit-
+ * reproducible. */
+int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* levels,
+                     const void* scales, int32_t group, int32_t n_dim, int32_t dtype, void* y,
+                     void* stream);
+size_t moe_b200_int4_experts_scratch_bytes(int64_t n_tokens, int32_t top_k, int32_t n_shared,
+                                           int32_t d_model, int32_t d_hidden);
+int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t d_model,
+                          int32_t d_hidden, const void* topk_w, const int64_t* topk_idx, int32_t top_k,
+                          int32_t n_experts, const void* in_levels, const void* in_scales,
+                          const void* out_levels, const void* out_scales, int32_t n_shared,
+                          const void* sh_in_levels, const void* sh_in_scales, const void* sh_out_levels,
+                          const void* sh_out_scales, int32_t group, int32_t activation, int32_t dtype,
+                          void* out, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
+
+/* ---- Dropout -----------------------------------------------------------------------------------------
+ * out[i] = residual[i] (0 when NULL) + (word(i) >= p * 2^32 ? x[i] / (1 - p) : 0) over n elements,
+ * word(i) = word i % 4 of Philox4x32-10 at counter (i / 4, call) under the key seed, (seed, call) the two
+ * int64 at rng (device). used (may be NULL) receives a copy of them: the backward is the call on the
+ * gradient with that state and no residual. 0 <= p < 1; dtype bf16, fp16 or fp32. out may be x or
+ * residual. */
+int moe_b200_dropout(const void* x, const void* residual, int64_t n, int32_t dtype, double p,
+                     const int64_t* rng, int64_t* used, void* out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,7 +8,7 @@ namespace moe {
 enum Act { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3, ACT_TANH = 4 };
 
 // Status codes a kernel can leave in the status word (0 = fine).
-enum DevStatus { ST_OK = 0, ST_WAIT_TIMEOUT = 1, ST_BAD_EXPERT = 2 };
+enum DevStatus { ST_OK = 0, ST_WAIT_TIMEOUT = 1, ST_BAD_EXPERT = 2, ST_BAD_OFFSETS = 3 };
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float g) {

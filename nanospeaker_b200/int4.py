@@ -1,0 +1,229 @@
+"""Weights in 4 bits with group scales, for batches that generate: few rows, so that the weights' bytes are
+the time. W[k, n] = (level[k, n] - 8) * scale[k // group, n] with levels 0 .. 15.
+
+  quantize_int4(w)     a weight (or a stack of them) rounded to an Int4Weight, once
+  int4_mm(x, weight)   x @ W
+  int4_experts(...)    the block's routed and shared GLU experts; beside `fused_moe_forward`, whose
+                       weights are 16-bit
+
+Inference only: there are no gradients. Kernels: csrc/int4.cu.
+"""
+from typing import Optional
+
+import torch
+
+from . import kernels as K
+from .moe_kernel import _act_id
+
+INT4_DTYPES = (torch.bfloat16, torch.float16)
+
+
+class Int4Weight:
+    """A matrix [K, N] (x @ W), or a stack [G, K, N] of them, in 4 bits, laid out as the kernels read it.
+
+    shape     (K, N) or (G, K, N)
+    group     inputs that share a scale: 32 or a multiple of 64 (the last group of a matrix may be short)
+    levels    int32 [G, ceil(N / 16), ceil(K / 64), 32, 4]
+    scales    [G, ceil(N / 16), groups, 8, 2], bf16 or fp16: the dtype of the activations"""
+
+    def __init__(self, levels: torch.Tensor, scales: torch.Tensor, shape, group: int):
+        self.levels, self.scales, self.shape, self.group = levels, scales, tuple(shape), group
+
+    dtype = property(lambda self: self.scales.dtype)
+    device = property(lambda self: self.levels.device)
+
+    def to(self, device) -> "Int4Weight":
+        return Int4Weight(self.levels.to(device), self.scales.to(device), self.shape, self.group)
+
+    @classmethod
+    def from_levels(cls, levels: torch.Tensor, scales: torch.Tensor, group: int) -> "Int4Weight":
+        """From uint8 levels [..., K, N] (0 .. 15, the value is level - 8) and scales
+        [..., ceil(K / group), N]."""
+        if levels.dtype != torch.uint8 or levels.dim() not in (2, 3):
+            raise ValueError(f"levels are uint8 [K, N] or [G, K, N], got {levels.dtype} "
+                             f"{tuple(levels.shape)}")
+        if scales.dtype not in INT4_DTYPES:
+            raise ValueError(f"scales are bf16 or fp16, got {scales.dtype}")
+        _check_group(group)
+        k, n = levels.shape[-2:]
+        if k < 8 or k % 8 or n < 1:
+            raise ValueError(f"a weight of {k} inputs and {n} outputs: inputs have to be a multiple of 8")
+        if tuple(scales.shape) != (*levels.shape[:-2], -(-k // group), n):
+            raise ValueError(f"levels {tuple(levels.shape)} in groups of {group} do not take scales "
+                             f"{tuple(scales.shape)}")
+        q = levels.reshape(-1, k, n)
+        g, kb, ns = q.shape[0], -(-k // 64), -(-n // 16)
+        kg = -(-kb * 64 // group)
+        if (kb * 64, ns * 16) != (k, n):
+            padded = q.new_full((g, kb * 64, ns * 16), 8)
+            padded[:, :k, :n] = q
+            q = padded
+        # input 64 kb + 32 half + 8 t + 4 j + 2 hi + b, output 16 ns + 8 i + lane row: bit 4 (2 hi + i) + 16 b
+        # of word 2 half + j of lane 4 row + t
+        q = q.view(g, kb, 2, 4, 2, 2, 2, ns, 2, 8)
+        bits = torch.zeros((), dtype=torch.int32, device=q.device)
+        for hi in range(2):
+            for b in range(2):
+                for i in range(2):
+                    part = q[:, :, :, :, :, hi, b, :, i].to(torch.int32)
+                    bits = bits | (part << (4 * (2 * hi + i) + 16 * b))
+        # [g, kb, half, t, j, ns, row] -> [g, ns, kb, row, t, half, j]
+        packed = bits.permute(0, 5, 1, 6, 3, 2, 4).reshape(g, ns, kb, 32, 4).contiguous()
+        s = scales.new_zeros((g, kg, ns * 16))
+        s[:, :scales.shape[-2], :n] = scales.reshape(g, -1, n)
+        s = s.view(g, kg, ns, 2, 8).permute(0, 2, 1, 4, 3).contiguous()
+        return cls(packed, s, levels.shape, group)
+
+    def to_levels(self):
+        """(levels, scales) as from_levels takes them."""
+        k, n = self.shape[-2:]
+        g, ns, kb = self.levels.shape[:3]
+        words = self.levels.view(g, ns, kb, 8, 4, 2, 2)       # row, t, half, j
+        shift = torch.arange(2, device=self.device)
+        bit = (8 * shift[:, None, None] + 16 * shift[None, :, None] + 4 * shift[None, None, :])
+        q = (words[..., None, None, None] >> bit.to(torch.int32)) & 15   # hi, b, i
+        q = q.permute(0, 2, 5, 4, 6, 7, 8, 1, 9, 3).reshape(g, kb * 64, ns * 16)[:, :k, :n]
+        s = self.scales.permute(0, 2, 1, 4, 3).reshape(g, -1, ns * 16)[:, :-(-k // self.group), :n]
+        return (q.to(torch.uint8).reshape(self.shape),
+                s.reshape(*self.shape[:-2], *s.shape[-2:]).contiguous())
+
+    def dequantize(self) -> torch.Tensor:
+        """The weight in fp32."""
+        q, s = self.to_levels()
+        k = q.shape[-2]
+        return (q.float() - 8) * s.float().repeat_interleave(self.group, -2)[..., :k, :]
+
+
+def _check_group(group: int) -> None:
+    if group != 32 and (group < 64 or group % 64):
+        raise ValueError(f"scale groups of {group} inputs: 32 or a multiple of 64")
+
+
+def quantize_int4(w: torch.Tensor, group: int = 64, dtype: Optional[torch.dtype] = None) -> Int4Weight:
+    """w [K, N] or [G, K, N] rounded to 4 bits: a group's scale is its largest magnitude / 7, in `dtype`
+    (default: w's, bf16 for fp32), its levels the nearest ones. Non-finite weights raise."""
+    dtype = dtype or (w.dtype if w.dtype in INT4_DTYPES else torch.bfloat16)
+    if w.dim() not in (2, 3):
+        raise ValueError(f"a weight is [K, N] or [G, K, N], got {tuple(w.shape)}")
+    if dtype not in INT4_DTYPES:
+        raise ValueError(f"scales are bf16 or fp16, got {dtype}")
+    _check_group(group)
+    w = w.detach().float()
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("a weight with infinities or NaN cannot be held in 4 bits")
+    k, n = w.shape[-2:]
+    groups = -(-k // group)
+    padded = torch.nn.functional.pad(w, (0, 0, 0, groups * group - k))
+    blocks = padded.view(*w.shape[:-2], groups, group, n)
+    scales = (blocks.abs().amax(-2) / 7).to(dtype)
+    s = scales.float().unsqueeze(-2)
+    levels = torch.where(s > 0, blocks / s, 0.0).round().clamp(-8, 7) + 8
+    levels = levels.to(torch.uint8).view(*w.shape[:-2], groups * group, n)[..., :k, :].contiguous()
+    return Int4Weight.from_levels(levels, scales, group)
+
+
+def _check_types(x: torch.Tensor, *weights: Int4Weight) -> None:
+    for w in weights:
+        if not isinstance(w, Int4Weight):
+            raise TypeError(f"expected an Int4Weight (quantize_int4 makes one), got {type(w).__name__}")
+        if w.dtype != x.dtype:
+            raise ValueError(f"activations in {x.dtype} with scales in {w.dtype}: they have to be alike")
+
+
+def _check_call(x: torch.Tensor, tensors, weights) -> None:
+    if not x.is_cuda or any(t.device != x.device for t in (*tensors, *weights)):
+        raise ValueError("4-bit products take tensors of one CUDA device, got "
+                         f"{[str(t.device) for t in (x, *tensors, *weights)]}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *tensors)):
+        raise RuntimeError("products with 4-bit weights have no gradients: call them under "
+                           "torch.no_grad()")
+
+
+@torch.library.custom_op("moe_b200::int4_mm", mutates_args=())
+def _int4_mm(x: torch.Tensor, levels: torch.Tensor, scales: torch.Tensor, group: int,
+             n_dim: int) -> torch.Tensor:
+    with torch.cuda.device(x.device):
+        return K.int4_mm(x, levels, scales, group, n_dim)
+
+
+@_int4_mm.register_fake
+def _(x, levels, scales, group, n_dim):
+    return x.new_empty((x.shape[0], n_dim))
+
+
+def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
+    """x [..., K] times a weight [K, N] held in 4 bits -> [..., N], in x's dtype (that of the scales).
+
+    Made for few rows: up to 64 read the weight once, more read it once per 64. fp32 sums, rounded
+    once; bitwise reproducible."""
+    _check_types(x, weight)
+    if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"int4_mm takes x [..., K] and one matrix [K, N], got {tuple(x.shape)} and "
+                         f"{weight.shape}")
+    _check_call(x, (), (weight,))
+    out = _int4_mm(x.reshape(-1, x.shape[-1]), weight.levels, weight.scales, weight.group,
+                   weight.shape[1])
+    return out.view(*x.shape[:-1], weight.shape[1])
+
+
+@torch.library.custom_op("moe_b200::int4_experts", mutates_args=())
+def _int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, in_levels: torch.Tensor,
+                  in_scales: torch.Tensor, out_levels: torch.Tensor, out_scales: torch.Tensor,
+                  sh_in_levels: Optional[torch.Tensor], sh_in_scales: Optional[torch.Tensor],
+                  sh_out_levels: Optional[torch.Tensor], sh_out_scales: Optional[torch.Tensor],
+                  d_hidden: int, group: int, act: int) -> torch.Tensor:
+    shared = sh_in_levels is not None
+    with torch.cuda.device(x.device):
+        return K.int4_experts(
+            x, topk_w.contiguous(), topk_idx.contiguous(), (in_levels, in_scales),
+            (out_levels, out_scales), (sh_in_levels, sh_in_scales) if shared else None,
+            (sh_out_levels, sh_out_scales) if shared else None, d_hidden, group, act)
+
+
+@_int4_experts.register_fake
+def _(x, topk_w, topk_idx, in_levels, in_scales, out_levels, out_scales, sh_in_levels, sh_in_scales,
+      sh_out_levels, sh_out_scales, d_hidden, group, act):
+    return x.new_empty(x.shape)
+
+
+def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, w_in: Int4Weight,
+                 w_out: Int4Weight, activation: str = "silu", shared_in: Optional[Int4Weight] = None,
+                 shared_out: Optional[Int4Weight] = None) -> torch.Tensor:
+    """out[t] = sum_j topk_w[t, j] * expert topk_idx[t, j] of x[t], plus every shared expert of x[t]; an
+    expert is (act(gate) * up) @ w_out[e] with [gate | up] = x @ w_in[e].
+
+    x         [T, D] bf16 or fp16
+    topk_w    [T, k] in x's dtype, topk_idx [T, k] int64: what TopKRouter returns
+    w_in      Int4Weight [E, D, 2H], w_out [E, H, D], H a multiple of 16, one scale group size for all
+    shared_*  the same for the always-on experts, [S, D, 2H] and [S, H, D]
+
+    No dispatch comes before it and nothing synchronises: made for batches that generate. An id outside
+    [0, E) adds nothing and is reported by `kernels.check_status`. fp32 sums; the GLU's result is held in
+    x's dtype; bitwise reproducible."""
+    shared = () if shared_in is None and shared_out is None else (shared_in, shared_out)
+    weights = (w_in, w_out, *shared)
+    act = _act_id(activation)
+    _check_types(x, *weights)
+    if x.dim() != 2 or topk_idx.dim() != 2 or topk_w.shape != topk_idx.shape or \
+            topk_idx.shape[0] != x.shape[0] or topk_idx.shape[1] < 1:
+        raise ValueError(f"int4_experts takes x [T, D] with topk_w and topk_idx [T, k], got "
+                         f"{tuple(x.shape)}, {tuple(topk_w.shape)} and {tuple(topk_idx.shape)}")
+    if topk_w.dtype != x.dtype or topk_idx.dtype != torch.int64:
+        raise ValueError(f"topk_w has x's dtype and topk_idx is int64, got {topk_w.dtype} and "
+                         f"{topk_idx.dtype}")
+    d = x.shape[1]
+    h = w_out.shape[1] if len(w_out.shape) == 3 else 0
+    for pair in (weights[:2], weights[2:]):
+        if pair and not (len(pair[0].shape) == len(pair[1].shape) == 3
+                         and pair[0].shape == (pair[1].shape[0], d, 2 * h)
+                         and pair[1].shape == (pair[0].shape[0], h, d)):
+            raise ValueError(f"expert weights {pair[0].shape} and {pair[1].shape} do not fit "
+                             f"d_model {d} and d_hidden {h}")
+    if h % 16:
+        raise ValueError(f"experts of width {h}: a multiple of 16 is covered")
+    if len({w.group for w in weights}) > 1:
+        raise ValueError("the experts' weights have scale groups of different sizes")
+    _check_call(x, (topk_w, topk_idx), weights)
+    sh = [v for w in shared for v in (w.levels, w.scales)] or [None] * 4
+    return _int4_experts(x, topk_w, topk_idx, w_in.levels, w_in.scales, w_out.levels, w_out.scales, *sh,
+                         h, w_in.group, act)

@@ -83,7 +83,8 @@ def check_status(device) -> None:
     if code:
         w.zero_()
         what = {1: "a bounded wait inside a GEMM kernel ran out",
-                2: "an expert id outside [0, n_experts) reached the dispatch"}.get(code, "unknown")
+                2: "an expert id outside [0, n_experts) reached the dispatch",
+                3: "the starts of a grouped product's runs decrease or leave its rows"}.get(code, "unknown")
         raise RuntimeError(f"moe_b200 device status {code}: {what}")
 
 
@@ -812,4 +813,118 @@ def ep_pull_vec(v_ptrs, pair_rank, pair_row, n_tokens: int, k_all: int, top_k: i
         _ptr_array(v_ptrs), len(v_ptrs), pair_rank.data_ptr(), pair_row.data_ptr(), n_tokens,
         k_all, top_k, out.data_ptr(), _stream(like)), "moe_b200_ep_pull_vec")
     _count(1 if n_tokens else 0)
+    return out
+
+
+# ------------------------------------------------- ragged grouped products, 4-bit weights, dropout
+# element types of the entry points that take more than bf16 (MOE_B200_BF16, ...)
+DTYPE_IDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _rows8(t: torch.Tensor) -> torch.Tensor:
+    """t [rows, cols] as the kernels read it in place: unit column stride, row starts on 16 bytes;
+    otherwise a contiguous copy."""
+    if (t.stride(1) == 1 and t.stride(0) >= t.shape[1] and t.stride(0) % 8 == 0
+            and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _stack8(w: torch.Tensor):
+    """(w [G, K, N] as the kernels read it in place, 1 where n is its contiguous axis, 0 where k is);
+    any other layout is copied."""
+    if w.data_ptr() % 16 == 0 and (w.shape[0] == 1 or (w.stride(0) > 0 and w.stride(0) % 8 == 0)):
+        for inner, outer in ((2, 1), (1, 2)):
+            if (w.stride(inner) == 1 and w.stride(outer) >= w.shape[inner]
+                    and w.stride(outer) % 8 == 0):
+                return w, int(inner == 2)
+    return w.clone(memory_format=torch.contiguous_format), 1
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """y [R, N]: rows offsets[g] .. offsets[g + 1] of x [R, K] times w[g], w [G, K, N] with either of its
+    inner axes contiguous; rows of no run are zero. bf16 or fp16, K and N multiples of 8."""
+    _need_cuda(x, w, offsets)
+    x, (w, n_inner) = _rows8(x), _stack8(w)
+    g, k, n = w.shape
+    y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
+    # (a stack of one has no stride between matrices to speak of)
+    gstride = w.stride(0) if g > 1 else k * n
+    _lib.check(_lib.load().moe_b200_grouped_mm(
+        x.data_ptr(), x.shape[0], x.stride(0) if x.shape[0] > 1 else k, k, w.data_ptr(), g, gstride,
+        w.stride(1) if n_inner else w.stride(2), n_inner, n, offsets.data_ptr(),
+        DTYPE_IDS.get(x.dtype, -1), y.data_ptr(), status_word(x.device).data_ptr(), _stream(x)),
+        "moe_b200_grouped_mm")
+    _count(1 if x.shape[0] else 0)
+    return y
+
+
+def grouped_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """dw [G, M, N]: the sum over each run's rows of a[r]^T b[r] (a [R, M], b [R, N]); zero without
+    rows."""
+    _need_cuda(a, b, offsets)
+    a, b = _rows8(a), _rows8(b)
+    r, m = a.shape
+    n, g = b.shape[1], offsets.numel() - 1
+    lib = _lib.load()
+    dw = torch.empty((g, m, n), dtype=a.dtype, device=a.device)
+    nbytes = lib.moe_b200_grouped_wgrad_scratch_bytes(m, n, r, g)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+    _lib.check(lib.moe_b200_grouped_wgrad(
+        a.data_ptr(), a.stride(0) if r > 1 else m, m, b.data_ptr(), b.stride(0) if r > 1 else n, n, r,
+        offsets.data_ptr(), g, DTYPE_IDS.get(a.dtype, -1), dw.data_ptr(), _lib.ptr(scratch), nbytes,
+        status_word(a.device).data_ptr(), _stream(a)), "moe_b200_grouped_wgrad")
+    _count((2 if nbytes else 1) if r else 0)
+    return dw
+
+
+def int4_mm(x: torch.Tensor, levels, scales, group: int, n_dim: int) -> torch.Tensor:
+    """x [R, K] times one packed 4-bit matrix -> [R, n_dim]."""
+    _need_cuda(x, levels, scales)
+    x = _rows8(x)
+    r, k = x.shape
+    y = torch.empty((r, n_dim), dtype=x.dtype, device=x.device)
+    _lib.check(_lib.load().moe_b200_int4_mm(
+        x.data_ptr(), r, x.stride(0) if r > 1 else k, k, levels.data_ptr(), scales.data_ptr(), group,
+        n_dim, DTYPE_IDS.get(x.dtype, -1), y.data_ptr(), _stream(x)), "moe_b200_int4_mm")
+    _count(1 if r else 0)
+    return y
+
+
+def int4_experts(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out, d_hidden: int, group: int,
+                 act: int) -> torch.Tensor:
+    """out [T, D] of the block's experts with packed 4-bit weights; each weight a (levels, scales) pair,
+    the shared ones None without shared experts."""
+    _need_cuda(x, topk_w, topk_idx, *w_in, *w_out)
+    x = _rows8(x)
+    t, d = x.shape
+    k, e = topk_idx.shape[1], w_in[0].shape[0]
+    s = 0 if shared_in is None else shared_in[0].shape[0]
+    none = (None, None)
+    lib = _lib.load()
+    out = torch.empty((t, d), dtype=x.dtype, device=x.device)
+    nbytes = lib.moe_b200_int4_experts_scratch_bytes(t, k, s, d, d_hidden)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    ptrs = [_lib.ptr(v) for pair in (shared_in or none, shared_out or none) for v in pair]
+    _lib.check(lib.moe_b200_int4_experts(
+        x.data_ptr(), t, x.stride(0) if t > 1 else d, d, d_hidden, topk_w.data_ptr(),
+        topk_idx.data_ptr(), k, e, w_in[0].data_ptr(), w_in[1].data_ptr(), w_out[0].data_ptr(),
+        w_out[1].data_ptr(), s, *ptrs, group, act, DTYPE_IDS.get(x.dtype, -1), out.data_ptr(),
+        scratch.data_ptr(), nbytes, status_word(x.device).data_ptr(), _stream(x)),
+        "moe_b200_int4_experts")
+    _count(3 if t else 0)
+    return out
+
+
+def dropout(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng: torch.Tensor,
+            used: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """residual + dropout(x) (fresh, contiguous); used (int64 [2]) receives the state it was made with."""
+    _need_cuda(x, residual, rng, used)
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    out = torch.empty_like(x)
+    _lib.check(_lib.load().moe_b200_dropout(
+        x.data_ptr(), _lib.ptr(residual), x.numel(), DTYPE_IDS.get(x.dtype, -1), float(p),
+        rng.data_ptr(), _lib.ptr(used), out.data_ptr(), _stream(x)), "moe_b200_dropout")
+    _count(1 if x.numel() else 0)
     return out

@@ -1,0 +1,306 @@
+"""The ragged grouped products, 4-bit weights and dropout on the host: the schedule arithmetic and the
+generator compiled for the host, the packed layout, and what is refused before anything is launched."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+CSRC = os.path.join(ROOT, "nanospeaker_b200", "csrc")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from nanospeaker_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """The CUDA-free headers as a host library."""
+    d = tmp_path_factory.mktemp("host")
+    src = d / "host.cpp"
+    src.write_text('''
+#include "grouped_order.cuh"
+#include "philox.cuh"
+extern "C" {
+void tile(int l, int m, int n, int band, int* out) {
+  const moe::TileAt t = moe::tile_in_bands(l, m, n, band);
+  out[0] = t.m; out[1] = t.n;
+}
+int chunks(int rows, int ks) { return moe::run_chunks(rows, ks); }
+long long chunk_rows(long long rows, long long tiles, int ctas) { return moe::grouped_chunk_rows(rows, tiles, ctas); }
+void philox(unsigned long long low, unsigned long long high, unsigned long long key, unsigned* w) {
+  moe::philox4x32(low, high, key, w);
+}
+unsigned threshold(double p) { return moe::dropout_threshold(p); }
+}
+''')
+    so = d / "host.so"
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-std=c++17", f"-I{CSRC}", str(src), "-o", str(so)],
+                   check=True)
+    lib = ctypes.CDLL(str(so))
+    lib.chunk_rows.restype = ctypes.c_longlong
+    lib.chunk_rows.argtypes = [ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int]
+    lib.philox.argtypes = [ctypes.c_ulonglong] * 3 + [ctypes.c_void_p]
+    lib.threshold.restype = ctypes.c_uint
+    lib.threshold.argtypes = [ctypes.c_double]
+    return lib
+
+
+# ------------------------------------------------------------------------------------ schedules
+@pytest.mark.parametrize("m,n,band", [(1, 1, 8), (8, 3, 8), (9, 5, 8), (128, 16, 8), (3, 64, 8), (7, 1, 4)])
+def test_every_tile_is_walked_once_and_bands_stay_together(host, m, n, band):
+    at = (ctypes.c_int * 2)()
+    seen = []
+    for l in range(m * n):
+        host.tile(l, m, n, band, at)
+        seen.append((at[0], at[1]))
+    assert sorted(seen) == [(i, j) for i in range(m) for j in range(n)]
+    bands = [i // band for i, _ in seen]
+    assert bands == sorted(bands)
+
+
+@pytest.mark.parametrize("rows,ks,want", [(0, 512, 1), (1, 512, 1), (512, 512, 1), (513, 512, 2),
+                                          (1025, 512, 3)])
+def test_chunks_of_a_run(host, rows, ks, want):
+    assert host.chunks(rows, ks) == want
+
+
+def test_chunk_rows_are_a_share_of_the_work(host):
+    for rows, tiles in ((1, 1), (98304, 5), (32768, 256), (1 << 20, 1)):
+        ks = host.chunk_rows(rows, tiles, 148)
+        assert ks % 64 == 0 and ks >= 512
+        assert ks == 512 or (ks - 64) * 148 * 3 < rows * tiles <= ks * 148 * 3
+
+
+def test_scratch_covers_every_split_run(lib, host):
+    """Whatever the runs are, the chunks of split runs fit the scratch."""
+    rng = torch.Generator().manual_seed(0)
+    for rows, m, n, groups in ((98304, 576, 256, 76), (5000, 64, 64, 3), (20000, 8, 8, 1000)):
+        tiles = -(-m // 128) * -(-n // (256 if n > 128 else 128))
+        ks = host.chunk_rows(rows, tiles, 148)
+        have = lib.moe_b200_grouped_wgrad_scratch_bytes(m, n, rows, groups) // (m * n * 4)
+        for skew in (0.0, 1.0, 20.0):
+            load = torch.softmax(torch.randn(groups, generator=rng) * skew, 0)
+            counts = torch.bincount(torch.multinomial(load, rows, True, generator=rng), minlength=groups)
+            need = sum(host.chunks(int(c), ks) for c in counts if c > ks)
+            assert need <= have
+
+
+# ------------------------------------------------------------------------------------ generator
+# The published known answers of Philox4x32-10 (counter words, key words, output words).
+PHILOX_ANSWERS = [
+    ([0, 0, 0, 0], [0, 0], [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]),
+    ([0xffffffff] * 4, [0xffffffff] * 2, [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]),
+    ([0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344], [0xa4093822, 0x299f31d0],
+     [0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1]),
+]
+
+
+@pytest.mark.parametrize("counter,key,want", PHILOX_ANSWERS)
+def test_philox_known_answers(host, counter, key, want):
+    w = (ctypes.c_uint * 4)()
+    host.philox(counter[0] | counter[1] << 32, counter[2] | counter[3] << 32, key[0] | key[1] << 32, w)
+    assert list(w) == want
+
+
+def test_thresholds(host):
+    for p in (0.0, 0.1, 0.25, 0.5, 1 / 3, 0.9, 2.0 ** -33, 3 * 2.0 ** -33, 1 - 2.0 ** -40):
+        assert host.threshold(p) == min(round(p * 2 ** 32), 2 ** 32 - 1)
+
+
+# --------------------------------------------------------------------------------- 4-bit weights
+@pytest.mark.parametrize("shape,group", [((8, 1), 32), ((64, 16), 64), ((1000, 1537), 32), ((576, 256), 64),
+                                         ((3, 128, 40), 64), ((2, 72, 16), 128), ((1, 200, 33), 192)])
+def test_packing_returns_what_was_packed(shape, group):
+    from nanospeaker_b200 import Int4Weight
+    levels = torch.randint(0, 16, shape, dtype=torch.uint8)
+    k, n = shape[-2:]
+    scales = torch.rand(*shape[:-2], -(-k // group), n).bfloat16()
+    w = Int4Weight.from_levels(levels, scales, group)
+    back, s = w.to_levels()
+    assert torch.equal(back, levels) and torch.equal(s, scales)
+    assert w.levels.dtype == torch.int32 and w.levels.is_contiguous() and w.scales.is_contiguous()
+    assert w.shape == shape and w.dtype == torch.bfloat16
+
+
+def test_packed_layout_is_the_documented_one():
+    """Nibble i of half b of word j of lane 4 * row + t, written out level by level."""
+    from nanospeaker_b200 import Int4Weight
+    levels = torch.randint(0, 16, (128, 32), dtype=torch.uint8)
+    w = Int4Weight.from_levels(levels, torch.ones(2, 32).half(), 64)
+    words = w.levels[0].to(torch.int64) & 0xFFFFFFFF
+    for strip in range(2):
+        for kb in range(2):
+            for lane in range(32):
+                row, t = lane // 4, lane % 4
+                for j in range(4):
+                    for i in range(4):
+                        for b in range(2):
+                            k = 64 * kb + 32 * (j // 2) + 8 * t + 4 * (j % 2) + 2 * (i // 2) + b
+                            n = 16 * strip + row + 8 * (i % 2)
+                            got = (int(words[strip, kb, lane, j]) >> (4 * i + 16 * b)) & 15
+                            assert got == int(levels[k, n])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantisation_is_within_half_a_level(dtype, group):
+    """scale = largest / 7 rounded to 16 bits (relative 2^-8 at most): a level is at most half a scale
+    off, and the largest value, at 7 scales, at most 7 * 2^-8 of a scale more."""
+    from nanospeaker_b200 import quantize_int4
+    w = (torch.randn(2, 200, 48) * 0.1).to(dtype)
+    q = quantize_int4(w, group)
+    assert q.dtype == (torch.bfloat16 if dtype == torch.float32 else dtype)
+    _, scales = q.to_levels()
+    each = scales.float().repeat_interleave(group, 1)[:, :200]
+    assert ((q.dequantize() - w.float()).abs() <= each * (0.5 + 7 * 2.0 ** -8) * (1 + 1e-6)).all()
+
+
+def test_quantising_zeros_and_what_is_not_finite():
+    from nanospeaker_b200 import quantize_int4
+    assert (quantize_int4(torch.zeros(64, 16)).dequantize() == 0).all()
+    for bad in (float("inf"), float("nan")):
+        w = torch.zeros(64, 16)
+        w[3, 5] = bad
+        with pytest.raises(ValueError, match="infinities or NaN"):
+            quantize_int4(w)
+
+
+def test_weight_refusals():
+    from nanospeaker_b200 import Int4Weight, quantize_int4
+    q, s = torch.zeros(64, 16, dtype=torch.uint8), torch.ones(1, 16).half()
+    for group in (0, 16, 33, 96):
+        with pytest.raises(ValueError, match="scale groups"):
+            Int4Weight.from_levels(q, s, group)
+    with pytest.raises(ValueError, match="uint8"):
+        Int4Weight.from_levels(q.int(), s, 64)
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        Int4Weight.from_levels(q, s.float(), 64)
+    with pytest.raises(ValueError, match="do not take scales"):
+        Int4Weight.from_levels(q, s, 32)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        quantize_int4(torch.randn(60, 16))
+    with pytest.raises(ValueError, match=r"\[K, N\]"):
+        quantize_int4(torch.randn(60))
+
+
+# ------------------------------------------------------------------------------------- refusals
+def test_grouped_refusals():
+    from nanospeaker_b200 import grouped_mm
+    x, w = torch.randn(6, 16).bfloat16(), torch.randn(2, 16, 24).bfloat16()
+    off = torch.tensor([0, 2, 6], dtype=torch.int32)
+    bad = lambda msg, *a: _refused(grouped_mm, msg, *a)  # noqa: E731
+    bad("takes x", x[0], w, off)
+    bad("takes x", x, w[0], off)
+    bad("fit together", x, w, off[:2])
+    bad("fit together", x[:, :8], w, off)
+    bad("bf16 or fp16", x.float(), w.float(), off)
+    bad("bf16 or fp16", x, w.half(), off)
+    bad("int32", x, w, off.long())
+    bad("multiples of 8", x, w[:, :, :20], off)
+    bad("multiples of 8", torch.randn(6, 12).bfloat16(), torch.randn(2, 12, 16).bfloat16(), off)
+    bad("groups", torch.randn(1, 8).half(), torch.randn(1025, 8, 8).half(),
+        torch.zeros(1026, dtype=torch.int32))
+    bad("CUDA device", x, w, off)
+
+
+def _refused(fn, msg, *a, **kw):
+    with pytest.raises(ValueError, match=msg):
+        fn(*a, **kw)
+
+
+def test_int4_refusals():
+    from nanospeaker_b200 import int4_experts, int4_mm, quantize_int4
+    x = torch.randn(3, 64).half()
+    w = quantize_int4(torch.randn(64, 32).half())
+    with pytest.raises(TypeError):
+        int4_experts(x, x[:, :1], torch.zeros(3, 1, dtype=torch.int64), w, torch.zeros(3))
+    _refused(int4_mm, "one matrix", x, quantize_int4(torch.randn(2, 64, 32).half()))
+    _refused(int4_mm, "one matrix", x[:, :32], w)
+    _refused(int4_mm, "have to be alike", x.bfloat16(), w)
+    _refused(int4_mm, "CUDA device", x, w)
+    w_in, w_out = quantize_int4(torch.randn(4, 64, 64).half()), quantize_int4(torch.randn(4, 32, 64).half())
+    tw, idx = torch.ones(3, 2).half(), torch.zeros(3, 2, dtype=torch.int64)
+    _refused(int4_experts, "no kernel", x, tw, idx, w_in, w_out, activation="cube")
+    _refused(int4_experts, "takes x", x, tw, idx[:2], w_in, w_out)
+    _refused(int4_experts, "int64", x, tw, idx.int(), w_in, w_out)
+    _refused(int4_experts, "int64", x, tw.float(), idx, w_in, w_out)
+    _refused(int4_experts, "do not fit", x, tw, idx, w_out, w_in)
+    _refused(int4_experts, "do not fit", x[:, :32].contiguous(), tw, idx, w_in, w_out)
+    _refused(int4_experts, "do not fit", x, tw, idx, w_in, w_out, shared_in=w_out, shared_out=w_out)
+    _refused(int4_experts, "multiple of 16", x, tw, idx, quantize_int4(torch.randn(4, 64, 48).half()),
+             quantize_int4(torch.randn(4, 24, 64).half()))
+    _refused(int4_experts, "different sizes", x, tw, idx, w_in, quantize_int4(torch.randn(4, 32, 64).half(), 32))
+    _refused(int4_experts, "CUDA device", x, tw, idx, w_in, w_out)
+    with pytest.raises(TypeError):
+        int4_experts(x, tw, idx, w_in, w_out, shared_in=w_in)
+
+
+def test_dropout_refusals():
+    from nanospeaker_b200 import dropout_add
+    x, rng = torch.randn(4, 4), torch.zeros(2, dtype=torch.int64)
+    _refused(dropout_add, "fp32", x.double(), None, 0.1, rng)
+    _refused(dropout_add, "residual", x, x[:2], 0.1, rng)
+    _refused(dropout_add, "residual", x, x.half(), 0.1, rng)
+    for p in (-0.1, 1.0, 1.5, float("nan")):
+        _refused(dropout_add, "has to be in", x, None, p, rng)
+    _refused(dropout_add, "int64", x, None, 0.1, rng.int())
+    _refused(dropout_add, "int64", x, None, 0.1, torch.zeros(3, dtype=torch.int64))
+    _refused(dropout_add, "CUDA device", x, None, 0.1, rng)
+
+
+def test_entry_points_validate_before_any_launch(lib):
+    """Bad shapes, types, pointers and scratch come back as error codes (no GPU needed)."""
+    buf = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 63) & ~63)
+    odd = ctypes.c_void_p(p.value + 2)
+    null = ctypes.c_void_p(0)
+    mm = lambda x=p, rows=4, ld=64, k=64, w=p, g=2, gs=64 * 32, ldw=32, n=32, off=p, dt=0, y=p, st=p: \
+        lib.moe_b200_grouped_mm(x, rows, ld, k, w, g, gs, ldw, 1, n, off, dt, y, st, null)  # noqa: E731
+    assert mm(rows=0) == 0
+    assert mm(rows=-1) == mm(k=60) == mm(n=30) == mm(g=0) == mm(g=1025) == mm(ld=63) == mm(ld=56) == -1
+    assert mm(ldw=24) == mm(gs=33) == mm(rows=1 << 31) == -1
+    assert mm(dt=2) == mm(dt=-1) == -5
+    assert mm(x=null) == mm(w=null) == mm(off=null) == mm(y=null) == mm(st=null) == -2
+    assert mm(x=odd) == mm(w=odd) == mm(y=odd) == mm(off=odd) == -3
+    wg = lambda a=p, lda=64, m=64, b=p, ldb=32, n=32, rows=4, off=p, g=2, dt=0, dw=p, sc=null, nb=0, st=p: \
+        lib.moe_b200_grouped_wgrad(a, lda, m, b, ldb, n, rows, off, g, dt, dw, sc, nb, st, null)  # noqa: E731
+    assert wg(rows=-1) == wg(m=60) == wg(n=4) == wg(g=0) == wg(lda=56) == wg(ldb=28) == -1
+    assert wg(dt=2) == -5
+    assert wg(a=null) == wg(b=null) == wg(off=null) == wg(dw=null) == wg(st=null) == -2
+    assert wg(a=odd) == wg(b=odd) == wg(dw=odd) == -3
+    need = lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 100000, 2)
+    assert need > 0 and lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 512, 2) == 0
+    assert wg(rows=100000) == wg(rows=100000, sc=p, nb=need - 1) == -4
+    q = lambda x=p, rows=4, ld=64, k=64, lv=p, sc=p, grp=64, n=32, dt=0, y=p: \
+        lib.moe_b200_int4_mm(x, rows, ld, k, lv, sc, grp, n, dt, y, null)  # noqa: E731
+    assert q(rows=0) == 0
+    assert q(rows=-1) == q(k=60) == q(n=0) == q(ld=56) == q(grp=16) == q(grp=96) == -1
+    assert q(dt=2) == -5
+    assert q(x=null) == q(lv=null) == q(sc=null) == q(y=null) == -2
+    assert q(x=odd) == q(lv=odd) == q(sc=odd) == -3
+    ex = lambda t=4, d=64, h=32, k=2, e=4, s=0, w=p, idx=p, grp=64, act=0, dt=0, sc=p, nb=1 << 20, sh=null, o=p: \
+        lib.moe_b200_int4_experts(p, t, d, d, h, w, idx, k, e, p, p, p, p, s, sh, sh, sh, sh, grp, act,
+                                  dt, o, sc, nb, p, null)  # noqa: E731
+    assert ex(t=0) == 0
+    assert ex(t=-1) == ex(d=60) == ex(h=24) == ex(k=0) == ex(e=0) == ex(s=-1) == ex(grp=48) == -1
+    assert ex(e=65536) == ex(t=1 << 30) == -1
+    assert ex(dt=2) == ex(act=5) == ex(act=-1) == -5
+    assert ex(w=null) == ex(idx=null) == ex(o=null) == ex(s=1) == -2
+    assert ex(o=odd) == ex(idx=odd) == -3
+    bytes_ = lib.moe_b200_int4_experts_scratch_bytes(4, 2, 1, 64, 32)
+    assert bytes_ >= 12 * (32 * 2 + 64 * 4)
+    assert ex(s=1, sh=p, nb=bytes_ - 1) == ex(sc=null) == -4
+    dr = lambda x=p, r=null, n=8, dt=0, pr=0.1, rng=p, used=null, o=p: \
+        lib.moe_b200_dropout(x, r, n, dt, pr, rng, used, o, null)  # noqa: E731
+    assert dr(n=0) == 0
+    assert dr(n=-1) == dr(pr=1.0) == dr(pr=-0.5) == dr(pr=float("nan")) == -1
+    assert dr(dt=3) == -5
+    assert dr(x=null) == dr(rng=null) == dr(o=null) == -2
+    assert dr(rng=odd) == dr(used=odd) == dr(x=odd, dt=2) == -3
