@@ -47,6 +47,13 @@ struct Abi {
   decltype(&moe_b200_muon_step) muon_step;
   decltype(&moe_b200_rmsnorm) rmsnorm;
   decltype(&moe_b200_rmsnorm_bwd) rmsnorm_bwd;
+  decltype(&moe_b200_grouped_mm) grouped_mm;
+  decltype(&moe_b200_grouped_wgrad_scratch_bytes) grouped_wgrad_scratch_bytes;
+  decltype(&moe_b200_grouped_wgrad) grouped_wgrad;
+  decltype(&moe_b200_int4_mm) int4_mm;
+  decltype(&moe_b200_int4_experts_scratch_bytes) int4_experts_scratch_bytes;
+  decltype(&moe_b200_int4_experts) int4_experts;
+  decltype(&moe_b200_dropout) dropout;
 } abi{};
 
 py::object* status_word_of = nullptr;   // device index -> address of its status word
@@ -67,6 +74,13 @@ void bind(const py::dict& d, const py::object& status) {
   take(d, "moe_b200_muon_step", abi.muon_step);
   take(d, "moe_b200_rmsnorm", abi.rmsnorm);
   take(d, "moe_b200_rmsnorm_bwd", abi.rmsnorm_bwd);
+  take(d, "moe_b200_grouped_mm", abi.grouped_mm);
+  take(d, "moe_b200_grouped_wgrad_scratch_bytes", abi.grouped_wgrad_scratch_bytes);
+  take(d, "moe_b200_grouped_wgrad", abi.grouped_wgrad);
+  take(d, "moe_b200_int4_mm", abi.int4_mm);
+  take(d, "moe_b200_int4_experts_scratch_bytes", abi.int4_experts_scratch_bytes);
+  take(d, "moe_b200_int4_experts", abi.int4_experts);
+  take(d, "moe_b200_dropout", abi.dropout);
   status_word_of = new py::object(status);   // lives as long as the process
 }
 
@@ -333,12 +347,12 @@ Tensor as_grad_aux(const Tensor& g) {
 
 // What a backward returns. It is made without grad mode, so that under create_graph the gradients would
 // pass for constants; differentiating them again is an error.
-variable_list once(variable_list grads) {
+variable_list once(variable_list grads, const char* whose = "the MoE block's") {
   if (!at::GradMode::is_enabled()) return grads;
   for (Tensor& g : grads)
     if (g.defined()) g = g.detach().set_requires_grad(true);
   auto error = std::make_shared<torch::autograd::DelayedError>(
-      "the MoE block's backward cannot be differentiated again", int64_t(grads.size()));
+      std::string(whose) + " backward cannot be differentiated again", int64_t(grads.size()));
   return (*error)(std::move(grads));
 }
 
@@ -760,6 +774,253 @@ Tensor muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& g
   return norms.narrow(0, 0, 2);
 }
 
+// -------------------------------------------- ragged grouped products, 4-bit weights, dropout
+// The eager calls of grouped.py, int4.py and dropout.py. A call that is not as documented gives no result
+// here; the Python side then says what is wrong with it.
+int dtype_id(at::ScalarType t) {
+  return t == at::kBFloat16 ? MOE_B200_BF16 : t == at::kHalf ? MOE_B200_FP16
+         : t == at::kFloat  ? MOE_B200_FP32 : -1;
+}
+bool half16(const Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
+}
+bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+void* current_stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+
+// t [rows, cols] as the kernels read it in place, otherwise a contiguous copy.
+Tensor rows8(const Tensor& t) {
+  const int64_t ld = t.stride(0);
+  if (t.stride(1) == 1 && ld >= t.size(1) && ld % 8 == 0 && on16(t)) return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// w [G, K, N] as the kernels read it in place (n_inner: n is its contiguous axis, else k is); any other
+// layout is copied.
+struct Stack8 {
+  Tensor w;
+  bool n_inner;
+  explicit Stack8(const Tensor& t) : w(t), n_inner(true) {
+    if (on16(t) && (t.size(0) == 1 || (t.stride(0) > 0 && t.stride(0) % 8 == 0)))
+      for (const int inner : {2, 1}) {
+        const int outer = 3 - inner;
+        if (t.stride(inner) == 1 && t.stride(outer) >= t.size(inner) && t.stride(outer) % 8 == 0) {
+          n_inner = inner == 2;
+          return;
+        }
+      }
+    w = t.clone(at::MemoryFormat::Contiguous);
+  }
+};
+
+Tensor launch_grouped(const Tensor& x_in, const Tensor& w_in, const Tensor& offsets) {
+  const Tensor x = rows8(x_in);
+  const Stack8 s(w_in);
+  const int64_t r = x.size(0), k = x.size(1), g = s.w.size(0), n = s.w.size(2);
+  const Tensor y = at::empty({r, n}, x.options());
+  check(abi.grouped_mm(x.const_data_ptr(), r, row_stride(x), int32_t(k), s.w.const_data_ptr(), int32_t(g),
+                       g > 1 ? s.w.stride(0) : k * n, s.w.stride(s.n_inner ? 1 : 2), s.n_inner, int32_t(n),
+                       offsets.const_data_ptr<int32_t>(), dtype_id(x.scalar_type()), y.mutable_data_ptr(),
+                       status_word(x.get_device()), current_stream()),
+        "moe_b200_grouped_mm");
+  n_launched += r > 0;
+  return y;
+}
+Tensor launch_grouped_wgrad(const Tensor& a_in, const Tensor& b_in, const Tensor& offsets) {
+  const Tensor a = rows8(a_in), b = rows8(b_in);
+  const int64_t r = a.size(0), m = a.size(1), n = b.size(1), g = offsets.numel() - 1;
+  const Tensor dw = at::empty({g, m, n}, a.options());
+  const size_t bytes = abi.grouped_wgrad_scratch_bytes(int32_t(m), int32_t(n), r, int32_t(g));
+  const Tensor scratch = bytes ? bytes_like(a, bytes) : Tensor();
+  check(abi.grouped_wgrad(a.const_data_ptr(), row_stride(a), int32_t(m), b.const_data_ptr(), row_stride(b),
+                          int32_t(n), r, offsets.const_data_ptr<int32_t>(), int32_t(g),
+                          dtype_id(a.scalar_type()), dw.mutable_data_ptr(),
+                          bytes ? scratch.mutable_data_ptr() : nullptr, bytes, status_word(a.get_device()),
+                          current_stream()),
+        "moe_b200_grouped_wgrad");
+  n_launched += r > 0 ? (bytes ? 2 : 1) : 0;
+  return dw;
+}
+
+// Edges: x, w.
+struct GroupedMMBackward : public torch::autograd::Node {
+  SavedVariable x, w, offsets;
+  std::string name() const override { return "GroupedMMBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&x, &w, &offsets}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(2);
+    const Tensor xx = x.unpack(), ww = w.unpack(), off = offsets.unpack();
+    Tensor dx, dw;
+    {
+      at::NoGradGuard no_grad;
+      const c10::cuda::CUDAGuard on(xx.device());
+      const Tensor dy = grads[0].to(xx.scalar_type());
+      if (task_should_compute_output(0)) dx = launch_grouped(dy, ww.transpose(1, 2), off);
+      if (task_should_compute_output(1))   // (lies as w does)
+        dw = ww.stride(1) == 1 && ww.stride(2) != 1 ? launch_grouped_wgrad(dy, xx, off).transpose(1, 2)
+                                                    : launch_grouped_wgrad(xx, dy, off);
+    }
+    return once({dx, dw}, "grouped_mm's");
+  }
+};
+
+OptTensor grouped_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t max_groups) {
+  if (x.dim() != 2 || w.dim() != 3 || offsets.dim() != 1 || x.size(1) != w.size(1) ||
+      offsets.numel() != w.size(0) + 1 || !half16(x) || w.scalar_type() != x.scalar_type() ||
+      offsets.scalar_type() != at::kInt || w.size(1) < 8 || w.size(2) < 8 || w.size(1) % 8 || w.size(2) % 8 ||
+      w.size(0) < 1 || w.size(0) > max_groups || !x.is_cuda() || w.device() != x.device() ||
+      offsets.device() != x.device())
+    return {};
+  std::shared_ptr<GroupedMMBackward> node;
+  if (any_grad(x, w)) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined() && !w._fw_grad(0).defined(),
+                                "grouped_mm does not support forward mode AD");
+    node = new_node<GroupedMMBackward>();
+    node->set_next_edges(torch::autograd::collect_next_edges(x, w));
+  }
+  Tensor y, off;
+  {
+    at::NoGradGuard no_grad;
+    const c10::cuda::CUDAGuard on(x.device());
+    off = offsets.contiguous();
+    y = launch_grouped(x, w, off);
+  }
+  if (node) {
+    node->x = SavedVariable(x, false);
+    node->w = SavedVariable(w, false);
+    node->offsets = SavedVariable(off, false);
+    torch::autograd::set_history(y, node);
+  }
+  return y;
+}
+
+bool packed_as(const Tensor& levels, const Tensor& scales, const Tensor& x) {
+  return levels.device() == x.device() && scales.device() == x.device() &&
+         scales.scalar_type() == x.scalar_type();
+}
+
+OptTensor int4_mm(const Tensor& x, const Tensor& levels, const Tensor& scales,
+                  const std::vector<int64_t>& shape, int64_t group) {
+  if (shape.size() != 2 || x.dim() < 1 || x.size(-1) != shape[0] || !x.is_cuda() || !half16(x) ||
+      !packed_as(levels, scales, x) || any_grad(x))
+    return {};
+  at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard on(x.device());
+  const Tensor flat = rows8(x.dim() == 2 ? x : x.reshape({-1, shape[0]}));
+  const Tensor y = at::empty({flat.size(0), shape[1]}, x.options());
+  check(abi.int4_mm(flat.const_data_ptr(), flat.size(0), row_stride(flat), int32_t(shape[0]),
+                    levels.const_data_ptr(), scales.const_data_ptr(), int32_t(group), int32_t(shape[1]),
+                    dtype_id(x.scalar_type()), y.mutable_data_ptr(), current_stream()),
+        "moe_b200_int4_mm");
+  n_launched += flat.size(0) > 0;
+  if (x.dim() == 2) return y;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = shape[1];
+  return y.view(sizes);
+}
+
+// The weights come checked against one another.
+OptTensor int4_experts(const Tensor& x_in, const Tensor& topk_w, const Tensor& topk_idx,
+                       const Tensor& in_levels, const Tensor& in_scales, const Tensor& out_levels,
+                       const Tensor& out_scales, const OptTensor& sh_in_levels, const OptTensor& sh_in_scales,
+                       const OptTensor& sh_out_levels, const OptTensor& sh_out_scales, int64_t d_model,
+                       int64_t d_hidden, int64_t group, int64_t act) {
+  const bool shared = sh_in_levels.has_value();
+  if (x_in.dim() != 2 || topk_idx.dim() != 2 || topk_w.sizes() != topk_idx.sizes() ||
+      topk_idx.size(0) != x_in.size(0) || topk_idx.size(1) < 1 || !x_in.is_cuda() || !half16(x_in) ||
+      x_in.size(1) != d_model || topk_w.scalar_type() != x_in.scalar_type() ||
+      topk_idx.scalar_type() != at::kLong || topk_w.device() != x_in.device() ||
+      topk_idx.device() != x_in.device() || !packed_as(in_levels, in_scales, x_in) ||
+      !packed_as(out_levels, out_scales, x_in) ||
+      (shared && (!packed_as(*sh_in_levels, *sh_in_scales, x_in) ||
+                  !packed_as(*sh_out_levels, *sh_out_scales, x_in))) ||
+      any_grad(x_in, topk_w))
+    return {};
+  at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard on(x_in.device());
+  const Tensor x = rows8(x_in), w = topk_w.contiguous(), idx = topk_idx.contiguous();
+  const int64_t t = x.size(0), k = idx.size(1), s = shared ? sh_in_levels->size(0) : 0;
+  const Tensor out = at::empty({t, d_model}, x.options());
+  const size_t bytes = abi.int4_experts_scratch_bytes(t, int32_t(k), int32_t(s), int32_t(d_model),
+                                                      int32_t(d_hidden));
+  const Tensor scratch = bytes_like(x, bytes);
+  auto of = [](const OptTensor& v) { return v ? v->const_data_ptr() : nullptr; };
+  check(abi.int4_experts(x.const_data_ptr(), t, row_stride(x), int32_t(d_model), int32_t(d_hidden),
+                         w.const_data_ptr(), idx.const_data_ptr<int64_t>(), int32_t(k),
+                         int32_t(in_levels.size(0)), in_levels.const_data_ptr(), in_scales.const_data_ptr(),
+                         out_levels.const_data_ptr(), out_scales.const_data_ptr(), int32_t(s),
+                         of(sh_in_levels), of(sh_in_scales), of(sh_out_levels), of(sh_out_scales),
+                         int32_t(group), int32_t(act), dtype_id(x.scalar_type()), out.mutable_data_ptr(),
+                         scratch.mutable_data_ptr(), bytes, status_word(x.get_device()), current_stream()),
+        "moe_b200_int4_experts");
+  n_launched += t > 0 ? 3 : 0;
+  return out;
+}
+
+Tensor dropout_call(const Tensor& x, const Tensor& residual, double p, const Tensor& rng, bool keep_state);
+
+// Edges: x, residual.
+struct DropoutAddBackward : public torch::autograd::Node {
+  SavedVariable state;   // what the forward's mask was made with
+  double p = 0.0;
+  std::string name() const override { return "DropoutAddBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    state.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return variable_list(2);
+    // (linear: under create_graph the gradient of this is the same mask again)
+    Tensor dx;
+    if (task_should_compute_output(0)) dx = dropout_call(grads[0], Tensor(), p, state.unpack(), false);
+    return {dx, task_should_compute_output(1) ? grads[0] : Tensor()};
+  }
+};
+
+// keep_state: rng may change before the backward, which gets a copy that the kernel makes.
+Tensor dropout_call(const Tensor& x_in, const Tensor& res_in, double p, const Tensor& rng, bool keep_state) {
+  std::shared_ptr<DropoutAddBackward> node;
+  if (any_grad(x_in, res_in)) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!x_in._fw_grad(0).defined() && !(res_in.defined() && res_in._fw_grad(0).defined()),
+                                "dropout_add does not support forward mode AD");
+    node = new_node<DropoutAddBackward>();
+    node->set_next_edges(torch::autograd::collect_next_edges(x_in, res_in));
+  }
+  Tensor out, used;
+  {
+    at::NoGradGuard no_grad;
+    const c10::cuda::CUDAGuard on(x_in.device());
+    const Tensor x = x_in.contiguous(), res = res_in.defined() ? res_in.contiguous() : Tensor();
+    out = at::empty(x.sizes(), x.options());
+    if (node && keep_state) used = at::empty_like(rng);
+    check(abi.dropout(x.const_data_ptr(), ptr(res), x.numel(), dtype_id(x.scalar_type()), p,
+                      rng.const_data_ptr<int64_t>(), used.defined() ? used.mutable_data_ptr<int64_t>() : nullptr,
+                      out.mutable_data_ptr(), current_stream()),
+          "moe_b200_dropout");
+    n_launched += x.numel() > 0;
+  }
+  if (node) {
+    node->p = p;
+    node->state = SavedVariable(used.defined() ? used : rng, false);
+    torch::autograd::set_history(out, node);
+  }
+  return out;
+}
+
+OptTensor dropout_add(const Tensor& x, const OptTensor& residual, double p, const Tensor& rng) {
+  if (!x.is_cuda() || dtype_id(x.scalar_type()) < 0 || !(p >= 0.0 && p < 1.0) || rng.device() != x.device() ||
+      rng.scalar_type() != at::kLong || rng.dim() != 1 || rng.size(0) != 2 || rng.stride(0) != 1 ||
+      (residual && (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type() ||
+                    residual->device() != x.device())))
+    return {};
+  return dropout_call(x, residual.value_or(Tensor()), p, rng, true);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_moe_shim, m) {
@@ -768,6 +1029,10 @@ PYBIND11_MODULE(_moe_shim, m) {
   m.def("block", &block);
   m.def("sublayer", &sublayer);
   m.def("muon_step", &muon_step);
+  m.def("grouped_mm", &grouped_mm);
+  m.def("int4_mm", &int4_mm);
+  m.def("int4_experts", &int4_experts);
+  m.def("dropout_add", &dropout_add);
   py::class_<GraphedBlock, std::shared_ptr<GraphedBlock>>(m, "GraphedBlock")
       .def(py::init<const Tensor&, const Tensor&, const OptTensor&, const Tensor&, const Tensor&,
                     const OptTensor&, const OptTensor&, int64_t, bool, bool, double, int64_t, bool,

@@ -12,6 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import kernels as K
+from .moe_kernel import native_ok
 
 DROPOUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -78,6 +79,10 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float,
     rng       int64 [2] on x's device: (seed, call)
 
     A dropped element adds nothing even where it is infinite or NaN."""
+    if native_ok(x):
+        out = K.shim().dropout_add(x, residual, p, rng)
+        if out is not None:
+            return out
     if x.dtype not in DROPOUT_DTYPES:
         raise ValueError(f"dropout computes in bf16, fp16 or fp32, got {x.dtype}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):

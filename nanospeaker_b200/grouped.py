@@ -10,6 +10,7 @@ csrc/grouped.cu.
 import torch
 
 from . import kernels as K
+from .moe_kernel import native_ok
 
 MAX_GROUPS = 1024
 GROUPED_DTYPES = (torch.bfloat16, torch.float16)
@@ -90,7 +91,11 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch
 
     Returns [R, N]. Rows of no run (before offsets[0], from offsets[G] on) give zeros and take zero
     gradients. Offsets that decrease or leave [0, R] are taken into range and reported by
-    `kernels.check_status`. Sums are fp32, rounded once; both directions are bitwise reproducible. A
-    gradient cannot be differentiated again with respect to w's gradient."""
+    `kernels.check_status`. Sums are fp32, rounded once; both directions are bitwise reproducible. The
+    gradients cannot be differentiated again."""
+    if native_ok(x):
+        y = K.shim().grouped_mm(x, w, offsets, MAX_GROUPS)
+        if y is not None:
+            return y
     _check(x, w, offsets)
     return _grouped_mm(x, w, offsets)

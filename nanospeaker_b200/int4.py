@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import kernels as K
-from .moe_kernel import _act_id
+from .moe_kernel import _act_id, native_ok
 
 INT4_DTYPES = (torch.bfloat16, torch.float16)
 
@@ -156,6 +156,10 @@ def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
 
     Made for few rows: up to 64 read the weight once, more read it once per 64. fp32 sums, rounded
     once; bitwise reproducible."""
+    if type(weight) is Int4Weight and native_ok(x):
+        out = K.shim().int4_mm(x, weight.levels, weight.scales, weight.shape, weight.group)
+        if out is not None:
+            return out
     _check_types(x, weight)
     if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
         raise ValueError(f"int4_mm takes x [..., K] and one matrix [K, N], got {tuple(x.shape)} and "
@@ -200,9 +204,15 @@ def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, 
     No dispatch comes before it and nothing synchronises: made for batches that generate. An id outside
     [0, E) adds nothing and is reported by `kernels.check_status`. fp32 sums; the GLU's result is held in
     x's dtype; bitwise reproducible."""
+    act = _act_id(activation)
+    if native_ok(x):
+        plain = _experts_fit(w_in, w_out, shared_in, shared_out)
+        if plain is not None:
+            out = K.shim().int4_experts(x, topk_w, topk_idx, *plain, act)
+            if out is not None:
+                return out
     shared = () if shared_in is None and shared_out is None else (shared_in, shared_out)
     weights = (w_in, w_out, *shared)
-    act = _act_id(activation)
     _check_types(x, *weights)
     if x.dim() != 2 or topk_idx.dim() != 2 or topk_w.shape != topk_idx.shape or \
             topk_idx.shape[0] != x.shape[0] or topk_idx.shape[1] < 1:
@@ -227,3 +237,24 @@ def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, 
     sh = [v for w in shared for v in (w.levels, w.scales)] or [None] * 4
     return _int4_experts(x, topk_w, topk_idx, w_in.levels, w_in.scales, w_out.levels, w_out.scales, *sh,
                          h, w_in.group, act)
+
+
+def _experts_fit(w_in, w_out, shared_in, shared_out):
+    """The arguments of the native call for expert weights that fit one another, else None (the caller
+    then finds out what is wrong with them)."""
+    if type(w_in) is not Int4Weight or type(w_out) is not Int4Weight:
+        return None
+    (e, d, h2), (e2, h, d2) = (w.shape if len(w.shape) == 3 else (0, 0, 0) for w in (w_in, w_out))
+    if h < 16 or h % 16 or h2 != 2 * h or e2 != e or d2 != d or w_in.group != w_out.group:
+        return None
+    if shared_in is None and shared_out is None:
+        sh = (None, None, None, None)
+    else:
+        if type(shared_in) is not Int4Weight or type(shared_out) is not Int4Weight:
+            return None
+        s = shared_in.shape[0]
+        if (shared_in.shape != (s, d, h2) or shared_out.shape != (s, h, d)
+                or not shared_in.group == shared_out.group == w_in.group):
+            return None
+        sh = (shared_in.levels, shared_in.scales, shared_out.levels, shared_out.scales)
+    return (w_in.levels, w_in.scales, w_out.levels, w_out.scales, *sh, d, h, w_in.group)
