@@ -682,8 +682,8 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
                            void* stream);
 
 /* ---- Weights in 4 bits -----------------------------------------------------------------------------
- * W[k, n] = (level[k, n] - 8) * scale[k / group, n], level 0 .. 15, group 32 or a multiple of 64; the
- * last group may be short. Packed once per matrix (nanospeaker_b200/int4.py does it), the outputs in
+ * W[k, n] = (level[k, n] - 8) * scale[k / group, n], level 0 .. 15, group 32, 64 or 128; the last
+ * group may be short. Packed once per matrix (nanospeaker_b200/int4.py does it), the outputs in
  * strips of 16, the inputs in blocks of 64, padded with level 8:
  *   levels [strips][blocks][32 lanes][4 words]: nibble i of the low / high half of word j of lane
  *     4 * g + t is input 64 * block + 32 * (j / 2) + 8 * t + 4 * (j % 2) + 2 * (i / 2) + {0, 1},
@@ -699,7 +699,7 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
  * reproducible. */
 int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* levels,
                      const void* scales, int32_t group, int32_t n_dim, int32_t dtype, void* y,
-                     void* stream);
+                     int32_t* status, void* stream);
 size_t moe_b200_int4_experts_scratch_bytes(int64_t n_tokens, int32_t top_k, int32_t n_shared,
                                            int32_t d_model, int32_t d_hidden);
 int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t d_model,

@@ -179,7 +179,7 @@ SIGNATURES = {
                        _c_vp, _c_vp, _c_sz, _c_vp, _c_vp]),
     "moe_b200_int4_mm": (
         ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_vp, _c_i32, _c_i32, _c_i32, _c_vp,
-                       _c_vp]),
+                       _c_vp, _c_vp]),
     "moe_b200_int4_experts_scratch_bytes": (_c_sz, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32]),
     "moe_b200_int4_experts": (
         ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp, _c_vp, _c_i32, _c_i32, _c_vp,

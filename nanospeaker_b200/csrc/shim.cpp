@@ -914,7 +914,7 @@ OptTensor int4_mm(const Tensor& x, const Tensor& levels, const Tensor& scales,
   const Tensor y = at::empty({flat.size(0), shape[1]}, x.options());
   check(abi.int4_mm(flat.const_data_ptr(), flat.size(0), row_stride(flat), int32_t(shape[0]),
                     levels.const_data_ptr(), scales.const_data_ptr(), int32_t(group), int32_t(shape[1]),
-                    dtype_id(x.scalar_type()), y.mutable_data_ptr(), current_stream()),
+                    dtype_id(x.scalar_type()), y.mutable_data_ptr(), status_word(x.get_device()), current_stream()),
         "moe_b200_int4_mm");
   n_launched += flat.size(0) > 0;
   if (x.dim() == 2) return y;

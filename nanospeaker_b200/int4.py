@@ -16,13 +16,14 @@ from . import kernels as K
 from .moe_kernel import _act_id, native_ok
 
 INT4_DTYPES = (torch.bfloat16, torch.float16)
+GROUPS = (32, 64, 128)      # inputs that share a scale
 
 
 class Int4Weight:
     """A matrix [K, N] (x @ W), or a stack [G, K, N] of them, in 4 bits, laid out as the kernels read it.
 
     shape     (K, N) or (G, K, N)
-    group     inputs that share a scale: 32 or a multiple of 64 (the last group of a matrix may be short)
+    group     inputs that share a scale: 32, 64 or 128 (the last group of a matrix may be short)
     levels    int32 [G, ceil(N / 16), ceil(K / 64), 32, 4]
     scales    [G, ceil(N / 16), groups, 8, 2], bf16 or fp16: the dtype of the activations"""
 
@@ -95,8 +96,8 @@ class Int4Weight:
 
 
 def _check_group(group: int) -> None:
-    if group != 32 and (group < 64 or group % 64):
-        raise ValueError(f"scale groups of {group} inputs: 32 or a multiple of 64")
+    if group not in GROUPS:
+        raise ValueError(f"scale groups of {group} inputs: {GROUPS} are covered")
 
 
 def quantize_int4(w: torch.Tensor, group: int = 64, dtype: Optional[torch.dtype] = None) -> Int4Weight:
@@ -154,7 +155,7 @@ def _(x, levels, scales, group, n_dim):
 def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     """x [..., K] times a weight [K, N] held in 4 bits -> [..., N], in x's dtype (that of the scales).
 
-    Made for few rows: up to 64 read the weight once, more read it once per 64. fp32 sums, rounded
+    Made for few rows: up to 32 read the weight once, more read it once per 32. fp32 sums, rounded
     once; bitwise reproducible."""
     if type(weight) is Int4Weight and native_ok(x):
         out = K.shim().int4_mm(x, weight.levels, weight.scales, weight.shape, weight.group)

@@ -886,7 +886,8 @@ def int4_mm(x: torch.Tensor, levels, scales, group: int, n_dim: int) -> torch.Te
     y = torch.empty((r, n_dim), dtype=x.dtype, device=x.device)
     _lib.check(_lib.load().moe_b200_int4_mm(
         x.data_ptr(), r, x.stride(0) if r > 1 else k, k, levels.data_ptr(), scales.data_ptr(), group,
-        n_dim, DTYPE_IDS.get(x.dtype, -1), y.data_ptr(), _stream(x)), "moe_b200_int4_mm")
+        n_dim, DTYPE_IDS.get(x.dtype, -1), y.data_ptr(), status_word(x.device).data_ptr(), _stream(x)),
+        "moe_b200_int4_mm")
     _count(1 if r else 0)
     return y
 

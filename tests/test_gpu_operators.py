@@ -265,7 +265,7 @@ def exact_weight(q, s, group):
 
 @pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 17, 31, 33, 64, 65, 200])
 @pytest.mark.parametrize("k,n,group", [(64, 16, 64), (8, 1, 32), (1000, 1537, 32), (576, 100, 64),
-                                       (4096, 48, 128), (136, 33, 192)])
+                                       (4096, 48, 128), (136, 33, 128), (192, 40, 128)])
 @pytest.mark.parametrize("dtype", HALF)
 def test_int4_mm(rows, k, n, group, dtype):
     q, s = levels((k, n), group, dtype)

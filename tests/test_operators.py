@@ -116,7 +116,7 @@ def test_thresholds(host):
 
 # --------------------------------------------------------------------------------- 4-bit weights
 @pytest.mark.parametrize("shape,group", [((8, 1), 32), ((64, 16), 64), ((1000, 1537), 32), ((576, 256), 64),
-                                         ((3, 128, 40), 64), ((2, 72, 16), 128), ((1, 200, 33), 192)])
+                                         ((3, 128, 40), 64), ((2, 72, 16), 128), ((1, 200, 33), 128)])
 def test_packing_returns_what_was_packed(shape, group):
     from nanospeaker_b200 import Int4Weight
     levels = torch.randint(0, 16, shape, dtype=torch.uint8)
@@ -175,7 +175,7 @@ def test_quantising_zeros_and_what_is_not_finite():
 def test_weight_refusals():
     from nanospeaker_b200 import Int4Weight, quantize_int4
     q, s = torch.zeros(64, 16, dtype=torch.uint8), torch.ones(1, 16).half()
-    for group in (0, 16, 33, 96):
+    for group in (0, 16, 33, 96, 256):
         with pytest.raises(ValueError, match="scale groups"):
             Int4Weight.from_levels(q, s, group)
     with pytest.raises(ValueError, match="uint8"):
@@ -278,12 +278,12 @@ def test_entry_points_validate_before_any_launch(lib):
     need = lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 100000, 2)
     assert need > 0 and lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 512, 2) == 0
     assert wg(rows=100000) == wg(rows=100000, sc=p, nb=need - 1) == -4
-    q = lambda x=p, rows=4, ld=64, k=64, lv=p, sc=p, grp=64, n=32, dt=0, y=p: \
-        lib.moe_b200_int4_mm(x, rows, ld, k, lv, sc, grp, n, dt, y, null)  # noqa: E731
+    q = lambda x=p, rows=4, ld=64, k=64, lv=p, sc=p, grp=64, n=32, dt=0, y=p, st=p: \
+        lib.moe_b200_int4_mm(x, rows, ld, k, lv, sc, grp, n, dt, y, st, null)  # noqa: E731
     assert q(rows=0) == 0
-    assert q(rows=-1) == q(k=60) == q(n=0) == q(ld=56) == q(grp=16) == q(grp=96) == -1
+    assert q(rows=-1) == q(k=60) == q(n=0) == q(ld=56) == q(grp=16) == q(grp=96) == q(grp=256) == -1
     assert q(dt=2) == -5
-    assert q(x=null) == q(lv=null) == q(sc=null) == q(y=null) == -2
+    assert q(x=null) == q(lv=null) == q(sc=null) == q(y=null) == q(st=null) == -2
     assert q(x=odd) == q(lv=odd) == q(sc=odd) == -3
     ex = lambda t=4, d=64, h=32, k=2, e=4, s=0, w=p, idx=p, grp=64, act=0, dt=0, sc=p, nb=1 << 20, sh=null, o=p: \
         lib.moe_b200_int4_experts(p, t, d, d, h, w, idx, k, e, p, p, p, p, s, sh, sh, sh, sh, grp, act,
