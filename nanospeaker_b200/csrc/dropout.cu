@@ -21,12 +21,12 @@ namespace moe {
 
 constexpr int DROP_THREADS = 256;
 
-// 8 values of type T, as loaded and stored: one or two 16-byte pieces.
+// 16 bytes of type T as floats and back.
 template <typename T>
-struct Eight {
-  uint4 v[1];
-  __device__ __forceinline__ void to_float(float* f) const {
-    const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+struct Piece {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void to_float(const uint4& v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 p = Half16<T>::unpack(w[i]);
@@ -34,28 +34,22 @@ struct Eight {
       f[2 * i + 1] = p.y;
     }
   }
-  __device__ __forceinline__ void from_float(const float* f) {
-    v[0] = make_uint4(Half16<T>::pack(f[0], f[1]), Half16<T>::pack(f[2], f[3]),
-                      Half16<T>::pack(f[4], f[5]), Half16<T>::pack(f[6], f[7]));
+  static __device__ __forceinline__ uint4 from_float(const float* f) {
+    return make_uint4(Half16<T>::pack(f[0], f[1]), Half16<T>::pack(f[2], f[3]), Half16<T>::pack(f[4], f[5]),
+                      Half16<T>::pack(f[6], f[7]));
   }
 };
 template <>
-struct Eight<float> {
-  uint4 v[2];
-  __device__ __forceinline__ void to_float(float* f) const {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      f[4 * i] = __uint_as_float(v[i].x);
-      f[4 * i + 1] = __uint_as_float(v[i].y);
-      f[4 * i + 2] = __uint_as_float(v[i].z);
-      f[4 * i + 3] = __uint_as_float(v[i].w);
-    }
+struct Piece<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void to_float(const uint4& v, float* f) {
+    f[0] = __uint_as_float(v.x);
+    f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z);
+    f[3] = __uint_as_float(v.w);
   }
-  __device__ __forceinline__ void from_float(const float* f) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]),
-                        __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+  static __device__ __forceinline__ uint4 from_float(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
 };
 template <typename T>
@@ -67,47 +61,61 @@ __device__ __forceinline__ T one_from_float(float v) { return Half16<T>::from_fl
 template <>
 __device__ __forceinline__ float one_from_float<float>(float v) { return v; }
 
-// n8 = elements / 8 that lie in whole, 16-byte aligned pieces (0 where a pointer is not aligned); the rest
-// goes one by one. A dropped element adds nothing, whatever its value (a product would make NaN of an
-// infinity).
-template <typename T, bool RES>
+// `pieces` 16-byte pieces (0 where a pointer is not aligned); the rest goes one by one. A thread has 16
+// elements at a time, in pieces a block's width apart: four counters. A dropped element adds nothing, whatever
+// its value (a product would make NaN of an infinity). SMALL: no counter passes 32 bits; its upper word and
+// the call's are then the same for all threads, and the products of theirs in the first rounds are made once.
+template <typename T, bool RES, bool SMALL>
 __global__ void __launch_bounds__(DROP_THREADS)
     dropout_kernel(const T* x, const T* residual, const int64_t* rng, int64_t* used, T* out, int64_t n,
-                   int64_t n8, uint32_t threshold, float scale) {
+                   int64_t pieces, uint32_t threshold, float scale) {
+  constexpr int N = Piece<T>::N, PIECES = 16 / N, QUADS = N / 4;
   pdl_trigger();
   pdl_wait();
   const int64_t seed = ld_prev(rng), call = ld_prev(rng + 1);
-  const int64_t first = int64_t(blockIdx.x) * DROP_THREADS + threadIdx.x;
-  const int64_t step = int64_t(gridDim.x) * DROP_THREADS;
-  if (used != nullptr && first == 0) {
+  if (used != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
     used[0] = seed;
     used[1] = call;
   }
-  for (int64_t i = first; i < n8; i += step) {
-    const Eight<T> a = reinterpret_cast<const Eight<T>*>(x)[i];
-    Eight<T> r;
-    if constexpr (RES) r = reinterpret_cast<const Eight<T>*>(residual)[i];
-    uint32_t word[8];
-    philox4x32(uint64_t(2 * i), uint64_t(call), uint64_t(seed), word);
-    philox4x32(uint64_t(2 * i + 1), uint64_t(call), uint64_t(seed), word + 4);
-    float f[8], o[8];
-    a.to_float(f);
-    if constexpr (RES) {
-      r.to_float(o);
+  auto counter = [](int64_t quad) { return SMALL ? uint64_t(uint32_t(quad)) : uint64_t(quad); };
+  const int64_t block = int64_t(DROP_THREADS) * PIECES;
+  for (int64_t at = blockIdx.x * block + threadIdx.x; at < pieces; at += gridDim.x * block) {
+    uint4 a[PIECES], r[PIECES];
+    uint64_t low[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = word[k] >= threshold ? fmaf(f[k], scale, o[k]) : o[k];
-    } else {
+    for (int h = 0; h < PIECES; ++h) {
+      const int64_t i = at + h * DROP_THREADS;
+      if (i < pieces) {
+        a[h] = reinterpret_cast<const uint4*>(x)[i];
+        if constexpr (RES) r[h] = reinterpret_cast<const uint4*>(residual)[i];
+      }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = word[k] >= threshold ? f[k] * scale : 0.f;
+      for (int q = 0; q < QUADS; ++q) low[h * QUADS + q] = counter(i * QUADS + q);
     }
-    Eight<T> to;
-    to.from_float(o);
-    reinterpret_cast<Eight<T>*>(out)[i] = to;
+    uint32_t word[4][4];
+    philox4x32<4>(low, uint64_t(call), uint64_t(seed), word);
+#pragma unroll
+    for (int h = 0; h < PIECES; ++h) {
+      const int64_t i = at + h * DROP_THREADS;
+      if (i >= pieces) break;
+      float f[N], o[N];
+      Piece<T>::to_float(a[h], f);
+      if constexpr (RES) Piece<T>::to_float(r[h], o);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const bool keep = word[h * QUADS + k / 4][k % 4] >= threshold;
+        if constexpr (RES) o[k] = keep ? fmaf(f[k], scale, o[k]) : o[k];
+        else o[k] = keep ? f[k] * scale : 0.f;
+      }
+      reinterpret_cast<uint4*>(out)[i] = Piece<T>::from_float(o);
+    }
   }
-  for (int64_t i = n8 * 8 + first; i < n; i += step) {
-    uint32_t word[4];
-    philox4x32(uint64_t(i >> 2), uint64_t(call), uint64_t(seed), word);
-    const uint32_t mine = (i & 2) ? ((i & 1) ? word[3] : word[2]) : ((i & 1) ? word[1] : word[0]);
+  const int64_t first = int64_t(blockIdx.x) * DROP_THREADS + threadIdx.x;
+  for (int64_t i = pieces * N + first; i < n; i += int64_t(gridDim.x) * DROP_THREADS) {
+    uint32_t word[1][4];
+    const uint64_t low = counter(i >> 2);
+    philox4x32<1>(&low, uint64_t(call), uint64_t(seed), word);
+    const uint32_t mine = (i & 2) ? ((i & 1) ? word[0][3] : word[0][2]) : ((i & 1) ? word[0][1] : word[0][0]);
     float o = 0.f;
     if constexpr (RES) o = one_to_float<T>(residual[i]);
     if (mine >= threshold) o = fmaf(one_to_float<T>(x[i]), scale, o);
@@ -121,12 +129,15 @@ static int launch_dropout(const void* x, const void* residual, const int64_t* rn
   const uintptr_t any = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
                         reinterpret_cast<uintptr_t>(out);
   if (any % sizeof(T)) return MOE_B200_ERR_ALIGN;
-  const int64_t n8 = any % 16 ? 0 : n / 8;
-  const int64_t work = std::max(n8, n - n8 * 8);
+  constexpr int N = Piece<T>::N;
+  const int64_t pieces = any % 16 ? 0 : n / N;
+  const int64_t work = std::max((pieces * N + 15) / 16, n - pieces * N);
   const int64_t blocks = std::min<int64_t>((work + DROP_THREADS - 1) / DROP_THREADS, 148 * 8);
-  auto kern = residual ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+  const bool small = n <= int64_t(4) << 32;
+  auto kern = residual ? (small ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>)
+                       : (small ? dropout_kernel<T, false, true> : dropout_kernel<T, false, false>);
   return launch_pdl(kern, dim3(unsigned(blocks)), dim3(DROP_THREADS), 0, st, static_cast<const T*>(x),
-                    static_cast<const T*>(residual), rng, used, static_cast<T*>(out), n, n8, threshold,
+                    static_cast<const T*>(residual), rng, used, static_cast<T*>(out), n, pieces, threshold,
                     scale) == cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;

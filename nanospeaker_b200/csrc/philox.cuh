@@ -12,26 +12,38 @@
 
 namespace moe {
 
-// The four words at counter (low, high) under `key`.
-MOE_PHILOX_FN void philox4x32(uint64_t low, uint64_t high, uint64_t key, uint32_t* word) {
-  uint32_t c0 = uint32_t(low), c1 = uint32_t(low >> 32), c2 = uint32_t(high), c3 = uint32_t(high >> 32);
+// The words at counters (low[j], high) under `key`, four each: N counters side by side, so that they share the
+// key's schedule and fill each other's waits.
+template <int N>
+MOE_PHILOX_FN void philox4x32(const uint64_t* low, uint64_t high, uint64_t key, uint32_t (*word)[4]) {
   uint32_t k0 = uint32_t(key), k1 = uint32_t(key >> 32);
 #ifdef __CUDACC__
 #pragma unroll
 #endif
+  for (int j = 0; j < N; ++j) {
+    word[j][0] = uint32_t(low[j]);
+    word[j][1] = uint32_t(low[j] >> 32);
+    word[j][2] = uint32_t(high);
+    word[j][3] = uint32_t(high >> 32);
+  }
+#ifdef __CUDACC__
+#pragma unroll
+#endif
   for (int i = 0; i < 10; ++i) {
-    const uint64_t p0 = uint64_t(0xD2511F53u) * c0, p1 = uint64_t(0xCD9E8D57u) * c2;
-    c0 = uint32_t(p1 >> 32) ^ c1 ^ k0;
-    c1 = uint32_t(p1);
-    c2 = uint32_t(p0 >> 32) ^ c3 ^ k1;
-    c3 = uint32_t(p0);
+#ifdef __CUDACC__
+#pragma unroll
+#endif
+    for (int j = 0; j < N; ++j) {
+      uint32_t* c = word[j];
+      const uint64_t p0 = uint64_t(0xD2511F53u) * c[0], p1 = uint64_t(0xCD9E8D57u) * c[2];
+      c[0] = uint32_t(p1 >> 32) ^ c[1] ^ k0;
+      c[1] = uint32_t(p1);
+      c[2] = uint32_t(p0 >> 32) ^ c[3] ^ k1;
+      c[3] = uint32_t(p0);
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  word[0] = c0;
-  word[1] = c1;
-  word[2] = c2;
-  word[3] = c3;
 }
 
 // An element whose word is below this is dropped: p in [0, 1) in units of 2^-32, to the nearest (ties to

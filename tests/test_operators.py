@@ -35,7 +35,12 @@ void tile(int l, int m, int n, int band, int* out) {
 int chunks(int rows, int ks) { return moe::run_chunks(rows, ks); }
 long long chunk_rows(long long rows, long long tiles, int ctas) { return moe::grouped_chunk_rows(rows, tiles, ctas); }
 void philox(unsigned long long low, unsigned long long high, unsigned long long key, unsigned* w) {
-  moe::philox4x32(low, high, key, w);
+  const uint64_t at = low;
+  moe::philox4x32<1>(&at, high, key, reinterpret_cast<uint32_t(*)[4]>(w));
+}
+void philox4(unsigned long long low, unsigned long long high, unsigned long long key, unsigned* w) {
+  const uint64_t at[4] = {low, low + 1, low + 2, low + 3};
+  moe::philox4x32<4>(at, high, key, reinterpret_cast<uint32_t(*)[4]>(w));
 }
 unsigned threshold(double p) { return moe::dropout_threshold(p); }
 }
@@ -46,7 +51,7 @@ unsigned threshold(double p) { return moe::dropout_threshold(p); }
     lib = ctypes.CDLL(str(so))
     lib.chunk_rows.restype = ctypes.c_longlong
     lib.chunk_rows.argtypes = [ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int]
-    lib.philox.argtypes = [ctypes.c_ulonglong] * 3 + [ctypes.c_void_p]
+    lib.philox.argtypes = lib.philox4.argtypes = [ctypes.c_ulonglong] * 3 + [ctypes.c_void_p]
     lib.threshold.restype = ctypes.c_uint
     lib.threshold.argtypes = [ctypes.c_double]
     return lib
@@ -107,6 +112,15 @@ def test_philox_known_answers(host, counter, key, want):
     w = (ctypes.c_uint * 4)()
     host.philox(counter[0] | counter[1] << 32, counter[2] | counter[3] << 32, key[0] | key[1] << 32, w)
     assert list(w) == want
+
+
+def test_counters_side_by_side_are_the_single_ones(host):
+    for low in (0, 12, (1 << 32) - 4, 1 << 32, 0x123456789ABCDEF0):
+        four, one = (ctypes.c_uint * 16)(), (ctypes.c_uint * 4)()
+        host.philox4(low, 77, 0x1122334455667788, four)
+        for j in range(4):
+            host.philox(low + j, 77, 0x1122334455667788, one)
+            assert list(four[4 * j:4 * j + 4]) == list(one)
 
 
 def test_thresholds(host):
