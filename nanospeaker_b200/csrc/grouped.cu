@@ -325,7 +325,7 @@ struct WgradArgs {
   int32_t n_groups, rows;
   int32_t ks;               // rows of a chunk
   int32_t m_dim, n_dim;     // one dw[g]
-  int32_t m_tiles, n_tiles;
+  int32_t m_tiles, n_tiles; // tiles of a CTA pair
   int32_t a_fused, b_fused; // the operand's width is a multiple of 64: one copy brings a stage of it
   void* out;                // [n_groups, m_dim, n_dim]
   int32_t wide;
@@ -333,24 +333,41 @@ struct WgradArgs {
   int32_t* status;
 };
 
+constexpr int MAX_SORTED = 512;   // chunks that are put in order of their length
+constexpr int WGRAD_THREADS = 96 + EPI_WARPS * 32;
+
 template <int BN, int STAGES>
 struct WgradSmem {
-  static constexpr int B_BYTES = BN * BK * 2;
+  static constexpr int B_BYTES = (BN / 2) * BK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int BARS = STAGES * STAGE;
-  static constexpr int MISC = BARS + 8 * (2 * STAGES + 6);
+  static constexpr int TAILS = STAGES * STAGE;             // two stages for the ends of runs
+  static constexpr int BARS = TAILS + 2 * STAGE;
+  static constexpr int MISC = BARS + 8 * (2 * STAGES + 10);
   static constexpr int TABLE = (MISC + 16 + 15) / 16 * 16;
   static constexpr int SPLIT = TABLE + int(sizeof(RunTable));   // first chunk of every split run
-  static constexpr int TOTAL = SPLIT + (RUNS_MAX_GROUPS + 1) * 4;
+  static constexpr int LENGTHS = SPLIT + (RUNS_MAX_GROUPS + 1) * 4;
+  static constexpr int ORDER = LENGTHS + MAX_SORTED * 4;
+  static constexpr int TOTAL = ORDER + MAX_SORTED * 2;
   static constexpr int DYNAMIC = TOTAL + 1024;
+  static_assert(STAGE % 1024 == 0, "stages must keep the 1024-byte swizzle alignment");
   static_assert(DYNAMIC <= 232448, "more shared memory than a CTA has");
 };
 
-// 128 x BN tiles of dw[g], one CTA each; both operands are MN-major (their rows are the contraction). Warps:
-// 0 loads, 1 multiplies, 2 .. 9 store, 10 sets the rows behind the end of a run to zero in its last stage.
-// Runs of more than ks rows are cut into chunks whose fp32 tiles wgrad_join_kernel adds in order.
+// 256 x BN tiles of dw[g] on CTA pairs: each CTA loads 128 columns of the first operand and half of the
+// second's, both MN-major (their rows are the contraction). A single CTA's 128 x 256 tile takes 48 KB for 512
+// cycles of MMAs, more than an SM gets out of L2; the pair's takes 32 KB per CTA (32768 rows x 2048 x 4096 in
+// 16 groups: 471 us alone, the pairs' figure in the table of the documentation).
+//
+// A run's last rows, fewer than a stage, go through two stages of their own: they land on a barrier of their
+// CTA, a warp sets the rows behind the run's end to zero (up to the next 16, which is what an MMA takes) and
+// tells the leader. That happens ahead of the MMAs and keeps them out of it. Warps: 0 loads, 1 multiplies (the
+// leader's), 2 .. 9 store, 10 clears.
+//
+// Work items are chunks of runs (at most ks rows), longest first, every tile of one after another; the
+// clusters take them in turns, back and forth, so that the long ones do not come last. The fp32 tiles of runs
+// with several chunks are added in order by wgrad_join_kernel.
 template <typename T, int BN, int STAGES>
-__global__ void __launch_bounds__(96 + EPI_WARPS * 32, 1)
+__global__ void __launch_bounds__(WGRAD_THREADS, 1)
     grouped_wgrad_kernel(const __grid_constant__ CUtensorMap tmA,
                          const __grid_constant__ CUtensorMap tmB, const WgradArgs p) {
   using L = WgradSmem<BN, STAGES>;
@@ -363,15 +380,21 @@ __global__ void __launch_bounds__(96 + EPI_WARPS * 32, 1)
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint64_t* dirty_bar = tempty_bar + 2;   // a run's last stage has landed, with rows behind the run's end
-  uint64_t* clean_bar = dirty_bar + 1;    // they are zero
+  uint64_t* landed_bar = tempty_bar + 2;    // a run's end is in this CTA's tail stage
+  uint64_t* cleared_bar = landed_bar + 2;   // leader: and clean in both CTAs'
+  uint64_t* used_bar = cleared_bar + 2;     // and multiplied
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  RunTable& table = *reinterpret_cast<RunTable*>(smem + L::TABLE);
+  RunTable& table = *reinterpret_cast<RunTable*>(smem + L::TABLE);   // first: in chunks
   int* split_first = reinterpret_cast<int*>(smem + L::SPLIT);
+  int* lengths = reinterpret_cast<int*>(smem + L::LENGTHS);
+  uint16_t* order = reinterpret_cast<uint16_t*>(smem + L::ORDER);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int n_clusters = int(gridDim.x) >> 1;
+  const int cluster = int(blockIdx.x) >> 1;
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmA);
@@ -380,148 +403,216 @@ __global__ void __launch_bounds__(96 + EPI_WARPS * 32, 1)
       mbar_init(full_bar + s, 1);
       mbar_init(empty_bar + s, 1);
     }
-    mbar_init(dirty_bar, 1);
-    mbar_init(clean_bar, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar + b, 1);
-      mbar_init(tempty_bar + b, EPI_WARPS);
+      mbar_init(tempty_bar + b, 2 * EPI_WARPS);
+      mbar_init(landed_bar + b, 1);
+      mbar_init(cleared_bar + b, 2);
+      mbar_init(used_bar + b, 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
-    tmem_relinquish();
+    tmem_alloc2(tmem_slot, TMEM_COLS);
+    tmem_relinquish2();
     pdl_trigger();
   }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
   pdl_wait();
+
+  const int tiles = p.m_tiles * p.n_tiles;
   if (warp == 2) {
     const bool bad = load_run_starts(p.offsets, p.n_groups, p.rows, lane, table.start);
     if (bad && blockIdx.x == 0 && lane == 0) atomicExch(p.status, ST_BAD_OFFSETS);
-    const int ks = p.ks, tiles = p.m_tiles * p.n_tiles;
-    count_run_units(table.start, p.n_groups, lane, table.first,
-                    [=](int rows) { return run_chunks(rows, ks) * tiles; });
+    const int ks = p.ks;
+    count_run_units(table.start, p.n_groups, lane, table.first, [=](int rows) { return run_chunks(rows, ks); });
     count_run_units(table.start, p.n_groups, lane, split_first,
                     [=](int rows) { return rows > ks ? run_chunks(rows, ks) : 0; });
   }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  struct Chunk {
+    int group, at, len;   // `at`: which of its run
+  };
+  auto chunk_of = [&](int i) {
+    Chunk c;
+    c.group = run_of_unit(table.first, p.n_groups, i);
+    c.at = i - table.first[c.group];
+    c.len = min(p.ks, table.start[c.group + 1] - table.start[c.group] - c.at * p.ks);
+    return c;
+  };
+  const int n_chunks = table.first[p.n_groups];
+  const bool sorted = n_chunks <= MAX_SORTED;
+  if (sorted) {
+    for (int i = threadIdx.x; i < n_chunks; i += WGRAD_THREADS) lengths[i] = chunk_of(i).len;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_chunks; i += WGRAD_THREADS) {
+      const int mine = lengths[i];
+      int before = 0;
+      for (int j = 0; j < n_chunks; ++j) before += lengths[j] > mine || (lengths[j] == mine && j < i);
+      order[before] = uint16_t(i);
+    }
+    __syncthreads();
+  }
 
-  const int n_units = table.first[p.n_groups];
+  const int n_units = n_chunks * tiles;
+  const int n_rounds = (n_units + n_clusters - 1) / n_clusters;
   struct Unit {
     int group, row0, len, m0, n0;
-    int part;   // its chunk among those of split runs, -1: the run's only one
+    int part;   // its chunk among those of split runs, -1: the run's only one; -2: no unit in this round
   };
-  auto unit_of = [&](int u) {
+  auto unit_of = [&](int round) {
     Unit c;
-    c.group = run_of_unit(table.first, p.n_groups, u);
-    const int start = table.start[c.group], rows = table.start[c.group + 1] - start;
-    const int l = u - table.first[c.group], tiles = p.m_tiles * p.n_tiles;
-    const int chunk = l / tiles;
-    const TileAt t = tile_in_bands(l - chunk * tiles, p.m_tiles, p.n_tiles, BAND);
-    c.row0 = start + chunk * p.ks;
-    c.len = min(p.ks, rows - chunk * p.ks);
-    c.m0 = t.m * BM;
+    const int u = round * n_clusters + (round & 1 ? n_clusters - 1 - cluster : cluster);
+    if (u >= n_units) {
+      c.part = -2;
+      c.len = 0;
+      return c;
+    }
+    const int k = u / tiles;
+    const Chunk ch = chunk_of(sorted ? order[k] : k);
+    const TileAt t = tile_in_bands(u - k * tiles, p.m_tiles, p.n_tiles, BAND);
+    c.group = ch.group;
+    c.row0 = table.start[ch.group] + ch.at * p.ks;
+    c.len = ch.len;
+    c.m0 = (t.m * 2 + int(rank)) * BM;   // this CTA's rows of dw
     c.n0 = t.n * BN;
-    c.part = rows > p.ks ? split_first[c.group] + chunk : -1;
+    c.part = split_first[ch.group + 1] > split_first[ch.group] ? split_first[ch.group] + ch.at : -1;
     return c;
   };
 
   if (warp == 0) {
     if (elect_one()) {
       uint32_t it = 0;
-      for (int u = blockIdx.x; u < n_units && !*abort_flag; u += gridDim.x) {
-        const Unit c = unit_of(u);
-        const int num_k = (c.len + BK - 1) / BK;
-        for (int kt = 0; kt < num_k; ++kt, ++it) {
+      int tails = 0;
+      auto give_up = [&] {
+        *abort_flag = 1;
+        atomicExch(p.status, ST_WAIT_TIMEOUT);
+      };
+      for (int round = 0; round < n_rounds && !*abort_flag; ++round) {
+        const Unit c = unit_of(round);
+        const int full = c.len / BK, nb = c.n0 + int(rank) * (BN / 2);
+        for (int kt = 0; kt < full; ++kt, ++it) {
           const int s = it % STAGES;
           const uint32_t use = it / STAGES;
           if (use > 0 && !mbar_wait(empty_bar + s, (use - 1) & 1, p.status)) {
-            *abort_flag = 1;
-            atomicExch(p.status, ST_WAIT_TIMEOUT);
+            give_up();
             break;
           }
           uint8_t* sA = smem + s * L::STAGE;
           uint8_t* sB = sA + A_BYTES;
-          mbar_expect_tx(full_bar + s, L::STAGE);
+          if (rank == 0) mbar_expect_tx(full_bar + s, 2 * L::STAGE);
           const int row = c.row0 + kt * BK;
           if (p.a_fused) {
-            tma_load_3d(sA, &tmA, full_bar + s, 0, row, c.m0 / 64);
+            tma_load_3d_2cta(sA, &tmA, full_bar + s, 0, row, c.m0 / 64);
           } else {
 #pragma unroll
             for (int i = 0; i < BM / 64; ++i)
-              tma_load_2d(sA + i * 64 * BK * 2, &tmA, full_bar + s, c.m0 + 64 * i, row);
+              tma_load_3d_2cta(sA + i * 64 * BK * 2, &tmA, full_bar + s, c.m0 + 64 * i, row, 0);
           }
           if (p.b_fused) {
-            tma_load_3d(sB, &tmB, full_bar + s, 0, row, c.n0 / 64);
+            tma_load_3d_2cta(sB, &tmB, full_bar + s, 0, row, nb / 64);
           } else {
 #pragma unroll
-            for (int i = 0; i < BN / 64; ++i)
-              tma_load_2d(sB + i * 64 * BK * 2, &tmB, full_bar + s, c.n0 + 64 * i, row);
+            for (int i = 0; i < BN / 128; ++i)
+              tma_load_3d_2cta(sB + i * 64 * BK * 2, &tmB, full_bar + s, nb + 64 * i, row, 0);
           }
         }
+        if (c.len % BK == 0 || *abort_flag) continue;
+        const int b = tails & 1;
+        const uint32_t use = uint32_t(tails) >> 1;
+        if (use > 0 && !mbar_wait(used_bar + b, (use - 1) & 1, p.status)) {
+          give_up();
+          break;
+        }
+        ++tails;
+        uint8_t* sA = smem + L::TAILS + b * L::STAGE;
+        uint8_t* sB = sA + A_BYTES;
+        mbar_expect_tx(landed_bar + b, L::STAGE);
+        const int row = c.row0 + full * BK;
+        if (p.a_fused) {
+          tma_load_3d(sA, &tmA, landed_bar + b, 0, row, c.m0 / 64);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BM / 64; ++i)
+            tma_load_3d(sA + i * 64 * BK * 2, &tmA, landed_bar + b, c.m0 + 64 * i, row, 0);
+        }
+        if (p.b_fused) {
+          tma_load_3d(sB, &tmB, landed_bar + b, 0, row, nb / 64);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BN / 128; ++i)
+            tma_load_3d(sB + i * 64 * BK * 2, &tmB, landed_bar + b, nb + 64 * i, row, 0);
+        }
       }
-      if (*abort_flag) drain_ring<STAGES>(full_bar, it);
+      if (*abort_flag) {   // (the leader's barriers count both CTAs' bytes, and the pair leaves together)
+        if (rank == 0) drain_ring<STAGES>(full_bar, it);
+        drain_ring<2>(landed_bar, uint32_t(tails));
+      }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc = umma_idesc(BM, BN, true, true, Half16<T>::UMMA_FMT);
-      uint32_t it = 0, tails = 0;
-      int j = 0;
-      for (int u = blockIdx.x; u < n_units && !*abort_flag; u += gridDim.x) {
-        const Unit c = unit_of(u);
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = umma_idesc(2 * BM, BN, true, true, Half16<T>::UMMA_FMT);
+      uint32_t it = 0;
+      int j = 0, tails = 0;
+      for (int round = 0; round < n_rounds && !*abort_flag; ++round) {
+        const Unit c = unit_of(round);
         if (c.len <= 0) continue;
-        const int num_k = (c.len + BK - 1) / BK;
         const int b = j & 1;
         const uint32_t use = uint32_t(j) >> 1;
         ++j;
-        if (use > 0 && !mbar_wait(tempty_bar + b, (use - 1) & 1, p.status)) {
+        bool ok = use == 0 || mbar_wait(tempty_bar + b, (use - 1) & 1, p.status);
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + b * TMEM_BUF;
+        uint32_t more = 0;
+        auto multiply = [&](uint32_t sA, int steps) {
+          const uint32_t sB = sA + A_BYTES;
+#pragma unroll
+          for (int k16 = 0; k16 < BK / 16; ++k16)
+            if (k16 < steps) {
+              umma_f16_2cta(d_tmem, umma_desc(sA + k16 * MN_KADV, MN_LBO, MN_SBO),
+                            umma_desc(sB + k16 * MN_KADV, MN_LBO, MN_SBO), idesc, more);
+              more = 1;
+            }
+        };
+        const int full = c.len / BK, tail = c.len % BK;
+        for (int kt = 0; kt < full && ok; ++kt, ++it) {
+          const int s = it % STAGES;
+          ok = mbar_wait(full_bar + s, (it / STAGES) & 1, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          multiply(smem_u32(smem + s * L::STAGE), BK / 16);
+          umma_commit_2cta(empty_bar + s, 3);
+        }
+        if (ok && tail > 0) {
+          const int tb = tails & 1;
+          ok = mbar_wait_cluster(cleared_bar + tb, (uint32_t(tails) >> 1) & 1, p.status);
+          ++tails;
+          if (ok) {
+            tc_fence_after();
+            multiply(smem_u32(smem + L::TAILS + tb * L::STAGE), (tail + 15) / 16);
+            umma_commit_2cta(used_bar + tb, 3);
+          }
+        }
+        if (!ok) {
           *abort_flag = 1;
           atomicExch(p.status, ST_WAIT_TIMEOUT);
           break;
         }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + b * TMEM_BUF;
-        for (int kt = 0; kt < num_k; ++kt, ++it) {
-          const int s = it % STAGES;
-          bool ok = mbar_wait(full_bar + s, (it / STAGES) & 1, p.status);
-          if (ok && (kt + 1) * BK > c.len) {
-            mbar_arrive(dirty_bar);
-            ok = mbar_wait(clean_bar, tails & 1, p.status);
-            ++tails;
-          }
-          if (!ok) {
-            *abort_flag = 1;
-            atomicExch(p.status, ST_WAIT_TIMEOUT);
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sA = smem_u32(smem + s * L::STAGE);
-          const uint32_t sB = sA + A_BYTES;
-#pragma unroll
-          for (int k16 = 0; k16 < BK / 16; ++k16)
-            umma_f16(d_tmem, umma_desc(sA + k16 * MN_KADV, MN_LBO, MN_SBO),
-                     umma_desc(sB + k16 * MN_KADV, MN_LBO, MN_SBO), idesc,
-                     (kt == 0 && k16 == 0) ? 0u : 1u);
-          umma_commit(empty_bar + s);
-        }
-        umma_commit(tfull_bar + b);
+        umma_commit_2cta(tfull_bar + b, 3);
       }
     }
   } else if (warp == 2 + EPI_WARPS) {
-    uint32_t it = 0, tails = 0;
-    for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
-      const Unit c = unit_of(u);
-      const int num_k = (c.len + BK - 1) / BK;
-      it += num_k;
-      const int tail = c.len - (num_k - 1) * BK;
-      if (c.len <= 0 || tail == BK) continue;
-      const int s = (it - 1) % STAGES;
-      // (the MMA thread's word for it, not the ring's barrier: this warp does not see the ring's other
-      // uses, and a barrier tells a phase from the one before it only. The lanes go on together or not at all.)
-      const bool ok = mbar_wait(dirty_bar, tails & 1, p.status);
+    int tails = 0;
+    for (int round = 0; round < n_rounds; ++round) {
+      const int tail = unit_of(round).len % BK;
+      if (tail == 0) continue;
+      const int b = tails & 1;
+      // (the lanes go on together or not at all)
+      const bool ok = mbar_wait(landed_bar + b, (uint32_t(tails) >> 1) & 1, p.status);
       ++tails;
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) {
@@ -531,16 +622,14 @@ __global__ void __launch_bounds__(96 + EPI_WARPS * 32, 1)
         break;
       }
       // a 64 x 64 box keeps its row r in bytes r * 128 .. r * 128 + 127, in whatever order
-      const uint32_t base = smem_u32(smem + s * L::STAGE);
-      const int pieces = (BK - tail) * 8;
-      constexpr int BOXES = BM / 64 + BN / 64;
-      for (int i = lane; i < BOXES * pieces; i += 32) {
-        const int box = i / pieces;
-        st_shared_v4(base + box * (64 * BK * 2) + tail * 128 + (i - box * pieces) * 16, 0, 0, 0, 0);
-      }
+      const uint32_t first = smem_u32(smem + L::TAILS + b * L::STAGE) + tail * 128;
+      const int bytes = ((tail + 15) / 16 * 16 - tail) * 128;
+#pragma unroll
+      for (int box = 0; box < BM / 64 + BN / 128; ++box)
+        for (int i = lane * 16; i < bytes; i += 512) st_shared_v4(first + box * (64 * BK * 2) + i, 0, 0, 0, 0);
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(clean_bar);
+      if (lane == 0) mbar_arrive_release_cluster(mapa_u32(smem_u32(cleared_bar + b), 0));
     }
   } else {
     const int ew = warp - 2;
@@ -548,11 +637,13 @@ __global__ void __launch_bounds__(96 + EPI_WARPS * 32, 1)
     const int half = ew >> 2;
     const int row = q * 32 + lane;
     constexpr int NCH = BN / 32;
+    const uint32_t tempty_leader = mapa_u32(smem_u32(tempty_bar), 0);
     T* out = static_cast<T*>(p.out);
     const int64_t matrix = int64_t(p.m_dim) * p.n_dim;
     int j = 0;
-    for (int u = blockIdx.x; u < n_units; u += gridDim.x) {
-      const Unit c = unit_of(u);
+    for (int round = 0; round < n_rounds; ++round) {
+      const Unit c = unit_of(round);
+      if (c.part == -2) continue;
       const bool have = c.len > 0;
       const int b = j & 1;
       if (have) {
@@ -592,14 +683,15 @@ __global__ void __launch_bounds__(96 + EPI_WARPS * 32, 1)
       if (have) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar + b);
+        if (lane == 0) mbar_arrive_cluster(tempty_leader + b * 8);
       }
     }
   }
 
+  // Nobody leaves while the other CTA may still signal its barriers or read its shared memory.
   tc_fence_before();
-  __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+  cluster_sync_all();
+  if (warp == 1) tmem_dealloc2(tmem_base, TMEM_COLS);
 }
 
 // dw[g] = sum of the fp32 partials of its chunks, in order, for the runs that were cut. blockIdx.y walks the
@@ -680,7 +772,8 @@ static bool map_w_mnmajor(CUtensorMap* m, const void* w, int64_t groups, int64_t
   const uint32_t box[3] = {64, 64, 1};
   return make_map(m, w, 3, dims, strides, box);
 }
-// A [rows, cols] matrix as an MN-major operand of the weight gradient.
+// A [rows, cols] matrix as an MN-major operand of the weight gradient: `boxes` 64 x 64 boxes per copy where cols
+// is a multiple of 64.
 static bool map_mn(CUtensorMap* m, const void* x, int64_t rows, int64_t ld, int64_t cols, int boxes,
                    int32_t* fused) {
   *fused = cols % 64 == 0;
@@ -690,10 +783,7 @@ static bool map_mn(CUtensorMap* m, const void* x, int64_t rows, int64_t ld, int6
     const uint32_t box[3] = {64, 64, uint32_t(boxes)};
     return make_map(m, x, 3, dims, strides, box);
   }
-  const uint64_t dims[2] = {uint64_t(cols), uint64_t(rows)};
-  const uint64_t strides[1] = {uint64_t(ld) * 2};
-  const uint32_t box[2] = {64, 64};
-  return make_map(m, x, 2, dims, strides, box);
+  return map_x(m, x, rows, ld, cols, 64);
 }
 
 // Clusters of two of `kern` that are resident at once (fewer than half the SMs: they pair up inside a
@@ -769,12 +859,13 @@ static int rows_product(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
                  : launch_rows<T, 128, false>(tmA, tmShort, tmB, a, units, dev, st);
 }
 
-constexpr int WGRAD_BN_WIDE = 256;
-static int wgrad_bn(int32_t n_dim) { return n_dim > 128 ? WGRAD_BN_WIDE : 128; }
+static int wgrad_bn(int32_t n_dim) { return n_dim > 128 ? 256 : 128; }
 static int64_t wgrad_tiles(int32_t m_dim, int32_t n_dim) {
   const int bn = wgrad_bn(n_dim);
-  return int64_t((m_dim + BM - 1) / BM) * ((n_dim + bn - 1) / bn);
+  return int64_t((m_dim + 2 * BM - 1) / (2 * BM)) * ((n_dim + bn - 1) / bn);
 }
+// (of every device alike: the scratch is sized before it is known where)
+static int64_t wgrad_chunk(int64_t rows, int64_t tiles) { return grouped_chunk_rows(rows, tiles, 74); }
 // Chunks of the runs that are split: each has more than ks rows or is its run's last.
 static int64_t split_chunks(int64_t rows, int64_t ks, int32_t n_groups) {
   return rows <= ks ? 0 : rows / ks + std::min<int64_t>(rows / ks, n_groups);
@@ -786,13 +877,11 @@ static int launch_wgrad(const CUtensorMap& tmA, const CUtensorMap& tmB, const Wg
   constexpr int STAGES = BN == 256 ? 4 : 6;
   auto kern = grouped_wgrad_kernel<T, BN, STAGES>;
   constexpr int smem = WgradSmem<BN, STAGES>::DYNAMIC;
-  static PerDevice<cudaError_t> ready;
-  const cudaError_t* ok = ready.get(dev, [&](int) {
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  });
-  if (ok == nullptr || *ok != cudaSuccess) return MOE_B200_ERR_CUDA;
-  const int64_t n = std::min<int64_t>(max_units, sm_count(dev));
-  return launch_pdl(kern, dim3(unsigned(n)), dim3(96 + EPI_WARPS * 32), size_t(smem), st, tmA, tmB, args) ==
+  static PerDevice<int> clusters;
+  const int* resident = clusters.get(dev, [&](int d) { return pair_clusters(kern, WGRAD_THREADS, smem, d); });
+  if (resident == nullptr || *resident < 1) return MOE_B200_ERR_CUDA;
+  const int64_t n = std::min<int64_t>(max_units, *resident);
+  return launch_pdl_pairs(kern, dim3(unsigned(2 * n)), dim3(WGRAD_THREADS), size_t(smem), st, tmA, tmB, args) ==
                  cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
@@ -805,7 +894,7 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   const int dev = current_device();
   const int bn = wgrad_bn(n_dim);
   const int64_t tiles = wgrad_tiles(m_dim, n_dim);
-  const int64_t ks = grouped_chunk_rows(rows, tiles, 148);
+  const int64_t ks = wgrad_chunk(rows, tiles);
   WgradArgs p{};
   p.offsets = offsets;
   p.n_groups = n_groups;
@@ -813,7 +902,7 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   p.ks = int32_t(std::min<int64_t>(ks, INT_MAX / 2));
   p.m_dim = m_dim;
   p.n_dim = n_dim;
-  p.m_tiles = (m_dim + BM - 1) / BM;
+  p.m_tiles = (m_dim + 2 * BM - 1) / (2 * BM);
   p.n_tiles = (n_dim + bn - 1) / bn;
   p.out = dw;
   p.wide = n_dim % 16 == 0 && reinterpret_cast<uintptr_t>(dw) % 32 == 0;
@@ -823,7 +912,7 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   if (units > INT_MAX) return MOE_B200_ERR_UNSUPPORTED;
   CUtensorMap tmA, tmB;
   if (!map_mn(&tmA, a, rows, ld_a, m_dim, BM / 64, &p.a_fused) ||
-      !map_mn(&tmB, b, rows, ld_b, n_dim, bn / 64, &p.b_fused))
+      !map_mn(&tmB, b, rows, ld_b, n_dim, bn / 128, &p.b_fused))
     return MOE_B200_ERR_TMA;
   const int rc = bn == 256 ? launch_wgrad<T, 256>(tmA, tmB, p, units, dev, st)
                            : launch_wgrad<T, 128>(tmA, tmB, p, units, dev, st);
@@ -869,7 +958,7 @@ int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
 
 size_t moe_b200_grouped_wgrad_scratch_bytes(int32_t m_dim, int32_t n_dim, int64_t rows, int32_t n_groups) {
   if (m_dim < 8 || n_dim < 8 || rows < 0 || n_groups < 1) return 0;
-  const int64_t ks = grouped_chunk_rows(rows, grouped::wgrad_tiles(m_dim, n_dim), 148);
+  const int64_t ks = grouped::wgrad_chunk(rows, grouped::wgrad_tiles(m_dim, n_dim));
   return size_t(grouped::split_chunks(rows, ks, n_groups)) * size_t(m_dim) * size_t(n_dim) * sizeof(float);
 }
 

@@ -33,10 +33,10 @@ MOE_ORDER_FN TileAt tile_in_bands(int l, int m_tiles, int n_tiles, int band) {
 // still has its (zero) result stored.
 MOE_ORDER_FN int run_chunks(int rows, int ks) { return rows <= ks ? 1 : (rows + ks - 1) / ks; }
 
-// Rows per chunk for runs of `rows` rows in all whose result has `tiles` tiles each: a third of a CTA's
+// Rows per chunk for runs of `rows` rows in all whose result has `tiles` tiles each: half of a cluster's
 // share, a multiple of 64, at least 512.
-MOE_ORDER_FN int64_t grouped_chunk_rows(int64_t rows, int64_t tiles, int ctas) {
-  const int64_t share = (rows * tiles + int64_t(ctas) * 3 - 1) / (int64_t(ctas) * 3);
+MOE_ORDER_FN int64_t grouped_chunk_rows(int64_t rows, int64_t tiles, int clusters) {
+  const int64_t share = (rows * tiles + int64_t(clusters) * 2 - 1) / (int64_t(clusters) * 2);
   const int64_t ks = (share + 63) / 64 * 64;
   return ks < 512 ? 512 : ks;
 }

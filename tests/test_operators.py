@@ -78,17 +78,17 @@ def test_chunks_of_a_run(host, rows, ks, want):
 
 def test_chunk_rows_are_a_share_of_the_work(host):
     for rows, tiles in ((1, 1), (98304, 5), (32768, 256), (1 << 20, 1)):
-        ks = host.chunk_rows(rows, tiles, 148)
+        ks = host.chunk_rows(rows, tiles, 74)
         assert ks % 64 == 0 and ks >= 512
-        assert ks == 512 or (ks - 64) * 148 * 3 < rows * tiles <= ks * 148 * 3
+        assert ks == 512 or (ks - 64) * 74 * 2 < rows * tiles <= ks * 74 * 2
 
 
 def test_scratch_covers_every_split_run(lib, host):
     """Whatever the runs are, the chunks of split runs fit the scratch."""
     rng = torch.Generator().manual_seed(0)
     for rows, m, n, groups in ((98304, 576, 256, 76), (5000, 64, 64, 3), (20000, 8, 8, 1000)):
-        tiles = -(-m // 128) * -(-n // (256 if n > 128 else 128))
-        ks = host.chunk_rows(rows, tiles, 148)
+        tiles = -(-m // 256) * -(-n // (256 if n > 128 else 128))
+        ks = host.chunk_rows(rows, tiles, 74)
         have = lib.moe_b200_grouped_wgrad_scratch_bytes(m, n, rows, groups) // (m * n * 4)
         for skew in (0.0, 1.0, 20.0):
             load = torch.softmax(torch.randn(groups, generator=rng) * skew, 0)
