@@ -89,6 +89,23 @@ __device__ __forceinline__ void drain_ring(uint64_t* full_bar, uint32_t it) {
     }
 }
 
+// N chunks of 32 accumulator columns from column `col` of the result on, those that start below n_dim: each is
+// read from TMEM while the one before it is stored.
+template <int N, typename Store>
+__device__ __forceinline__ void store_columns(uint32_t taddr, int col, int n_dim, Store store) {
+  const int n = min(N, (n_dim - col + 31) / 32);
+  if (n <= 0) return;
+  float v[2][32];
+  tmem_ld32(taddr, v[0]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i >= n) break;
+    tmem_ld_wait();
+    if (i + 1 < n) tmem_ld32(taddr + (i + 1) * 32, v[(i + 1) & 1]);
+    store(col + i * 32, v[i & 1]);
+  }
+}
+
 struct RowsArgs {
   const int32_t* offsets;
   int32_t n_groups, rows;
@@ -180,9 +197,9 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
   struct Unit {
     int group, row0, left, n0;   // first row of the pair's tile, rows of the run from there on
   };
-  auto unit_of = [&](int u) {
+  auto unit_of = [&](int u, int group) {
     Unit c;
-    c.group = run_of_unit(table.first, p.n_groups, u);
+    c.group = group;
     const int start = table.start[c.group], rows = table.start[c.group + 1] - start;
     const TileAt t = tile_in_bands(u - table.first[c.group], (rows + 2 * BM - 1) / (2 * BM),
                                    p.n_chunks, BAND);
@@ -201,7 +218,7 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
     if (elect_one()) {
       uint32_t it = 0;
       for (int u = cluster; u < n_units && !*abort_flag; u += n_clusters) {
-        const Unit c = unit_of(u);
+        const Unit c = unit_of(u, run_of_unit(table.first, p.n_groups, u));
         const int own = a_bytes(c.left, int(rank));
         const uint32_t both = a_bytes(c.left, 0) + a_bytes(c.left, 1) + 2 * L::B_BYTES;
         const CUtensorMap* ma = own == A_BYTES ? &tmA : &tmShort;
@@ -279,9 +296,10 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
     constexpr int NCH = BN / 32;
     const uint32_t tempty_leader = mapa_u32(smem_u32(tempty_bar), 0);
     T* out = static_cast<T*>(p.out);
-    int j = 0;
+    int j = 0, group = 0;
     for (int u = cluster; u < n_units; u += n_clusters, ++j) {
-      const Unit c = unit_of(u);
+      group = run_of_unit_warp(table.first, p.n_groups, u, group, lane);
+      const Unit c = unit_of(u, group);
       const int b = j & 1;
       if (!mbar_wait(tfull_bar + b, (uint32_t(j) >> 1) & 1, p.status))
         atomicExch(p.status, ST_WAIT_TIMEOUT);
@@ -290,15 +308,10 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
       const int r = int(rank) * BM + row;
       T* mine = r < c.left ? out + int64_t(c.row0 + r) * p.n_dim : nullptr;
       if (__any_sync(0xffffffffu, mine != nullptr)) {
-#pragma unroll 1
-        for (int ch = half * (NCH / 2); ch < (half + 1) * (NCH / 2); ++ch) {
-          const int col = c.n0 + ch * 32;
-          if (col >= p.n_dim) break;
-          float v[32];
-          tmem_ld32(taddr + ch * 32, v);
-          tmem_ld_wait();
-          store32(mine, p.n_dim, col, p.n_dim, p.wide && col + 32 <= p.n_dim, v);
-        }
+        store_columns<NCH / 2>(taddr + half * (BN / 2), c.n0 + half * (BN / 2), p.n_dim,
+                               [&](int col, const float* v) {
+                                 store32(mine, p.n_dim, col, p.n_dim, p.wide && col + 32 <= p.n_dim, v);
+                               });
       }
       tc_fence_before();
       __syncwarp();
@@ -326,6 +339,7 @@ struct WgradArgs {
   int32_t ks;               // rows of a chunk
   int32_t m_dim, n_dim;     // one dw[g]
   int32_t m_tiles, n_tiles; // tiles of a CTA pair
+  uint32_t tiles_inv;       // (quotient)
   int32_t a_fused, b_fused; // the operand's width is a multiple of 64: one copy brings a stage of it
   void* out;                // [n_groups, m_dim, n_dim]
   int32_t wide;
@@ -345,9 +359,9 @@ struct WgradSmem {
   static constexpr int MISC = BARS + 8 * (2 * STAGES + 10);
   static constexpr int TABLE = (MISC + 16 + 15) / 16 * 16;
   static constexpr int SPLIT = TABLE + int(sizeof(RunTable));   // first chunk of every split run
-  static constexpr int LENGTHS = SPLIT + (RUNS_MAX_GROUPS + 1) * 4;
-  static constexpr int ORDER = LENGTHS + MAX_SORTED * 4;
-  static constexpr int TOTAL = ORDER + MAX_SORTED * 2;
+  static constexpr int LENGTHS = (SPLIT + (RUNS_MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
+  static constexpr int SORTED = LENGTHS + MAX_SORTED * 4;
+  static constexpr int TOTAL = SORTED + MAX_SORTED * int(sizeof(int4));
   static constexpr int DYNAMIC = TOTAL + 1024;
   static_assert(STAGE % 1024 == 0, "stages must keep the 1024-byte swizzle alignment");
   static_assert(DYNAMIC <= 232448, "more shared memory than a CTA has");
@@ -388,7 +402,7 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
   RunTable& table = *reinterpret_cast<RunTable*>(smem + L::TABLE);   // first: in chunks
   int* split_first = reinterpret_cast<int*>(smem + L::SPLIT);
   int* lengths = reinterpret_cast<int*>(smem + L::LENGTHS);
-  uint16_t* order = reinterpret_cast<uint16_t*>(smem + L::ORDER);
+  int4* sorted_chunks = reinterpret_cast<int4*>(smem + L::SORTED);   // group, first row, length, part
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -434,26 +448,34 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
                     [=](int rows) { return rows > ks ? run_chunks(rows, ks) : 0; });
   }
   __syncthreads();
-  struct Chunk {
-    int group, at, len;   // `at`: which of its run
-  };
+  // chunk i: its group, first row, length, and its place among the chunks of split runs (-1: it is its run's only
+  // one)
   auto chunk_of = [&](int i) {
-    Chunk c;
-    c.group = run_of_unit(table.first, p.n_groups, i);
-    c.at = i - table.first[c.group];
-    c.len = min(p.ks, table.start[c.group + 1] - table.start[c.group] - c.at * p.ks);
-    return c;
+    const int g = run_of_unit(table.first, p.n_groups, i), at = i - table.first[g];
+    const int start = table.start[g] + at * p.ks;
+    return make_int4(g, start, min(p.ks, table.start[g + 1] - start),
+                     split_first[g + 1] > split_first[g] ? split_first[g] + at : -1);
   };
   const int n_chunks = table.first[p.n_groups];
   const bool sorted = n_chunks <= MAX_SORTED;
   if (sorted) {
-    for (int i = threadIdx.x; i < n_chunks; i += WGRAD_THREADS) lengths[i] = chunk_of(i).len;
+    int4 mine[(MAX_SORTED + WGRAD_THREADS - 1) / WGRAD_THREADS];
+#pragma unroll
+    for (int k = 0; k < int(sizeof(mine) / sizeof(int4)); ++k) {
+      const int i = threadIdx.x + k * WGRAD_THREADS;
+      if (i < n_chunks) {
+        mine[k] = chunk_of(i);
+        lengths[i] = mine[k].z;
+      }
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < n_chunks; i += WGRAD_THREADS) {
-      const int mine = lengths[i];
+#pragma unroll
+    for (int k = 0; k < int(sizeof(mine) / sizeof(int4)); ++k) {
+      const int i = threadIdx.x + k * WGRAD_THREADS;
+      if (i >= n_chunks) break;
       int before = 0;
-      for (int j = 0; j < n_chunks; ++j) before += lengths[j] > mine || (lengths[j] == mine && j < i);
-      order[before] = uint16_t(i);
+      for (int j = 0; j < n_chunks; ++j) before += lengths[j] > mine[k].z || (lengths[j] == mine[k].z && j < i);
+      sorted_chunks[before] = mine[k];
     }
     __syncthreads();
   }
@@ -472,15 +494,15 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
       c.len = 0;
       return c;
     }
-    const int k = u / tiles;
-    const Chunk ch = chunk_of(sorted ? order[k] : k);
+    const int k = quotient(u, tiles, p.tiles_inv);
+    const int4 ch = sorted ? sorted_chunks[k] : chunk_of(k);
     const TileAt t = tile_in_bands(u - k * tiles, p.m_tiles, p.n_tiles, BAND);
-    c.group = ch.group;
-    c.row0 = table.start[ch.group] + ch.at * p.ks;
-    c.len = ch.len;
+    c.group = ch.x;
+    c.row0 = ch.y;
+    c.len = ch.z;
+    c.part = ch.w;
     c.m0 = (t.m * 2 + int(rank)) * BM;   // this CTA's rows of dw
     c.n0 = t.n * BN;
-    c.part = split_first[ch.group + 1] > split_first[ch.group] ? split_first[ch.group] + ch.at : -1;
     return c;
   };
 
@@ -656,28 +678,26 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
       const int m = c.m0 + row;
       const bool ok = m < p.m_dim;
       T* mine = ok ? out + c.group * matrix + int64_t(m) * p.n_dim : nullptr;
-      if (__any_sync(0xffffffffu, ok)) {
-#pragma unroll 1
-        for (int ch = half * (NCH / 2); ch < (half + 1) * (NCH / 2); ++ch) {
-          const int col = c.n0 + ch * 32;
-          if (col >= p.n_dim) break;
-          float v[32];
-          if (have) {
-            tmem_ld32(taddr + ch * 32, v);
-            tmem_ld_wait();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          }
-          if (c.part < 0) {
+      const int col0 = c.n0 + half * (BN / 2);
+      if (!have) {   // a run without rows: zeros, row by row
+        const int pieces = min(BN / 2, p.n_dim - col0) / 8;
+        for (int r = 0; r < 32 && c.m0 + q * 32 + r < p.m_dim; ++r) {
+          uint4* to = reinterpret_cast<uint4*>(out + c.group * matrix + int64_t(c.m0 + q * 32 + r) * p.n_dim + col0);
+          for (int i = lane; i < pieces; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+        }
+      } else if (__any_sync(0xffffffffu, ok)) {
+        if (c.part < 0) {
+          store_columns<NCH / 2>(taddr + half * (BN / 2), col0, p.n_dim, [&](int col, const float* v) {
             store32(mine, p.n_dim, col, p.n_dim, p.wide && col + 32 <= p.n_dim, v);
-          } else if (ok) {
-            float* part = p.partials + c.part * matrix + int64_t(m) * p.n_dim + col;
+          });
+        } else {
+          float* part = p.partials + c.part * matrix + int64_t(m) * p.n_dim;
+          store_columns<NCH / 2>(taddr + half * (BN / 2), col0, p.n_dim, [&](int col, const float* v) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (col + 8 * i < p.n_dim)
-                store_v8(part + 8 * i, reinterpret_cast<const uint32_t*>(v) + 8 * i);
-          }
+              if (ok && col + 8 * i < p.n_dim)
+                store_v8(part + col + 8 * i, reinterpret_cast<const uint32_t*>(v) + 8 * i);
+          });
         }
       }
       if (have) {
@@ -694,10 +714,12 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
   if (warp == 1) tmem_dealloc2(tmem_base, TMEM_COLS);
 }
 
-// dw[g] = sum of the fp32 partials of its chunks, in order, for the runs that were cut. blockIdx.y walks the
-// groups, blockIdx.x a matrix in pieces of 8 values.
+// dw[g] = sum of the fp32 partials of its chunks, in order, for the runs that were cut: the blocks share these
+// runs' matrices in pieces of 8 values per thread. (Few blocks: where no run was cut, all this takes is the
+// table, and a block per matrix and piece would take it thousands of times.)
+constexpr int JOIN_THREADS = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) wgrad_join_kernel(const WgradArgs p) {
+__global__ void __launch_bounds__(JOIN_THREADS) wgrad_join_kernel(const WgradArgs p) {
   __shared__ int start[RUNS_MAX_GROUPS + 1], split_first[RUNS_MAX_GROUPS + 1];
   pdl_trigger();
   pdl_wait();
@@ -708,23 +730,32 @@ __global__ void __launch_bounds__(256) wgrad_join_kernel(const WgradArgs p) {
                     [=](int rows) { return rows > ks ? run_chunks(rows, ks) : 0; });
   }
   __syncthreads();
+  if (split_first[p.n_groups] == 0) return;
   const int64_t matrix = int64_t(p.m_dim) * p.n_dim;
-  for (int g = blockIdx.y; g < p.n_groups; g += gridDim.y) {
-    const int n = split_first[g + 1] - split_first[g];
-    if (n == 0) continue;
-    const float* part = p.partials + split_first[g] * matrix;
-    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + g * matrix);
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < matrix / 8; i += int64_t(gridDim.x) * 256) {
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-      for (int c = 0; c < n; ++c) {
-        const float4* from = reinterpret_cast<const float4*>(part + c * matrix + i * 8);
-        const float4 x = from[0], y = from[1];
-        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-        b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
-      }
-      out[i] = make_uint4(Half16<T>::pack(a.x, a.y), Half16<T>::pack(a.z, a.w),
-                          Half16<T>::pack(b.x, b.y), Half16<T>::pack(b.z, b.w));
+  const int blocks_each = int((matrix / 8 + JOIN_THREADS - 1) / JOIN_THREADS);
+  int g = -1;
+  int64_t before = 0;   // pieces of the cut runs up to g
+  for (int64_t piece = blockIdx.x;; piece += gridDim.x) {
+    while (piece >= before) {   // the next cut run
+      do ++g;
+      while (g < p.n_groups && split_first[g + 1] == split_first[g]);
+      if (g == p.n_groups) return;
+      before += blocks_each;
     }
+    const int64_t i = (piece - (before - blocks_each)) * JOIN_THREADS + threadIdx.x;
+    if (i >= matrix / 8) continue;
+    const int n = split_first[g + 1] - split_first[g];
+    const float4* from = reinterpret_cast<const float4*>(p.partials + split_first[g] * matrix) + i * 2;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+#pragma unroll 4
+    for (int c = 0; c < n; ++c, from += matrix / 4) {
+      const float4 x = from[0], y = from[1];
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+      b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+    }
+    reinterpret_cast<uint4*>(static_cast<T*>(p.out) + g * matrix)[i] =
+        make_uint4(Half16<T>::pack(a.x, a.y), Half16<T>::pack(a.z, a.w), Half16<T>::pack(b.x, b.y),
+                   Half16<T>::pack(b.z, b.w));
   }
 }
 
@@ -904,6 +935,7 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   p.n_dim = n_dim;
   p.m_tiles = (m_dim + 2 * BM - 1) / (2 * BM);
   p.n_tiles = (n_dim + bn - 1) / bn;
+  p.tiles_inv = quotient_inverse(uint32_t(p.m_tiles * p.n_tiles));
   p.out = dw;
   p.wide = n_dim % 16 == 0 && reinterpret_cast<uintptr_t>(dw) % 32 == 0;
   p.partials = partials;
@@ -917,10 +949,8 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   const int rc = bn == 256 ? launch_wgrad<T, 256>(tmA, tmB, p, units, dev, st)
                            : launch_wgrad<T, 128>(tmA, tmB, p, units, dev, st);
   if (rc != MOE_B200_OK || rows <= p.ks) return rc;
-  const int64_t matrix = int64_t(m_dim) * n_dim;
-  const unsigned gx = unsigned(std::min<int64_t>((matrix / 8 + 255) / 256, 64));
-  return launch_pdl(wgrad_join_kernel<T>, dim3(gx, unsigned(std::min<int32_t>(n_groups, 256))), dim3(256), 0,
-                    st, p) == cudaSuccess
+  return launch_pdl(wgrad_join_kernel<T>, dim3(unsigned(sm_count(dev) * 4)), dim3(JOIN_THREADS), 0, st, p) ==
+                 cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
 }

@@ -11,6 +11,14 @@
 
 namespace moe {
 
+// x / d for 0 <= x < 2^31 with inverse = ceil(2^32 / d): a multiplication, at most one too much, put right.
+MOE_ORDER_FN uint32_t quotient_inverse(uint32_t d) { return uint32_t((0x100000000ull + d - 1) / d); }
+MOE_ORDER_FN int quotient(int x, int d, uint32_t inverse) {
+  if (d == 1) return x;
+  const int q = int(uint64_t(uint32_t(x)) * inverse >> 32);
+  return q * int64_t(d) > x ? q - 1 : q;
+}
+
 struct TileAt {
   int m, n;
 };

@@ -35,17 +35,26 @@ __device__ __forceinline__ int warp_prefix_max(int v, int lane) {   // inclusive
 // least every earlier one. True when any had to be changed (the caller reports it).
 __device__ __forceinline__ bool load_run_starts(const int32_t* offsets, int n_groups, int rows, int lane,
                                                 int* start) {
+  constexpr int AT_ONCE = 4;   // loads in flight: this is a kernel's first work
   int high = 0;
   bool changed = false;
-  for (int base = 0; base <= n_groups; base += 32) {
-    const int g = base + lane;
-    const int raw = g <= n_groups ? ld_prev(offsets + g) : 0;
-    const int v = max(high, warp_prefix_max(min(max(raw, 0), rows), lane));
-    if (g <= n_groups) {
-      start[g] = v;
-      changed |= v != raw;
+  for (int base = 0; base <= n_groups; base += 32 * AT_ONCE) {
+    int raw[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int g = base + 32 * i + lane;
+      raw[i] = g <= n_groups ? ld_prev(offsets + g) : 0;
     }
-    high = __shfl_sync(0xffffffffu, v, 31);   // (behind the last start the lanes repeat the highest)
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int g = base + 32 * i + lane;
+      const int v = max(high, warp_prefix_max(min(max(raw[i], 0), rows), lane));
+      if (g <= n_groups) {
+        start[g] = v;
+        changed |= v != raw[i];
+      }
+      high = __shfl_sync(0xffffffffu, v, 31);   // (behind the last start the lanes repeat the highest)
+    }
   }
   __syncwarp();
   return __any_sync(0xffffffffu, changed);
@@ -78,6 +87,14 @@ __device__ __forceinline__ int run_of_unit(const int* first, int n_groups, int u
     else hi = mid;
   }
   return lo;
+}
+
+// The same by a warp together, from a run at or before it on.
+__device__ __forceinline__ int run_of_unit_warp(const int* first, int n_groups, int u, int from, int lane) {
+  for (;; from += 32) {
+    const uint32_t behind = __ballot_sync(0xffffffffu, from + lane + 1 < n_groups && first[from + lane + 1] <= u);
+    if (behind != 0xffffffffu) return from + __popc(behind);
+  }
 }
 
 }  // namespace moe

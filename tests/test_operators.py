@@ -32,6 +32,7 @@ void tile(int l, int m, int n, int band, int* out) {
   const moe::TileAt t = moe::tile_in_bands(l, m, n, band);
   out[0] = t.m; out[1] = t.n;
 }
+int quotient(int x, int d) { return moe::quotient(x, d, moe::quotient_inverse(d)); }
 int chunks(int rows, int ks) { return moe::run_chunks(rows, ks); }
 long long chunk_rows(long long rows, long long tiles, int ctas) { return moe::grouped_chunk_rows(rows, tiles, ctas); }
 void philox(unsigned long long low, unsigned long long high, unsigned long long key, unsigned* w) {
@@ -68,6 +69,13 @@ def test_every_tile_is_walked_once_and_bands_stay_together(host, m, n, band):
     assert sorted(seen) == [(i, j) for i in range(m) for j in range(n)]
     bands = [i // band for i, _ in seen]
     assert bands == sorted(bands)
+
+
+def test_quotients(host):
+    for d in (1, 2, 3, 5, 7, 12, 96, 127, 1000, 65535, 1 << 20, (1 << 31) - 1):
+        for x in [0, 1, d - 1, d, 2 * d - 1, 2 * d, (1 << 31) - 1, (1 << 31) // d * d - 1, (1 << 31) // d * d]:
+            if 0 <= x < 1 << 31:
+                assert host.quotient(x, d) == x // d
 
 
 @pytest.mark.parametrize("rows,ks,want", [(0, 512, 1), (1, 512, 1), (512, 512, 1), (513, 512, 2),
