@@ -343,7 +343,8 @@ struct WgradArgs {
   int32_t a_fused, b_fused; // the operand's width is a multiple of 64: one copy brings a stage of it
   void* out;                // [n_groups, m_dim, n_dim]
   int32_t wide;
-  float* partials;          // [chunks of split runs, m_dim, n_dim]
+  float* partials;          // [chunks of split runs][tiles][2][BN / 8][128][8]: a CTA's tile, eight columns of all its
+                            // rows together (a warp's store is then 1 KB in one piece)
   int32_t* status;
 };
 
@@ -485,6 +486,7 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
   struct Unit {
     int group, row0, len, m0, n0;
     int part;   // its chunk among those of split runs, -1: the run's only one; -2: no unit in this round
+    int tile;
   };
   auto unit_of = [&](int round) {
     Unit c;
@@ -496,7 +498,8 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
     }
     const int k = quotient(u, tiles, p.tiles_inv);
     const int4 ch = sorted ? sorted_chunks[k] : chunk_of(k);
-    const TileAt t = tile_in_bands(u - k * tiles, p.m_tiles, p.n_tiles, BAND);
+    c.tile = u - k * tiles;
+    const TileAt t = tile_in_bands(c.tile, p.m_tiles, p.n_tiles, BAND);
     c.group = ch.x;
     c.row0 = ch.y;
     c.len = ch.z;
@@ -681,9 +684,13 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
       const int col0 = c.n0 + half * (BN / 2);
       if (!have) {   // a run without rows: zeros, row by row
         const int pieces = min(BN / 2, p.n_dim - col0) / 8;
-        for (int r = 0; r < 32 && c.m0 + q * 32 + r < p.m_dim; ++r) {
-          uint4* to = reinterpret_cast<uint4*>(out + c.group * matrix + int64_t(c.m0 + q * 32 + r) * p.n_dim + col0);
-          for (int i = lane; i < pieces; i += 32) to[i] = make_uint4(0, 0, 0, 0);
+        constexpr int ACROSS = BN / 16, DOWN = 32 / ACROSS;   // lanes along a row, rows at a time
+#pragma unroll 4
+        for (int r = lane / ACROSS; r < 32; r += DOWN) {
+          const int at = c.m0 + q * 32 + r;
+          if (at < p.m_dim && lane % ACROSS < pieces)
+            *reinterpret_cast<uint4*>(out + c.group * matrix + int64_t(at) * p.n_dim + col0 +
+                                      lane % ACROSS * 8) = make_uint4(0, 0, 0, 0);
         }
       } else if (__any_sync(0xffffffffu, ok)) {
         if (c.part < 0) {
@@ -691,12 +698,11 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
             store32(mine, p.n_dim, col, p.n_dim, p.wide && col + 32 <= p.n_dim, v);
           });
         } else {
-          float* part = p.partials + c.part * matrix + int64_t(m) * p.n_dim;
+          float* part = p.partials + ((int64_t(c.part) * tiles + c.tile) * 2 + rank) * (BM * BN) + row * 8;
           store_columns<NCH / 2>(taddr + half * (BN / 2), col0, p.n_dim, [&](int col, const float* v) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (ok && col + 8 * i < p.n_dim)
-                store_v8(part + col + 8 * i, reinterpret_cast<const uint32_t*>(v) + 8 * i);
+              store_v8(part + ((col - c.n0) / 8 + i) * (BM * 8), reinterpret_cast<const uint32_t*>(v) + 8 * i);
           });
         }
       }
@@ -714,25 +720,33 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
   if (warp == 1) tmem_dealloc2(tmem_base, TMEM_COLS);
 }
 
-// dw[g] = sum of the fp32 partials of its chunks, in order, for the runs that were cut: the blocks share these
-// runs' matrices in pieces of 8 values per thread. (Few blocks: where no run was cut, all this takes is the
-// table, and a block per matrix and piece would take it thousands of times.)
+// dw[g] = sum of the fp32 partials of its chunks, in order, for the runs that were cut. The blocks share these
+// runs' tiles in pieces of 128 rows x 32 columns; a warp takes 8 rows x 32 columns at a time, 256 bytes in one
+// piece of each partial and 64 of a row of dw.
 constexpr int JOIN_THREADS = 256;
-template <typename T>
+template <typename T, int BN>
 __global__ void __launch_bounds__(JOIN_THREADS) wgrad_join_kernel(const WgradArgs p) {
   __shared__ int start[RUNS_MAX_GROUPS + 1], split_first[RUNS_MAX_GROUPS + 1];
   pdl_trigger();
   pdl_wait();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x, ks = p.ks;
+  // is there a long run at all? (starts that are not in order go the long way too)
+  bool maybe = false;
+  for (int g = threadIdx.x; g < p.n_groups; g += JOIN_THREADS) {
+    const int a = ld_prev(p.offsets + g), b = ld_prev(p.offsets + g + 1);
+    maybe |= a < 0 || b < a || b > p.rows || b - a > p.ks;
+  }
+  if (!__syncthreads_or(maybe)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    const int ks = p.ks;
     load_run_starts(p.offsets, p.n_groups, p.rows, lane, start);
     count_run_units(start, p.n_groups, lane, split_first,
                     [=](int rows) { return rows > ks ? run_chunks(rows, ks) : 0; });
   }
   __syncthreads();
-  if (split_first[p.n_groups] == 0) return;
   const int64_t matrix = int64_t(p.m_dim) * p.n_dim;
-  const int blocks_each = int((matrix / 8 + JOIN_THREADS - 1) / JOIN_THREADS);
+  const int tiles = p.m_tiles * p.n_tiles;
+  const int pieces = tiles * 2 * (BN / 32);   // of a run
   int g = -1;
   int64_t before = 0;   // pieces of the cut runs up to g
   for (int64_t piece = blockIdx.x;; piece += gridDim.x) {
@@ -740,22 +754,34 @@ __global__ void __launch_bounds__(JOIN_THREADS) wgrad_join_kernel(const WgradArg
       do ++g;
       while (g < p.n_groups && split_first[g + 1] == split_first[g]);
       if (g == p.n_groups) return;
-      before += blocks_each;
+      before += pieces;
     }
-    const int64_t i = (piece - (before - blocks_each)) * JOIN_THREADS + threadIdx.x;
-    if (i >= matrix / 8) continue;
+    const int i = int(piece - (before - pieces));
+    const int chunk32 = i % (BN / 32), half_tile = i / (BN / 32);
+    const TileAt t = tile_in_bands(half_tile >> 1, p.m_tiles, p.n_tiles, BAND);
+    const int m0 = (t.m * 2 + (half_tile & 1)) * BM, col = t.n * BN + chunk32 * 32 + (lane >> 3) * 8;
+    if (m0 >= p.m_dim || col >= p.n_dim) continue;
     const int n = split_first[g + 1] - split_first[g];
-    const float4* from = reinterpret_cast<const float4*>(p.partials + split_first[g] * matrix) + i * 2;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    const int64_t step = int64_t(tiles) * 2 * (BM * BN);
+    const float* from = p.partials + split_first[g] * step + int64_t(half_tile) * (BM * BN) +
+                        (chunk32 * 4 + (lane >> 3)) * (BM * 8);
+    T* out = static_cast<T*>(p.out) + g * matrix + col;
+#pragma unroll
+    for (int h = 0; h < BM / 64; ++h) {
+      const int row = h * 64 + warp * 8 + (lane & 7);
+      if (m0 + row >= p.m_dim) break;
+      const float4* at = reinterpret_cast<const float4*>(from + row * 8);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
 #pragma unroll 4
-    for (int c = 0; c < n; ++c, from += matrix / 4) {
-      const float4 x = from[0], y = from[1];
-      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
-      b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+      for (int c = 0; c < n; ++c, at += step / 4) {
+        const float4 x = at[0], y = at[1];
+        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        b.x += y.x; b.y += y.y; b.z += y.z; b.w += y.w;
+      }
+      *reinterpret_cast<uint4*>(out + int64_t(m0 + row) * p.n_dim) =
+          make_uint4(Half16<T>::pack(a.x, a.y), Half16<T>::pack(a.z, a.w), Half16<T>::pack(b.x, b.y),
+                     Half16<T>::pack(b.z, b.w));
     }
-    reinterpret_cast<uint4*>(static_cast<T*>(p.out) + g * matrix)[i] =
-        make_uint4(Half16<T>::pack(a.x, a.y), Half16<T>::pack(a.z, a.w), Half16<T>::pack(b.x, b.y),
-                   Half16<T>::pack(b.z, b.w));
   }
 }
 
@@ -896,7 +922,9 @@ static int64_t wgrad_tiles(int32_t m_dim, int32_t n_dim) {
   return int64_t((m_dim + 2 * BM - 1) / (2 * BM)) * ((n_dim + bn - 1) / bn);
 }
 // (of every device alike: the scratch is sized before it is known where)
-static int64_t wgrad_chunk(int64_t rows, int64_t tiles) { return grouped_chunk_rows(rows, tiles, 74); }
+static int64_t wgrad_chunk(int64_t rows, int32_t n_groups, int64_t tiles) {
+  return grouped_chunk_rows(rows, n_groups, tiles, 74);
+}
 // Chunks of the runs that are split: each has more than ks rows or is its run's last.
 static int64_t split_chunks(int64_t rows, int64_t ks, int32_t n_groups) {
   return rows <= ks ? 0 : rows / ks + std::min<int64_t>(rows / ks, n_groups);
@@ -925,7 +953,7 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   const int dev = current_device();
   const int bn = wgrad_bn(n_dim);
   const int64_t tiles = wgrad_tiles(m_dim, n_dim);
-  const int64_t ks = wgrad_chunk(rows, tiles);
+  const int64_t ks = wgrad_chunk(rows, n_groups, tiles);
   WgradArgs p{};
   p.offsets = offsets;
   p.n_groups = n_groups;
@@ -949,8 +977,8 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   const int rc = bn == 256 ? launch_wgrad<T, 256>(tmA, tmB, p, units, dev, st)
                            : launch_wgrad<T, 128>(tmA, tmB, p, units, dev, st);
   if (rc != MOE_B200_OK || rows <= p.ks) return rc;
-  return launch_pdl(wgrad_join_kernel<T>, dim3(unsigned(sm_count(dev) * 4)), dim3(JOIN_THREADS), 0, st, p) ==
-                 cudaSuccess
+  auto join = bn == 256 ? wgrad_join_kernel<T, 256> : wgrad_join_kernel<T, 128>;
+  return launch_pdl(join, dim3(unsigned(sm_count(dev) * 4)), dim3(JOIN_THREADS), 0, st, p) == cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
 }
@@ -988,8 +1016,10 @@ int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
 
 size_t moe_b200_grouped_wgrad_scratch_bytes(int32_t m_dim, int32_t n_dim, int64_t rows, int32_t n_groups) {
   if (m_dim < 8 || n_dim < 8 || rows < 0 || n_groups < 1) return 0;
-  const int64_t ks = grouped::wgrad_chunk(rows, grouped::wgrad_tiles(m_dim, n_dim));
-  return size_t(grouped::split_chunks(rows, ks, n_groups)) * size_t(m_dim) * size_t(n_dim) * sizeof(float);
+  const int64_t tiles = grouped::wgrad_tiles(m_dim, n_dim);
+  const int64_t ks = grouped::wgrad_chunk(rows, n_groups, tiles);
+  return size_t(grouped::split_chunks(rows, ks, n_groups)) * size_t(tiles) * 2 * grouped::BM *
+         size_t(grouped::wgrad_bn(n_dim)) * sizeof(float);
 }
 
 int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const void* b, int64_t ld_b,

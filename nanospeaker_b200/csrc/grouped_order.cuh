@@ -41,12 +41,30 @@ MOE_ORDER_FN TileAt tile_in_bands(int l, int m_tiles, int n_tiles, int band) {
 // still has its (zero) result stored.
 MOE_ORDER_FN int run_chunks(int rows, int ks) { return rows <= ks ? 1 : (rows + ks - 1) / ks; }
 
-// Rows per chunk for runs of `rows` rows in all whose result has `tiles` tiles each: half of a cluster's
-// share, a multiple of 64, at least 512.
-MOE_ORDER_FN int64_t grouped_chunk_rows(int64_t rows, int64_t tiles, int clusters) {
-  const int64_t share = (rows * tiles + int64_t(clusters) * 2 - 1) / (int64_t(clusters) * 2);
-  const int64_t ks = (share + 63) / 64 * 64;
-  return ks < 512 ? 512 : ks;
+// Rows per chunk for n_groups runs of `rows` rows in all whose result has `tiles` tiles each. The runs being
+// alike, `n` chunks each give rounds of all clusters that take (a 64-row step 0.5 us, a tile's end 2 us, all
+// measured) some time, and cutting costs the partial tiles' way through L2 and the join: the cheapest n is
+// taken, and a quarter more rows, so that a run a little longer than the rest is not cut for it. A run that is
+// much longer than the rest is cut into pieces of two thirds of a cluster's share.
+MOE_ORDER_FN int64_t grouped_chunk_rows(int64_t rows, int32_t n_groups, int64_t tiles, int clusters) {
+  const int64_t run = (rows + n_groups - 1) / n_groups;
+  double best = 0;
+  int64_t chunks = 1;
+  for (int64_t n = 1; n <= 32; ++n) {
+    const int64_t units = n_groups * tiles * n;
+    const double rounds = double((units + clusters - 1) / clusters);
+    const double steps = double((run + n * 64 - 1) / (n * 64));
+    const double us = rounds * (steps * 0.5 + 2.0) + (n > 1 ? 5.0 + double(units) * 0.1 : 0.0);
+    if (n == 1 || us < best) {
+      best = us;
+      chunks = n;
+    }
+  }
+  const int64_t typical = run * 5 / (chunks * 4);
+  const int64_t share = rows * tiles * 2 / (int64_t(clusters) * 3);
+  const int64_t most = chunks == 1 ? (share > typical ? share : typical) : typical;
+  const int64_t ks = (most + 63) / 64 * 64;
+  return ks < 256 ? 256 : ks;
 }
 
 }  // namespace moe

@@ -34,7 +34,9 @@ void tile(int l, int m, int n, int band, int* out) {
 }
 int quotient(int x, int d) { return moe::quotient(x, d, moe::quotient_inverse(d)); }
 int chunks(int rows, int ks) { return moe::run_chunks(rows, ks); }
-long long chunk_rows(long long rows, long long tiles, int ctas) { return moe::grouped_chunk_rows(rows, tiles, ctas); }
+long long chunk_rows(long long rows, int groups, long long tiles, int clusters) {
+  return moe::grouped_chunk_rows(rows, groups, tiles, clusters);
+}
 void philox(unsigned long long low, unsigned long long high, unsigned long long key, unsigned* w) {
   const uint64_t at = low;
   moe::philox4x32<1>(&at, high, key, reinterpret_cast<uint32_t(*)[4]>(w));
@@ -51,7 +53,7 @@ unsigned threshold(double p) { return moe::dropout_threshold(p); }
                    check=True)
     lib = ctypes.CDLL(str(so))
     lib.chunk_rows.restype = ctypes.c_longlong
-    lib.chunk_rows.argtypes = [ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int]
+    lib.chunk_rows.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_longlong, ctypes.c_int]
     lib.philox.argtypes = lib.philox4.argtypes = [ctypes.c_ulonglong] * 3 + [ctypes.c_void_p]
     lib.threshold.restype = ctypes.c_uint
     lib.threshold.argtypes = [ctypes.c_double]
@@ -84,11 +86,16 @@ def test_chunks_of_a_run(host, rows, ks, want):
     assert host.chunks(rows, ks) == want
 
 
-def test_chunk_rows_are_a_share_of_the_work(host):
-    for rows, tiles in ((1, 1), (98304, 5), (32768, 256), (1 << 20, 1)):
-        ks = host.chunk_rows(rows, tiles, 74)
-        assert ks % 64 == 0 and ks >= 512
-        assert ks == 512 or (ks - 64) * 74 * 2 < rows * tiles <= ks * 74 * 2
+def test_chunk_rows(host):
+    """Runs are cut where there are too few tiles for the clusters, or where one is far longer than the
+    rest."""
+    ks = lambda rows, groups, tiles: host.chunk_rows(rows, groups, tiles, 74)  # noqa: E731
+    for rows, groups, tiles in ((1, 1, 1), (98304, 76, 3), (32768, 16, 128), (1 << 20, 1, 1), (5, 1024, 9)):
+        assert ks(rows, groups, tiles) % 64 == 0 and ks(rows, groups, tiles) >= 256
+    assert ks(98304, 76, 3) >= 2 * 98304 // 76             # many tiles: only long runs
+    assert ks(98304, 76, 3) <= 98304 * 3 // 74             # but those
+    assert ks(102400, 8, 2) <= 12800 // 3                  # sixteen tiles, 74 clusters
+    assert ks(1 << 20, 1, 1) <= (1 << 20) // 16
 
 
 def test_scratch_covers_every_split_run(lib, host):
@@ -96,8 +103,9 @@ def test_scratch_covers_every_split_run(lib, host):
     rng = torch.Generator().manual_seed(0)
     for rows, m, n, groups in ((98304, 576, 256, 76), (5000, 64, 64, 3), (20000, 8, 8, 1000)):
         tiles = -(-m // 256) * -(-n // (256 if n > 128 else 128))
-        ks = host.chunk_rows(rows, tiles, 74)
-        have = lib.moe_b200_grouped_wgrad_scratch_bytes(m, n, rows, groups) // (m * n * 4)
+        ks = host.chunk_rows(rows, groups, tiles, 74)
+        each = tiles * 256 * (256 if n > 128 else 128) * 4
+        have = lib.moe_b200_grouped_wgrad_scratch_bytes(m, n, rows, groups) // each
         for skew in (0.0, 1.0, 20.0):
             load = torch.softmax(torch.randn(groups, generator=rng) * skew, 0)
             counts = torch.bincount(torch.multinomial(load, rows, True, generator=rng), minlength=groups)
@@ -298,7 +306,7 @@ def test_entry_points_validate_before_any_launch(lib):
     assert wg(a=null) == wg(b=null) == wg(off=null) == wg(dw=null) == wg(st=null) == -2
     assert wg(a=odd) == wg(b=odd) == wg(dw=odd) == -3
     need = lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 100000, 2)
-    assert need > 0 and lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 512, 2) == 0
+    assert need > 0 and lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 256, 2) == 0
     assert wg(rows=100000) == wg(rows=100000, sc=p, nb=need - 1) == -4
     q = lambda x=p, rows=4, ld=64, k=64, lv=p, sc=p, grp=64, n=32, dt=0, y=p, st=p: \
         lib.moe_b200_int4_mm(x, rows, ld, k, lv, sc, grp, n, dt, y, st, null)  # noqa: E731
