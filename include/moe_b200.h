@@ -683,32 +683,34 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
 
 /* ---- Weights in 4 bits -----------------------------------------------------------------------------
  * W[k, n] = (level[k, n] - 8) * scale[k / group, n], level 0 .. 15, group 32, 64 or 128; the last
- * group may be short. Packed once per matrix (nanospeaker_b200/int4.py does it), the outputs in
- * strips of 16, the inputs in blocks of 64, padded with level 8:
- *   levels [strips][blocks][32 lanes][4 words]: nibble i of the low / high half of word j of lane
- *     4 * g + t is input 64 * block + 32 * (j / 2) + 8 * t + 4 * (j % 2) + 2 * (i / 2) + {0, 1},
- *     output 16 * strip + g + 8 * (i % 2)
- *   scales [strips][groups][8][2] in the activations' type: outputs g and g + 8
- * x, y, topk_w: bf16 or fp16 (dtype), k_dim a multiple of 8; fp32 sums.
+ * group may be short. Packed once per matrix (nanospeaker_b200/int4.py does it): the outputs in
+ * strips of 16, the inputs in chunks of up to 8 blocks of 64, padded with level 8. A matrix is its
+ * chunks one after another, a chunk its strips, a strip's piece of a chunk
+ *   [blocks][32 lanes][4 words], nibble i of the low / high half of word j of lane 4 * g + t being
+ *     input 64 * block + 32 * (j / 2) + 8 * t + 4 * (j % 2) + 2 * (i / 2) + {0, 1}, output
+ *     16 * strip + g + 8 * (i % 2), and behind them
+ *   [scale groups of the chunk][8][2] scales in the activations' type: outputs g and g + 8.
+ * moe_b200_int4_bytes: bytes of one matrix (a multiple of 32); 0 for a bad shape.
+ * x, y, topk_w: bf16 or fp16 (dtype), k_dim a multiple of 8; fp32 sums. Weights 16-byte aligned.
  *
  * moe_b200_int4_mm: y [rows, n_dim] = x [rows, k_dim] @ W.
  * moe_b200_int4_experts: out[t] = sum_j topk_w[t, j] * expert topk_idx[t, j] of x[t], plus the shared
  * experts of x[t]; an expert is (act(gate) * up) @ W_out with gate | up = x @ W_in, W_in
- * [d_model, 2 * d_hidden], d_hidden a multiple of 16. No dispatch comes before it. A pair whose expert
- * does not exist adds nothing and is reported through status. scratch: 16-byte aligned. Bit-
- * reproducible. */
-int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* levels,
-                     const void* scales, int32_t group, int32_t n_dim, int32_t dtype, void* y,
-                     int32_t* status, void* stream);
+ * [d_model, 2 * d_hidden], d_hidden a multiple of 16; w_in and w_out are n_experts matrices one after
+ * another, w_sh_in and w_sh_out n_shared. No dispatch comes before it. A pair whose expert does not
+ * exist adds nothing and is reported through status. scratch: 16-byte aligned. Bit-reproducible. */
+size_t moe_b200_int4_bytes(int32_t k_dim, int32_t n_dim, int32_t group);
+int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* w,
+                     int32_t group, int32_t n_dim, int32_t dtype, void* y, int32_t* status,
+                     void* stream);
 size_t moe_b200_int4_experts_scratch_bytes(int64_t n_tokens, int32_t top_k, int32_t n_shared,
                                            int32_t d_model, int32_t d_hidden);
 int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t d_model,
                           int32_t d_hidden, const void* topk_w, const int64_t* topk_idx, int32_t top_k,
-                          int32_t n_experts, const void* in_levels, const void* in_scales,
-                          const void* out_levels, const void* out_scales, int32_t n_shared,
-                          const void* sh_in_levels, const void* sh_in_scales, const void* sh_out_levels,
-                          const void* sh_out_scales, int32_t group, int32_t activation, int32_t dtype,
-                          void* out, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
+                          int32_t n_experts, const void* w_in, const void* w_out, int32_t n_shared,
+                          const void* w_sh_in, const void* w_sh_out, int32_t group, int32_t activation,
+                          int32_t dtype, void* out, void* scratch, size_t scratch_bytes, int32_t* status,
+                          void* stream);
 
 /* ---- Dropout -----------------------------------------------------------------------------------------
  * out[i] = residual[i] (0 when NULL) + (word(i) >= p * 2^32 ? x[i] / (1 - p) : 0) over n elements,

@@ -177,14 +177,15 @@ SIGNATURES = {
     "moe_b200_grouped_wgrad": (
         ctypes.c_int, [_c_vp, _c_i64, _c_i32, _c_vp, _c_i64, _c_i32, _c_i64, _c_vp, _c_i32, _c_i32,
                        _c_vp, _c_vp, _c_sz, _c_vp, _c_vp]),
+    "moe_b200_int4_bytes": (_c_sz, [_c_i32, _c_i32, _c_i32]),
     "moe_b200_int4_mm": (
-        ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_vp, _c_i32, _c_i32, _c_i32, _c_vp,
-                       _c_vp, _c_vp]),
+        ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i32, _c_vp, _c_i32, _c_i32, _c_i32, _c_vp, _c_vp,
+                       _c_vp]),
     "moe_b200_int4_experts_scratch_bytes": (_c_sz, [_c_i64, _c_i32, _c_i32, _c_i32, _c_i32]),
     "moe_b200_int4_experts": (
         ctypes.c_int, [_c_vp, _c_i64, _c_i64, _c_i32, _c_i32, _c_vp, _c_vp, _c_i32, _c_i32, _c_vp,
-                       _c_vp, _c_vp, _c_vp, _c_i32, _c_vp, _c_vp, _c_vp, _c_vp, _c_i32, _c_i32,
-                       _c_i32, _c_vp, _c_vp, _c_sz, _c_vp, _c_vp]),
+                       _c_vp, _c_i32, _c_vp, _c_vp, _c_i32, _c_i32, _c_i32, _c_vp, _c_vp, _c_sz, _c_vp,
+                       _c_vp]),
     "moe_b200_dropout": (
         ctypes.c_int, [_c_vp, _c_vp, _c_i64, _c_i32, ctypes.c_double, _c_vp, _c_vp, _c_vp, _c_vp]),
     "moe_b200_wgrad": (

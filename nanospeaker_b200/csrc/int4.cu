@@ -12,8 +12,10 @@
 // scale is applied to that sum: no rounding but the final one (and the GLU's result, which is held in the
 // activations' type between the two products).
 //
-// A strip of 16 outputs is one contiguous piece, and so is a row's share of the inputs: both come to shared
-// memory by bulk copies, which a warp of their own issues as far ahead as the ring holds.
+// A chunk of 512 inputs of neighbouring strips (16 outputs each), levels and scales together, is one contiguous
+// piece: it comes to shared memory by one bulk copy (which costs the SM's copy engine some 50 cycles however
+// small it is). The rows of x, few, in any place and read by every CTA, come by 16-byte asynchronous copies.
+// Warps of their own issue both as far ahead as the ring holds.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -29,15 +31,16 @@
 namespace moe {
 namespace q4 {
 
-constexpr int MAX_WARPS = 8;     // that multiply; one more copies
+constexpr int MAX_WARPS = 4;     // of a CTA that multiply (copy_warps more copy)
 constexpr int STRIPS = 2;        // strips of 16 outputs a warp computes
 constexpr int MAX_DEPTH = 6;     // stages of the ring
-constexpr int PAIR_WINDOW = 1024;   // pairs whose expert ids are looked at in one go
+constexpr int PAIR_WINDOW = 512;   // pairs whose expert ids are looked at in one go
 
-// One matrix stack in the packed layout.
+constexpr int CHUNK = 8;         // blocks of 64 inputs in a chunk
+
+// A stack of matrices in the packed layout (include/moe_b200.h).
 struct Stack {
-  const uint4* levels;      // [groups][strips][kblocks][32 lanes]
-  const uint32_t* scales;   // [groups][strips][kgroups][8]: outputs g and g + 8 of the strip
+  const uint8_t* data;
   int32_t groups;
 };
 
@@ -48,11 +51,14 @@ struct Args {
   int64_t ld_x;
   Stack routed, shared;
   int32_t k_dim, n_dim;        // valid inputs and outputs (GLU: outputs = the hidden width)
-  int32_t kblocks, kgroups, strips;   // of both stacks
+  int32_t kblocks, strips;     // of both stacks
   int32_t group_shift;         // scale group = 32 << group_shift inputs
+  int32_t n_stages, depth;     // chunks of a strip = stages of a pass; stages of the ring
+  int32_t full_blocks, last_blocks;   // blocks of a chunk, of the last one
+  int32_t full, last;          // bytes of a strip's piece of a chunk
+  int64_t matrix;              // bytes of a matrix
   int32_t wk, wn, kpb;         // warps that share a strip's inputs, pairs of strips per CTA, blocks of a warp
-                               // in a stage
-  int32_t n_stages, depth;     // stages of a pass, stages of the ring
+                               // in a chunk
   int32_t x_rows;              // rows of x that a stage has room for
   int32_t rows;                // DENSE: rows of x; else tokens
   // GLU / PAIRS: row p of the result is pair p of topk_idx, row n_pairs + s * rows + t token t of shared expert s
@@ -132,6 +138,11 @@ __device__ __forceinline__ float activation(int act, float g) {
   }
 }
 
+__device__ __forceinline__ uint32_t ld_shared_b32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ void compute_sync(int nthreads) {
   asm volatile("bar.sync 1, %0;" ::"r"(nthreads) : "memory");
 }
@@ -141,39 +152,43 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// A stage of the ring, `blocks` blocks of 64 inputs: per strip their levels and scales, then the rows of x (64
-// bytes behind each, so that the two rows that a quarter of a warp reads at a time lie in different banks).
+// A stage of the ring, a chunk of up to `blocks` blocks: the strips' pieces, then the rows of x. A row's 16-byte
+// piece c lies at c, in odd rows at c ^ 4: the two rows that a quarter of a warp reads at a time then lie in
+// different banks.
 struct StageShape {
-  int strip, x, row, bytes;
-  __host__ __device__ StageShape(int blocks, int strips, int rows)
-      : strip(blocks * (512 + 64)), x(strips * strip), row(blocks * 128 + 64),
-        bytes((x + rows * row + 127) / 128 * 128) {}
+  int x, row, bytes;
+  __host__ __device__ StageShape(int blocks, int strips, int piece, int rows)
+      : x((strips * piece + 127) / 128 * 128), row(blocks * 128), bytes((x + rows * row + 127) / 128 * 128) {}
 };
 
-// CTAs that an SM holds (their registers and shared memory are sized for it): few warps each and many at a
-// time, so that one CTA's start and end lie under the others' copies and the grid is one wave.
-__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
+// CTAs that an SM holds (their registers and shared memory are sized for it): many at a time, so that one's
+// start and end lie under the others' work. One row of 4096 x 16384: at 5 CTAs 15.2 us, at 4, with the
+// registers to have two blocks in the works, 12.7; 64 tokens of the experts, short strips: 19.6 at 5, 22.5 at 4.
+__host__ __device__ constexpr int ctas_per_sm(int nt, int mode) {
+  return nt == 1 ? (mode == 0 ? 4 : 5) : nt == 2 ? 3 : 2;
+}
+__host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 
 // A CTA: wn pairs of strips of one matrix (GLU: a pair is a gate strip and its up strip), wk warps on each that
-// share the inputs (a stage is a block of 64 for each) and add their sums in shared memory, and a warp that
-// copies. NT: tiles of 8 rows per pass; more rows of one expert take more passes, which copy the weights
+// share the inputs (of a chunk, kpb blocks of 64 each) and add their sums in shared memory, and warps that
+// copy. NT: tiles of 8 rows per pass; more rows of one expert take more passes, which copy the weights
 // again. FINE: scale groups of 32 inputs (two per block).
 template <typename T, int NT, bool FINE, int MODE>
-__global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_kernel(const Args p) {
+__global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm(NT, MODE)) int4_kernel(const Args p) {
   constexpr int ROWS = NT * 8, RED = ROWS + 1;   // (odd: a column of sums meets every bank)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_bar[MAX_DEPTH], empty_bar[MAX_DEPTH];
   __shared__ int list[MODE == DENSE ? 1 : PAIR_WINDOW];
-  __shared__ int warp_count[MAX_WARPS + 1];
+  __shared__ int warp_count[MAX_WARPS + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_warps = p.wk * p.wn;
-  const int span = p.wk * p.kpb;   // blocks of a stage
-  const StageShape sh(span, p.wn * STRIPS, p.x_rows);
+  constexpr int COPY_WARPS = copy_warps(NT);
+  const StageShape sh(p.full_blocks, p.wn * STRIPS, p.full, p.x_rows);
   float* red = reinterpret_cast<float*>(smem + p.depth * sh.bytes);   // [ceil(wk / 2)][wn][STRIPS * 16][RED]
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.depth; ++i) {
-      mbar_init(full_bar + i, 1);
+      mbar_init(full_bar + i, 1 + 32 * COPY_WARPS);   // the weights' bytes, and every copying lane's rows
       mbar_init(empty_bar + i, n_warps);
     }
     fence_mbar_init();
@@ -196,67 +211,64 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
     return MODE == DENSE ? r : MODE == PAIRS ? out_row(r) : all_rows ? r : list[r] / p.top_k;
   };
 
-  // ---- the copying warp's side, kept to few instructions a stage (a warp by itself takes a hundred cycles for
-  // twenty): lane i has strip i of the CTA and row i of the pass. A pass is n_stages stages, the weights the
-  // same ones in each; w_issued and x_issued count stages whose weights and rows have been asked for.
-  const bool copies = warp == n_warps;
-  const Stack w = MODE != DENSE && all_rows ? p.shared : p.routed;
-  int w_issued = 0, w_stage = 0, w_slot = 0, w_phase = 1;   // (phase: of the slot's release before)
-  int x_issued = 0, x_stage = 0, x_slot = 0;
-  bool dead = false;
-  int strip = p.strips;
-  if (copies && lane < p.wn * STRIPS) {
-    const int pair = blockIdx.x * p.wn + lane / STRIPS, s = lane % STRIPS;
-    strip = MODE == GLU ? (pair < strip_step ? pair + s * strip_step : p.strips) : pair * STRIPS + s;
-  }
-  const int live_strips = __popc(__ballot_sync(0xffffffffu, strip < p.strips));
+  // ---- the copying warps' side. A pass is n_stages stages, the weights the same ones in each; the first of
+  // them copies the weights too, w_issued and x_issued count stages whose weights and rows have been asked for.
+  const int copier = warp - n_warps;   // negative: this warp multiplies
   const uint32_t ring = smem_u32(smem);
-  const uint4* levels = w.levels + (int64_t(e) * p.strips + strip) * p.kblocks * 32;
-  const uint32_t* scales = w.scales + (int64_t(e) * p.strips + strip) * p.kgroups * 8;
-  auto groups = [&](int blocks) { return ((2 * blocks - 1) >> p.group_shift) + 1; };   // that blocks reach into
-  const int last_blocks = p.kblocks - (n_stages - 1) * span;
-  const int full_groups = groups(span), last_groups = groups(last_blocks);
-  const int last_k = p.k_dim - (n_stages - 1) * span * 64;
-  auto issue_weights = [&] {
-    if (w_issued >= p.depth) {
-      if (!mbar_wait(empty_bar + w_slot, w_phase, p.status)) dead = true;
-      dead = __any_sync(0xffffffffu, dead);
-      if (dead) return;
-    }
-    if (strip < p.strips) {
-      const bool last = w_stage == n_stages - 1;
-      const uint32_t dst = ring + w_slot * sh.bytes + lane * sh.strip;
-      bulk_load(dst, levels + int64_t(w_stage) * span * 32, (last ? last_blocks : span) * 512, full_bar + w_slot);
-      bulk_load(dst + span * 512, scales + int64_t(w_stage) * full_groups * 8, (last ? last_groups : full_groups) * 32,
-                full_bar + w_slot);
+  const int first_strip = MODE == GLU ? blockIdx.x * p.wn : blockIdx.x * p.wn * STRIPS;
+  // strips in one piece: the CTA's, or (GLU) its gate strips, with the up strips in a piece of their own
+  const int live_strips = min(MODE == GLU ? p.wn : p.wn * STRIPS, (MODE == GLU ? strip_step : p.strips) - first_strip);
+  const uint8_t* matrix = (MODE != DENSE && all_rows ? p.shared : p.routed).data + e * p.matrix;
+  int w_issued = 0, w_stage = 0, w_slot = 0;
+  int x_issued = 0, x_stage = 0, x_slot = 0, x_phase = 1;   // (phase: of the slot's release before)
+  bool dead = false;
+  auto issue_weights = [&] {   // (the slot is free)
+    const int piece = w_stage == n_stages - 1 ? p.last : p.full;
+    if (lane < (MODE == GLU ? 2 : 1)) {
+      const uint8_t* from = matrix + int64_t(w_stage) * p.strips * p.full + int64_t(first_strip + lane * strip_step) * piece;
+      bulk_load(ring + w_slot * sh.bytes + lane * p.wn * p.full, from, live_strips * piece, full_bar + w_slot);
     }
     ++w_issued;
     if (++w_stage == n_stages) w_stage = 0;
-    if (++w_slot == p.depth) {
-      w_slot = 0;
-      w_phase ^= 1;
-    }
+    if (++w_slot == p.depth) w_slot = 0;
   };
-  auto issue_rows = [&](const T* row, int rows) {   // (rows 0: the stage's weights alone)
+  // `row`: lane r's row r of x; rows 0: the stage's weights alone
+  auto issue_stage = [&](const T* row, int rows) {
+    if (x_issued >= p.depth) {
+      if (!mbar_wait(empty_bar + x_slot, x_phase, p.status)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
+      if (dead) return;
+    }
     const bool last = x_stage == n_stages - 1;
-    const uint32_t bytes = (last ? last_k : span * 64) * 2;
-    if (lane == 0)
-      mbar_expect_tx(full_bar + x_slot, live_strips * ((last ? last_blocks : span) * 512 +
-                                                       (last ? last_groups : full_groups) * 32) + rows * bytes);
-    __syncwarp();
-    if (lane < rows)
-      bulk_load(ring + x_slot * sh.bytes + sh.x + lane * sh.row, row + x_stage * span * 64, bytes,
-                full_bar + x_slot);
+    if (copier == 0) {
+      if (w_issued == x_issued) issue_weights();
+      if (lane == 0)
+        mbar_expect_tx(full_bar + x_slot, (MODE == GLU ? 2 : 1) * live_strips * (last ? p.last : p.full));
+    }
+    const int at = x_stage * p.full_blocks * 64;
+    const int pieces = min(p.full_blocks * 8, (p.k_dim - at) / 8);
+    const uint32_t to = ring + x_slot * sh.bytes + sh.x;
+    for (int r = copier; r < rows; r += COPY_WARPS) {
+      const T* from = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r)) + at;
+#pragma unroll
+      for (int h = 0; h < CHUNK * 8 / 32; ++h)
+        if (lane + 32 * h < pieces)
+          cp_async_16(to + r * sh.row + (((lane + 32 * h) ^ ((r & 1) << 2)) << 4), from + (lane + 32 * h) * 8, 16);
+    }
+    cp_async_arrive(full_bar + x_slot);
     ++x_issued;
     if (++x_stage == n_stages) x_stage = 0;
-    if (++x_slot == p.depth) x_slot = 0;
+    if (++x_slot == p.depth) {
+      x_slot = 0;
+      x_phase ^= 1;
+    }
   };
 
   // The down projection's weights and ids are older than the kernel before it, whose result (the rows of
   // x) it waits for behind this: that kernel lets this one start when it has itself waited for all before it.
   if (MODE != PAIRS) pdl_wait();
   pdl_trigger();
-  if (copies && (p.eager || all_rows))
+  if (copier == 0 && (p.eager || all_rows))
     for (int i = min(p.depth, n_stages); i > 0; --i) issue_weights();
 
   const int windows = all_rows ? 1 : (p.n_pairs + PAIR_WINDOW - 1) / PAIR_WINDOW;
@@ -267,12 +279,19 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
     if (!all_rows) {
       // the pairs of this expert among the window's, in order: every warp looks at a share of them
       const int base = win * PAIR_WINDOW, n = min(PAIR_WINDOW, p.n_pairs - base);
-      const int all = n_warps + 1;
+      const int all = n_warps + COPY_WARPS;
       const int share = ((n + all - 1) / all + 31) / 32 * 32;
       const int lo = warp * share, hi = min(n, lo + share);
+      constexpr int EACH = (PAIR_WINDOW / 2 + 31) / 32;   // (two warps at least)
+      uint32_t who[EACH];
       int count = 0;
-      for (int i = lo; i < hi; i += 32)
-        count += __popc(__ballot_sync(0xffffffffu, i + lane < hi && p.topk_idx[base + i + lane] == e));
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int at = lo + 32 * i;
+        who[i] = 0;
+        if (at < hi) who[i] = __ballot_sync(0xffffffffu, at + lane < hi && p.topk_idx[base + at + lane] == e);
+        count += __popc(who[i]);
+      }
       if (win > 0) __syncthreads();     // (the list of the window before has been used)
       if (lane == 0) warp_count[warp] = count;
       __syncthreads();
@@ -282,11 +301,10 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
         n_rows += warp_count[i];
       }
       if (count > 0) {
-        for (int i = lo; i < hi; i += 32) {
-          const bool mine = i + lane < hi && p.topk_idx[base + i + lane] == e;
-          const uint32_t who = __ballot_sync(0xffffffffu, mine);
-          if (mine) list[at + __popc(who & ((1u << lane) - 1))] = base + i + lane;
-          at += __popc(who);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          if ((who[i] >> lane) & 1) list[at + __popc(who[i] & ((1u << lane) - 1))] = base + lo + 32 * i + lane;
+          at += __popc(who[i]);
         }
       }
       __syncthreads();
@@ -296,14 +314,11 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
       pdl_wait();
       waited = true;
     }
-    if (copies) {
+    if (copier >= 0) {
       for (int r0 = first; r0 < n_rows && !dead; r0 += ROWS) {
         const int rows = min(ROWS, n_rows - r0);
         const T* row = static_cast<const T*>(p.x) + (lane < rows ? x_row(r0 + lane) * p.ld_x : 0);
-        for (int i = 0; i < n_stages && !dead; ++i) {
-          if (x_issued == w_issued) issue_weights();
-          if (!dead) issue_rows(row, rows);
-        }
+        for (int i = 0; i < n_stages && !dead; ++i) issue_stage(row, rows);
       }
       if (dead && lane == 0) atomicExch(p.status, ST_WAIT_TIMEOUT);
       continue;
@@ -320,43 +335,47 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc[s][i][k] = 0.f;
 
-      // where this lane's pieces of a stage are: levels, the rows of x (those that a tile lacks are taken from
-      // its last one: their sums are not stored)
-      const uint8_t* const q_at = smem + wn * STRIPS * sh.strip + wk * p.kpb * 512 + lane * 16;
-      const uint8_t* const s_at = smem + wn * STRIPS * sh.strip + span * 512 + g * 4;
-      const uint8_t* x_at[NT];
+      uint32_t x_at[NT];   // (rows that a tile lacks are taken from its last one: their sums are not stored)
+      uint32_t other[NT];  // from a lane's first piece of a block's row to its second
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        x_at[i] = smem + sh.x + min(i * 8 + g, p.x_rows - 1) * sh.row + wk * p.kpb * 128 + t * 16;
-      int kb = wk * p.kpb;   // this warp's block
-      for (int st = 0; st < n_stages; ++st, kb += span - p.kpb) {
+      for (int i = 0; i < NT; ++i) {
+        const int r = min(i * 8 + g, p.x_rows - 1);
+        x_at[i] = ring + sh.x + r * sh.row + wk * p.kpb * 128 + (r & 1) * 64 + t * 16 + slot * sh.bytes;
+        other[i] = (r & 1) ? uint32_t(-64) : 64u;
+      }
+      for (int st = 0; st < n_stages; ++st) {
         if (!dead && !mbar_wait(full_bar + slot, phase, p.status)) {
           dead = true;
           atomicExch(p.status, ST_WAIT_TIMEOUT);
         }
-        int off = slot * sh.bytes;
+        // this warp's blocks of the chunk, and where its strips' pieces are
+        const bool last = st == n_stages - 1;
+        const int blocks = last ? p.last_blocks : p.full_blocks, piece = last ? p.last : p.full;
+        const int lb0 = wk * p.kpb;
+        const uint32_t mine = ring + slot * sh.bytes + wn * (MODE == GLU ? 1 : STRIPS) * piece;
+        const uint32_t strip = MODE == GLU ? p.wn * p.full : piece;   // from a pair's first to its second
+        const uint32_t q_at = mine + lb0 * 512 + lane * 16, s_at = mine + blocks * 512 + g * 4;
+        int kb = st * p.full_blocks + lb0;
         // one block of 64 inputs; cut: it is the last, inputs from k_dim on were not copied and count as zero
         auto block = [&](int j, bool cut) {
           uint32_t a[STRIPS][4][4];
           uint32_t sc[STRIPS][FINE ? 2 : 1];
-          const int lb = wk * p.kpb + j;
-          const uint8_t* s_of = s_at + off + ((2 * lb) >> p.group_shift) * 32;
+          const uint32_t s_of = s_at + ((2 * (lb0 + j)) >> p.group_shift) * 32;
 #pragma unroll
           for (int s = 0; s < STRIPS; ++s) {
-            const uint4 q = *reinterpret_cast<const uint4*>(q_at + off + j * 512 + s * sh.strip);
+            uint32_t q[4];
+            ld_shared_v4(q_at + j * 512 + s * strip, q[0], q[1], q[2], q[3]);
 #pragma unroll
-            for (int h = 0; h < (FINE ? 2 : 1); ++h)
-              sc[s][h] = *reinterpret_cast<const uint32_t*>(s_of + s * sh.strip + h * 32);
-            levels_of<T>(q.x, a[s][0]);
-            levels_of<T>(q.y, a[s][1]);
-            levels_of<T>(q.z, a[s][2]);
-            levels_of<T>(q.w, a[s][3]);
+            for (int h = 0; h < (FINE ? 2 : 1); ++h) sc[s][h] = ld_shared_b32(s_of + s * strip + h * 32);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) levels_of<T>(q[k], a[s][k]);
           }
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
             if (i > 0 && i >= tiles) break;
-            uint4 b0 = *reinterpret_cast<const uint4*>(x_at[i] + off + j * 128);
-            uint4 b1 = *reinterpret_cast<const uint4*>(x_at[i] + off + j * 128 + 64);
+            uint4 b0, b1;
+            ld_shared_v4(x_at[i] + j * 128, b0.x, b0.y, b0.z, b0.w);
+            ld_shared_v4(x_at[i] + j * 128 + other[i], b1.x, b1.y, b1.z, b1.w);
             if (cut) {
               const int k = kb * 64 + t * 8;
               if (k >= p.k_dim) b0 = make_uint4(0, 0, 0, 0);
@@ -390,16 +409,22 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
             scale_in(FINE ? 1 : 0);
           }
         };
-        for (int j = 0; j < p.kpb; ++j, ++kb) {
-          if ((kb + 1) * 64 <= p.k_dim) block(j, false);
-          else if (kb < p.kblocks) block(j, true);
+        if (MODE == DENSE && p.kpb == 2 && lb0 + 2 <= blocks && (kb + 2) * 64 <= p.k_dim) {   // (long strips: two side by side)
+          block(0, false);
+          block(1, false);
+        } else {
+          for (int j = 0; j < p.kpb && lb0 + j < blocks; ++j, ++kb) block(j, (kb + 1) * 64 > p.k_dim);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty_bar + slot);
+        int by = sh.bytes;
         if (++slot == p.depth) {
           slot = 0;
           phase ^= 1;
+          by -= p.depth * sh.bytes;
         }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x_at[i] += by;
       }
 
       // The warps' sums meet in shared memory, the upper half's added to the lower half's until one is left.
@@ -451,10 +476,13 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
     }
   }
   // weights copied for rows that did not come: nobody leaves with a copy in flight
-  if (copies) {
-    while (x_issued < w_issued) {
+  __shared__ int ahead;
+  if (copier == 0 && lane == 0) ahead = w_issued;
+  __syncthreads();
+  if (copier >= 0) {
+    while (x_issued < ahead && !dead) {
       const int s = x_slot, use = x_issued / p.depth;
-      issue_rows(nullptr, 0);
+      issue_stage(nullptr, 0);
       for (int n = 0; n < 4096 && !mbar_try_wait(full_bar + s, use & 1); ++n) {
       }
     }
@@ -464,52 +492,94 @@ __global__ void __launch_bounds__((MAX_WARPS + 1) * 32, ctas_per_sm(NT)) int4_ke
 }
 
 // out[t] = sum_j topk_w[t, j] * y[t * top_k + j] + sum_s y[n_pairs + s * n_tokens + t], fp32, in that order.
-// A pair whose expert does not exist has no row: it adds nothing and is reported.
+// A pair whose expert does not exist has no row: it adds nothing and is reported. Eight pairs' ids, weights and
+// then rows are asked for at once; the first ids and weights ahead of the wait (they are older than the kernel
+// before this one, which started behind the one that waited for them).
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
     int4_sum_kernel(const float* y, const T* topk_w, const int64_t* topk_idx, int32_t n_tokens, int32_t top_k,
                     int32_t n_experts, int32_t n_shared, int32_t d, T* out, int32_t* status) {
+  constexpr int AT_ONCE = 8;
   pdl_trigger();
-  pdl_wait();
+  bool waited = false;
   const int64_t n_pairs = int64_t(n_tokens) * top_k, n4 = int64_t(n_tokens) * (d / 4);
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n4; i += int64_t(gridDim.x) * 256) {
+  for (int64_t i = int64_t(blockIdx.x) * 128 + threadIdx.x; i < n4; i += int64_t(gridDim.x) * 128) {
     const int64_t tok = i / (d / 4);
     const int c = int(i - tok * (d / 4)) * 4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = 0; j < top_k; ++j) {
-      const int64_t pair = tok * top_k + j;
-      const int64_t e = ld_prev(topk_idx + pair);
-      if (e < 0 || e >= n_experts) {
-        if (c == 0) atomicExch(status, ST_BAD_EXPERT);
-        continue;
+    auto add = [&](float w, const float4& v) {
+      a.x += w * v.x;
+      a.y += w * v.y;
+      a.z += w * v.z;
+      a.w += w * v.w;
+    };
+    for (int j0 = 0; j0 < top_k; j0 += AT_ONCE) {
+      bool there[AT_ONCE];
+      float w[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        there[j] = false;
+        if (j0 + j < top_k) {
+          const int64_t e = ld_prev(topk_idx + tok * top_k + j0 + j);
+          w[j] = Half16<T>::to_float(ld_prev(topk_w + tok * top_k + j0 + j));
+          there[j] = e >= 0 && e < n_experts;
+          if (!there[j] && c == 0) atomicExch(status, ST_BAD_EXPERT);
+        }
       }
-      const float w = Half16<T>::to_float(ld_prev(topk_w + pair));
-      const float4 v = *reinterpret_cast<const float4*>(y + pair * d + c);
-      a.x += w * v.x; a.y += w * v.y; a.z += w * v.z; a.w += w * v.w;
+      if (!waited) {
+        pdl_wait();
+        waited = true;
+      }
+      float4 v[AT_ONCE];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j)
+        if (there[j]) v[j] = *reinterpret_cast<const float4*>(y + (tok * top_k + j0 + j) * d + c);
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j)
+        if (there[j]) add(w[j], v[j]);
     }
-    for (int s = 0; s < n_shared; ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(y + (n_pairs + int64_t(s) * n_tokens + tok) * d + c);
-      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-    }
+#pragma unroll 4
+    for (int s = 0; s < n_shared; ++s)
+      add(1.f, *reinterpret_cast<const float4*>(y + (n_pairs + int64_t(s) * n_tokens + tok) * d + c));
     *reinterpret_cast<uint2*>(out + tok * d + c) =
         make_uint2(Half16<T>::pack(a.x, a.y), Half16<T>::pack(a.z, a.w));
   }
+  if (!waited) pdl_wait();
 }
 
-// How a CTA's warps divide the work: eight on a strip's inputs where it is long, else fewer on
-// more strips. A stage is a multiple of every scale group, or the whole strip.
-static void set_shape(Args& a, int32_t k_dim, int32_t n_dim, int32_t n_cols, int32_t group, bool glu) {
+static void set_shape(Args& a, int32_t k_dim, int32_t n_dim, int32_t n_cols, int32_t group) {
   a.k_dim = k_dim;
   a.n_dim = n_dim;
   a.kblocks = (k_dim + 63) / 64;
-  a.kgroups = (a.kblocks * 64 + group - 1) / group;
   a.strips = (n_cols + 15) / 16;
   a.group_shift = group == 32 ? 0 : group == 64 ? 1 : 2;
-  a.wk = a.kblocks >= 32 ? 8 : a.kblocks >= 4 ? 4 : a.kblocks >= 2 ? 2 : 1;
-  a.kpb = a.kblocks >= 16 ? 2 : 1;
+  a.n_stages = (a.kblocks + CHUNK - 1) / CHUNK;
+  a.full_blocks = std::min(CHUNK, a.kblocks);
+  a.last_blocks = a.kblocks - (a.n_stages - 1) * CHUNK;
+  auto piece = [&](int blocks) { return blocks * 512 + (((2 * blocks - 1) >> a.group_shift) + 1) * 32; };
+  a.full = piece(a.full_blocks);
+  a.last = piece(a.last_blocks);
+  a.matrix = int64_t(a.strips) * (int64_t(a.n_stages - 1) * a.full + a.last);
+}
+// How a CTA's warps divide the work: on a strip's inputs where it has that many blocks; on more strips, which
+// share the rows of x, where the grid is more than the SMs hold at a time. False: no stage fits `memory`.
+static bool set_warps(Args& a, int nt, bool glu, int64_t matrices, int slots, int memory) {
   const int pairs = glu ? a.strips / 2 : (a.strips + 1) / 2;
-  a.wn = std::min(MAX_WARPS / a.wk, pairs);
-  a.n_stages = (a.kblocks + a.wk * a.kpb - 1) / (a.wk * a.kpb);
+  for (int wk = 4; wk > 0; wk /= 2) {
+    if (wk > a.kblocks && wk > 1) continue;
+    Args b = a;
+    b.wk = wk;
+    b.kpb = (a.full_blocks + wk - 1) / wk;
+    b.wn = std::min(MAX_WARPS / wk, pairs);
+    const int red = (wk + 1) / 2 * b.wn * STRIPS * 16 * (nt * 8 + 1) * int(sizeof(float));
+    const int fit = (memory - red) / StageShape(a.full_blocks, b.wn * STRIPS, a.full, a.x_rows).bytes;
+    b.depth = std::min(std::min(fit, a.n_stages), MAX_DEPTH);
+    if (b.depth < std::min(2, a.n_stages) && a.wk > 0) break;   // (the ring of the last try is longer)
+    if (b.depth < 1) return false;
+    a = b;
+    if ((pairs + b.wn - 1) / b.wn * matrices <= slots) break;
+  }
+  return true;
 }
 static unsigned ctas_for(const Args& a, bool glu) {
   const int pairs = glu ? a.strips / 2 : (a.strips + 1) / 2;
@@ -520,22 +590,21 @@ template <typename T, int NT, bool FINE, int MODE>
 static int launch(Args a, cudaStream_t st) {
   auto kern = int4_kernel<T, NT, FINE, MODE>;
   // shared memory of a CTA: an equal share for as many as the registers allow
-  constexpr int share = 227 * 1024 / ctas_per_sm(NT) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 4 * PAIR_WINDOW) - 256;
+  constexpr int share = 227 * 1024 / ctas_per_sm(NT, MODE) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 4 * PAIR_WINDOW) - 256;
   a.x_rows = MODE == DENSE ? std::min(a.rows, NT * 8) : NT * 8;
-  const StageShape sh(a.wk * a.kpb, a.wn * STRIPS, a.x_rows);
-  const int red = (a.wk + 1) / 2 * a.wn * STRIPS * 16 * (NT * 8 + 1) * int(sizeof(float));
-  a.depth = std::max(1, std::min(std::min((share - red) / sh.bytes, a.n_stages), MAX_DEPTH));
-  const int smem = a.depth * sh.bytes + red;
+  a.row_chunks = std::max(1, (a.rows + NT * 8 - 1) / (NT * 8));
+  const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
+  if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
+  if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT, MODE), share)) return MOE_B200_ERR_UNSUPPORTED;
+  const int smem = a.depth * StageShape(a.full_blocks, a.wn * STRIPS, a.full, a.x_rows).bytes +
+                   (a.wk + 1) / 2 * a.wn * STRIPS * 16 * (NT * 8 + 1) * int(sizeof(float));
   static PerDevice<cudaError_t> ready;
   int dev = -1;
   const cudaError_t* ok = cudaGetDevice(&dev) != cudaSuccess ? nullptr : ready.get(dev, [&](int) {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, share);
   });
   if (ok == nullptr || *ok != cudaSuccess || smem > share) return MOE_B200_ERR_CUDA;
-  a.row_chunks = std::max(1, (a.rows + NT * 8 - 1) / (NT * 8));
-  const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
-  if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
-  return launch_pdl(kern, dim3(ctas_for(a, MODE == GLU), unsigned(ys)), dim3((a.wk * a.wn + 1) * 32), size_t(smem), st,
+  return launch_pdl(kern, dim3(ctas_for(a, MODE == GLU), unsigned(ys)), dim3((a.wk * a.wn + copy_warps(NT)) * 32), size_t(smem), st,
                     a) == cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
@@ -566,7 +635,7 @@ static int experts(const void* x, int64_t ld_x, int64_t n_tokens, int32_t d, int
   a.ld_x = ld_x;
   a.routed = in;
   a.shared = in_sh;
-  set_shape(a, d, h, 2 * h, group, true);
+  set_shape(a, d, h, 2 * h, group);
   a.rows = int32_t(n_tokens);
   a.topk_idx = topk_idx;
   a.n_pairs = n_pairs;
@@ -582,13 +651,13 @@ static int experts(const void* x, int64_t ld_x, int64_t n_tokens, int32_t d, int
   a.ld_x = h;
   a.routed = down;
   a.shared = down_sh;
-  set_shape(a, h, d, d, group, false);
+  set_shape(a, h, d, d, group);
   a.out = y;
   a.ld_out = d;
   rc = launch_for<T, PAIRS>(a, rows, st);
   if (rc != MOE_B200_OK) return rc;
-  const int64_t blocks = std::min<int64_t>((n_tokens * (d / 4) + 255) / 256, 148 * 8);
-  return launch_pdl(int4_sum_kernel<T>, dim3(unsigned(blocks)), dim3(256), 0, st,
+  const int64_t blocks = std::min<int64_t>((n_tokens * (d / 4) + 127) / 128, 148 * 16);
+  return launch_pdl(int4_sum_kernel<T>, dim3(unsigned(blocks)), dim3(128), 0, st,
                     static_cast<const float*>(y), static_cast<const T*>(topk_w), topk_idx, int32_t(n_tokens),
                     top_k, in.groups, in_sh.groups, d, static_cast<T*>(out), status) == cudaSuccess
              ? MOE_B200_OK
@@ -602,22 +671,27 @@ using namespace moe;
 
 extern "C" {
 
-int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* levels,
-                     const void* scales, int32_t group, int32_t n_dim, int32_t dtype, void* y, int32_t* status,
-                     void* stream) {
+size_t moe_b200_int4_bytes(int32_t k_dim, int32_t n_dim, int32_t group) {
+  if (k_dim < 8 || k_dim % 8 || n_dim < 1 || !q4::group_ok(group)) return 0;
+  q4::Args a{};
+  q4::set_shape(a, k_dim, n_dim, n_dim, group);
+  return size_t(a.matrix);
+}
+
+int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* w, int32_t group,
+                     int32_t n_dim, int32_t dtype, void* y, int32_t* status, void* stream) {
   if (rows < 0 || rows > 0x7fffffff || k_dim < 8 || k_dim % 8 || n_dim < 1 || ld_x < k_dim || ld_x % 8 ||
       !q4::group_ok(group))
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
   if (rows == 0) return MOE_B200_OK;
-  if (!x || !levels || !scales || !y || !status) return MOE_B200_ERR_NULL;
-  if (!q4::aligned(x, 16) || !q4::aligned(levels, 16) || !q4::aligned(scales, 16) || !q4::aligned(y, 2))
-    return MOE_B200_ERR_ALIGN;
+  if (!x || !w || !y || !status) return MOE_B200_ERR_NULL;
+  if (!q4::aligned(x, 16) || !q4::aligned(w, 16) || !q4::aligned(y, 2)) return MOE_B200_ERR_ALIGN;
   q4::Args a{};
   a.x = x;
   a.ld_x = ld_x;
-  a.routed = {static_cast<const uint4*>(levels), static_cast<const uint32_t*>(scales), 1};
-  q4::set_shape(a, k_dim, n_dim, n_dim, group, false);
+  a.routed = {static_cast<const uint8_t*>(w), 1};
+  q4::set_shape(a, k_dim, n_dim, n_dim, group);
   a.rows = int32_t(rows);
   a.out = y;
   a.ld_out = n_dim;
@@ -637,11 +711,9 @@ size_t moe_b200_int4_experts_scratch_bytes(int64_t n_tokens, int32_t top_k, int3
 
 int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t d_model, int32_t d_hidden,
                           const void* topk_w, const int64_t* topk_idx, int32_t top_k, int32_t n_experts,
-                          const void* in_levels, const void* in_scales, const void* out_levels,
-                          const void* out_scales, int32_t n_shared, const void* sh_in_levels,
-                          const void* sh_in_scales, const void* sh_out_levels, const void* sh_out_scales,
-                          int32_t group, int32_t activation, int32_t dtype, void* out, void* scratch,
-                          size_t scratch_bytes, int32_t* status, void* stream) {
+                          const void* w_in, const void* w_out, int32_t n_shared, const void* w_sh_in,
+                          const void* w_sh_out, int32_t group, int32_t activation, int32_t dtype, void* out,
+                          void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
   if (n_tokens < 0 || top_k < 1 || n_experts < 1 || n_shared < 0 || n_experts + int64_t(n_shared) > 65535 ||
       d_model < 8 || d_model % 8 || d_hidden < 16 || d_hidden % 16 || ld_x < d_model || ld_x % 8 ||
       !q4::group_ok(group) || n_tokens * (int64_t(top_k) + n_shared) > 0x7fffffff)
@@ -649,24 +721,18 @@ int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
   if (activation < MOE_B200_ACT_SILU || activation > MOE_B200_ACT_TANH) return MOE_B200_ERR_UNSUPPORTED;
   if (n_tokens == 0) return MOE_B200_OK;
-  if (!x || !topk_w || !topk_idx || !in_levels || !in_scales || !out_levels || !out_scales || !out || !status ||
-      (n_shared > 0 && (!sh_in_levels || !sh_in_scales || !sh_out_levels || !sh_out_scales)))
+  if (!x || !topk_w || !topk_idx || !w_in || !w_out || !out || !status || (n_shared > 0 && (!w_sh_in || !w_sh_out)))
     return MOE_B200_ERR_NULL;
-  if (!q4::aligned(x, 16) || !q4::aligned(topk_w, 2) || !q4::aligned(topk_idx, 8) ||
-      !q4::aligned(in_levels, 16) || !q4::aligned(out_levels, 16) || !q4::aligned(sh_in_levels, 16) ||
-      !q4::aligned(sh_out_levels, 16) || !q4::aligned(in_scales, 16) || !q4::aligned(out_scales, 16) ||
-      !q4::aligned(sh_in_scales, 16) || !q4::aligned(sh_out_scales, 16) || !q4::aligned(out, 16) ||
+  if (!q4::aligned(x, 16) || !q4::aligned(topk_w, 2) || !q4::aligned(topk_idx, 8) || !q4::aligned(w_in, 16) ||
+      !q4::aligned(w_out, 16) || !q4::aligned(w_sh_in, 16) || !q4::aligned(w_sh_out, 16) || !q4::aligned(out, 16) ||
       !q4::aligned(scratch, 16))
     return MOE_B200_ERR_ALIGN;
   const size_t need = moe_b200_int4_experts_scratch_bytes(n_tokens, top_k, n_shared, d_model, d_hidden);
   if (!scratch || scratch_bytes < need) return MOE_B200_ERR_SCRATCH;
   const size_t hid = (size_t(n_tokens) * size_t(top_k + n_shared) * size_t(d_hidden) * 2 + 255) / 256 * 256;
-  auto stack = [](const void* l, const void* s, int32_t n) {
-    return q4::Stack{static_cast<const uint4*>(l), static_cast<const uint32_t*>(s), n};
-  };
-  const q4::Stack in = stack(in_levels, in_scales, n_experts), down = stack(out_levels, out_scales, n_experts);
-  const q4::Stack in_sh = stack(sh_in_levels, sh_in_scales, n_shared);
-  const q4::Stack down_sh = stack(sh_out_levels, sh_out_scales, n_shared);
+  auto stack = [](const void* w, int32_t n) { return q4::Stack{static_cast<const uint8_t*>(w), n}; };
+  const q4::Stack in = stack(w_in, n_experts), down = stack(w_out, n_experts);
+  const q4::Stack in_sh = stack(w_sh_in, n_shared), down_sh = stack(w_sh_out, n_shared);
   uint8_t* s = static_cast<uint8_t*>(scratch);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == MOE_B200_BF16

@@ -898,23 +898,18 @@ OptTensor grouped_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, in
   return y;
 }
 
-bool packed_as(const Tensor& levels, const Tensor& scales, const Tensor& x) {
-  return levels.device() == x.device() && scales.device() == x.device() &&
-         scales.scalar_type() == x.scalar_type();
-}
-
-OptTensor int4_mm(const Tensor& x, const Tensor& levels, const Tensor& scales,
-                  const std::vector<int64_t>& shape, int64_t group) {
-  if (shape.size() != 2 || x.dim() < 1 || x.size(-1) != shape[0] || !x.is_cuda() || !half16(x) ||
-      !packed_as(levels, scales, x) || any_grad(x))
+OptTensor int4_mm(const Tensor& x, const Tensor& data, at::ScalarType dtype, const std::vector<int64_t>& shape,
+                  int64_t group) {
+  if (shape.size() != 2 || x.dim() < 1 || x.size(-1) != shape[0] || !x.is_cuda() || x.scalar_type() != dtype ||
+      data.device() != x.device() || any_grad(x))
     return {};
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard on(x.device());
   const Tensor flat = rows8(x.dim() == 2 ? x : x.reshape({-1, shape[0]}));
   const Tensor y = at::empty({flat.size(0), shape[1]}, x.options());
   check(abi.int4_mm(flat.const_data_ptr(), flat.size(0), row_stride(flat), int32_t(shape[0]),
-                    levels.const_data_ptr(), scales.const_data_ptr(), int32_t(group), int32_t(shape[1]),
-                    dtype_id(x.scalar_type()), y.mutable_data_ptr(), status_word(x.get_device()), current_stream()),
+                    data.const_data_ptr(), int32_t(group), int32_t(shape[1]), dtype_id(dtype),
+                    y.mutable_data_ptr(), status_word(x.get_device()), current_stream()),
         "moe_b200_int4_mm");
   n_launched += flat.size(0) > 0;
   if (x.dim() == 2) return y;
@@ -924,37 +919,30 @@ OptTensor int4_mm(const Tensor& x, const Tensor& levels, const Tensor& scales,
 }
 
 // The weights come checked against one another.
-OptTensor int4_experts(const Tensor& x_in, const Tensor& topk_w, const Tensor& topk_idx,
-                       const Tensor& in_levels, const Tensor& in_scales, const Tensor& out_levels,
-                       const Tensor& out_scales, const OptTensor& sh_in_levels, const OptTensor& sh_in_scales,
-                       const OptTensor& sh_out_levels, const OptTensor& sh_out_scales, int64_t d_model,
-                       int64_t d_hidden, int64_t group, int64_t act) {
-  const bool shared = sh_in_levels.has_value();
+OptTensor int4_experts(const Tensor& x_in, const Tensor& topk_w, const Tensor& topk_idx, const Tensor& w_in,
+                       const Tensor& w_out, const OptTensor& sh_in, const OptTensor& sh_out,
+                       at::ScalarType dtype, int64_t d_model, int64_t d_hidden, int64_t group, int64_t act) {
+  const auto device = x_in.device();
   if (x_in.dim() != 2 || topk_idx.dim() != 2 || topk_w.sizes() != topk_idx.sizes() ||
-      topk_idx.size(0) != x_in.size(0) || topk_idx.size(1) < 1 || !x_in.is_cuda() || !half16(x_in) ||
-      x_in.size(1) != d_model || topk_w.scalar_type() != x_in.scalar_type() ||
-      topk_idx.scalar_type() != at::kLong || topk_w.device() != x_in.device() ||
-      topk_idx.device() != x_in.device() || !packed_as(in_levels, in_scales, x_in) ||
-      !packed_as(out_levels, out_scales, x_in) ||
-      (shared && (!packed_as(*sh_in_levels, *sh_in_scales, x_in) ||
-                  !packed_as(*sh_out_levels, *sh_out_scales, x_in))) ||
-      any_grad(x_in, topk_w))
+      topk_idx.size(0) != x_in.size(0) || topk_idx.size(1) < 1 || !x_in.is_cuda() ||
+      x_in.scalar_type() != dtype || x_in.size(1) != d_model || topk_w.scalar_type() != dtype ||
+      topk_idx.scalar_type() != at::kLong || topk_w.device() != device || topk_idx.device() != device ||
+      w_in.device() != device || w_out.device() != device ||
+      (sh_in && (sh_in->device() != device || sh_out->device() != device)) || any_grad(x_in, topk_w))
     return {};
   at::NoGradGuard no_grad;
-  const c10::cuda::CUDAGuard on(x_in.device());
+  const c10::cuda::CUDAGuard on(device);
   const Tensor x = rows8(x_in), w = topk_w.contiguous(), idx = topk_idx.contiguous();
-  const int64_t t = x.size(0), k = idx.size(1), s = shared ? sh_in_levels->size(0) : 0;
+  const int64_t t = x.size(0), k = idx.size(1), s = sh_in ? sh_in->size(0) : 0;
   const Tensor out = at::empty({t, d_model}, x.options());
   const size_t bytes = abi.int4_experts_scratch_bytes(t, int32_t(k), int32_t(s), int32_t(d_model),
                                                       int32_t(d_hidden));
   const Tensor scratch = bytes_like(x, bytes);
-  auto of = [](const OptTensor& v) { return v ? v->const_data_ptr() : nullptr; };
   check(abi.int4_experts(x.const_data_ptr(), t, row_stride(x), int32_t(d_model), int32_t(d_hidden),
-                         w.const_data_ptr(), idx.const_data_ptr<int64_t>(), int32_t(k),
-                         int32_t(in_levels.size(0)), in_levels.const_data_ptr(), in_scales.const_data_ptr(),
-                         out_levels.const_data_ptr(), out_scales.const_data_ptr(), int32_t(s),
-                         of(sh_in_levels), of(sh_in_scales), of(sh_out_levels), of(sh_out_scales),
-                         int32_t(group), int32_t(act), dtype_id(x.scalar_type()), out.mutable_data_ptr(),
+                         w.const_data_ptr(), idx.const_data_ptr<int64_t>(), int32_t(k), int32_t(w_in.size(0)),
+                         w_in.const_data_ptr(), w_out.const_data_ptr(), int32_t(s),
+                         sh_in ? sh_in->const_data_ptr() : nullptr, sh_out ? sh_out->const_data_ptr() : nullptr,
+                         int32_t(group), int32_t(act), dtype_id(dtype), out.mutable_data_ptr(),
                          scratch.mutable_data_ptr(), bytes, status_word(x.get_device()), current_stream()),
         "moe_b200_int4_experts");
   n_launched += t > 0 ? 3 : 0;

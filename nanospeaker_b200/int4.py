@@ -17,24 +17,25 @@ from .moe_kernel import _act_id, native_ok
 
 INT4_DTYPES = (torch.bfloat16, torch.float16)
 GROUPS = (32, 64, 128)      # inputs that share a scale
+BLOCK, CHUNK, STRIP = 64, 8, 16   # inputs of a block, blocks of a chunk, outputs of a strip
 
 
 class Int4Weight:
-    """A matrix [K, N] (x @ W), or a stack [G, K, N] of them, in 4 bits, laid out as the kernels read it.
+    """A matrix [K, N] (x @ W), or a stack [G, K, N] of them, in 4 bits, laid out as the kernels read it
+    (include/moe_b200.h).
 
     shape     (K, N) or (G, K, N)
     group     inputs that share a scale: 32, 64 or 128 (the last group of a matrix may be short)
-    levels    int32 [G, ceil(N / 16), ceil(K / 64), 32, 4]
-    scales    [G, ceil(N / 16), groups, 8, 2], bf16 or fp16: the dtype of the activations"""
+    dtype     of the scales, bf16 or fp16: that of the activations
+    data      uint8 [G, bytes of a matrix]"""
 
-    def __init__(self, levels: torch.Tensor, scales: torch.Tensor, shape, group: int):
-        self.levels, self.scales, self.shape, self.group = levels, scales, tuple(shape), group
+    def __init__(self, data: torch.Tensor, shape, group: int, dtype: torch.dtype):
+        self.data, self.shape, self.group, self.dtype = data, tuple(shape), group, dtype
 
-    dtype = property(lambda self: self.scales.dtype)
-    device = property(lambda self: self.levels.device)
+    device = property(lambda self: self.data.device)
 
     def to(self, device) -> "Int4Weight":
-        return Int4Weight(self.levels.to(device), self.scales.to(device), self.shape, self.group)
+        return Int4Weight(self.data.to(device), self.shape, self.group, self.dtype)
 
     @classmethod
     def from_levels(cls, levels: torch.Tensor, scales: torch.Tensor, group: int) -> "Int4Weight":
@@ -53,38 +54,54 @@ class Int4Weight:
             raise ValueError(f"levels {tuple(levels.shape)} in groups of {group} do not take scales "
                              f"{tuple(scales.shape)}")
         q = levels.reshape(-1, k, n)
-        g, kb, ns = q.shape[0], -(-k // 64), -(-n // 16)
-        kg = -(-kb * 64 // group)
-        if (kb * 64, ns * 16) != (k, n):
-            padded = q.new_full((g, kb * 64, ns * 16), 8)
+        g, kb, ns = q.shape[0], -(-k // BLOCK), -(-n // STRIP)
+        kg = -(-kb * BLOCK // group)
+        if (kb * BLOCK, ns * STRIP) != (k, n):
+            padded = q.new_full((g, kb * BLOCK, ns * STRIP), 8)
             padded[:, :k, :n] = q
             q = padded
         # input 64 kb + 32 half + 8 t + 4 j + 2 hi + b, output 16 ns + 8 i + lane row: bit 4 (2 hi + i) + 16 b
         # of word 2 half + j of lane 4 row + t
         q = q.view(g, kb, 2, 4, 2, 2, 2, ns, 2, 8)
-        bits = torch.zeros((), dtype=torch.int32, device=q.device)
+        words = torch.zeros((), dtype=torch.int32, device=q.device)
         for hi in range(2):
             for b in range(2):
                 for i in range(2):
                     part = q[:, :, :, :, :, hi, b, :, i].to(torch.int32)
-                    bits = bits | (part << (4 * (2 * hi + i) + 16 * b))
-        # [g, kb, half, t, j, ns, row] -> [g, ns, kb, row, t, half, j]
-        packed = bits.permute(0, 5, 1, 6, 3, 2, 4).reshape(g, ns, kb, 32, 4).contiguous()
-        s = scales.new_zeros((g, kg, ns * 16))
+                    words = words | (part << (4 * (2 * hi + i) + 16 * b))
+        # [g, kb, half, t, j, ns, row] -> [g, kb, ns, row, t, half, j]
+        words = words.permute(0, 1, 5, 6, 3, 2, 4).reshape(g, kb, ns, 512 // 4)
+        s = scales.new_zeros((g, kg, ns * STRIP))
         s[:, :scales.shape[-2], :n] = scales.reshape(g, -1, n)
-        s = s.view(g, kg, ns, 2, 8).permute(0, 2, 1, 4, 3).contiguous()
-        return cls(packed, s, levels.shape, group)
+        s = s.view(g, kg, ns, 2, 8).transpose(3, 4).reshape(g, kg, ns, STRIP)
+        # chunk by chunk, strip by strip: the levels of its blocks, its scales
+        pieces = []
+        for blocks, groups in _chunks(kb, kg, group):
+            w = words[:, blocks].transpose(1, 2).reshape(g, ns, -1).view(torch.uint8)
+            c = s[:, groups].transpose(1, 2).reshape(g, ns, -1).view(torch.uint8)
+            pieces.append(torch.cat([w, c], 2).view(g, -1))
+        return cls(torch.cat(pieces, 1) if len(pieces) > 1 else pieces[0], levels.shape, group,
+                   scales.dtype)
 
     def to_levels(self):
         """(levels, scales) as from_levels takes them."""
         k, n = self.shape[-2:]
-        g, ns, kb = self.levels.shape[:3]
-        words = self.levels.view(g, ns, kb, 8, 4, 2, 2)       # row, t, half, j
-        shift = torch.arange(2, device=self.device)
-        bit = (8 * shift[:, None, None] + 16 * shift[None, :, None] + 4 * shift[None, None, :])
+        g, kb, ns = self.data.shape[0], -(-k // BLOCK), -(-n // STRIP)
+        kg = -(-kb * BLOCK // self.group)
+        words, scales, at = [], [], 0
+        for blocks, groups in _chunks(kb, kg, self.group):
+            nb, ng = blocks.stop - blocks.start, groups.stop - groups.start
+            size = nb * 512 + ng * 32
+            piece = self.data[:, at:at + ns * size].view(g, ns, size)
+            at += ns * size
+            words.append(piece[:, :, :nb * 512].contiguous().view(torch.int32).view(g, ns, nb, 8, 4, 2, 2))
+            scales.append(piece[:, :, nb * 512:].contiguous().view(self.dtype).view(g, ns, ng, 8, 2))
+        words, s = torch.cat(words, 2), torch.cat(scales, 2)     # words: row, t, half, j
+        one = torch.arange(2, device=self.device)
+        bit = 8 * one[:, None, None] + 16 * one[None, :, None] + 4 * one[None, None, :]
         q = (words[..., None, None, None] >> bit.to(torch.int32)) & 15   # hi, b, i
-        q = q.permute(0, 2, 5, 4, 6, 7, 8, 1, 9, 3).reshape(g, kb * 64, ns * 16)[:, :k, :n]
-        s = self.scales.permute(0, 2, 1, 4, 3).reshape(g, -1, ns * 16)[:, :-(-k // self.group), :n]
+        q = q.permute(0, 2, 5, 4, 6, 7, 8, 1, 9, 3).reshape(g, kb * BLOCK, ns * STRIP)[:, :k, :n]
+        s = s.permute(0, 2, 1, 4, 3).reshape(g, kg, ns * STRIP)[:, :-(-k // self.group), :n]
         return (q.to(torch.uint8).reshape(self.shape),
                 s.reshape(*self.shape[:-2], *s.shape[-2:]).contiguous())
 
@@ -93,6 +110,13 @@ class Int4Weight:
         q, s = self.to_levels()
         k = q.shape[-2]
         return (q.float() - 8) * s.float().repeat_interleave(self.group, -2)[..., :k, :]
+
+
+def _chunks(kb: int, kg: int, group: int):
+    """(blocks, scale groups) of every chunk, as slices."""
+    each = CHUNK * BLOCK // group
+    for c in range(-(-kb // CHUNK)):
+        yield (slice(c * CHUNK, min(kb, (c + 1) * CHUNK)), slice(c * each, min(kg, (c + 1) * each)))
 
 
 def _check_group(group: int) -> None:
@@ -141,14 +165,13 @@ def _check_call(x: torch.Tensor, tensors, weights) -> None:
 
 
 @torch.library.custom_op("moe_b200::int4_mm", mutates_args=())
-def _int4_mm(x: torch.Tensor, levels: torch.Tensor, scales: torch.Tensor, group: int,
-             n_dim: int) -> torch.Tensor:
+def _int4_mm(x: torch.Tensor, data: torch.Tensor, group: int, n_dim: int) -> torch.Tensor:
     with torch.cuda.device(x.device):
-        return K.int4_mm(x, levels, scales, group, n_dim)
+        return K.int4_mm(x, data, group, n_dim)
 
 
 @_int4_mm.register_fake
-def _(x, levels, scales, group, n_dim):
+def _(x, data, group, n_dim):
     return x.new_empty((x.shape[0], n_dim))
 
 
@@ -158,7 +181,7 @@ def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     Made for few rows: up to 32 read the weight once, more read it once per 32. fp32 sums, rounded
     once; bitwise reproducible."""
     if type(weight) is Int4Weight and native_ok(x):
-        out = K.shim().int4_mm(x, weight.levels, weight.scales, weight.shape, weight.group)
+        out = K.shim().int4_mm(x, weight.data, weight.dtype, weight.shape, weight.group)
         if out is not None:
             return out
     _check_types(x, weight)
@@ -166,28 +189,21 @@ def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
         raise ValueError(f"int4_mm takes x [..., K] and one matrix [K, N], got {tuple(x.shape)} and "
                          f"{weight.shape}")
     _check_call(x, (), (weight,))
-    out = _int4_mm(x.reshape(-1, x.shape[-1]), weight.levels, weight.scales, weight.group,
-                   weight.shape[1])
+    out = _int4_mm(x.reshape(-1, x.shape[-1]), weight.data, weight.group, weight.shape[1])
     return out.view(*x.shape[:-1], weight.shape[1])
 
 
 @torch.library.custom_op("moe_b200::int4_experts", mutates_args=())
-def _int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, in_levels: torch.Tensor,
-                  in_scales: torch.Tensor, out_levels: torch.Tensor, out_scales: torch.Tensor,
-                  sh_in_levels: Optional[torch.Tensor], sh_in_scales: Optional[torch.Tensor],
-                  sh_out_levels: Optional[torch.Tensor], sh_out_scales: Optional[torch.Tensor],
-                  d_hidden: int, group: int, act: int) -> torch.Tensor:
-    shared = sh_in_levels is not None
+def _int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, w_in: torch.Tensor,
+                  w_out: torch.Tensor, shared_in: Optional[torch.Tensor],
+                  shared_out: Optional[torch.Tensor], d_hidden: int, group: int, act: int) -> torch.Tensor:
     with torch.cuda.device(x.device):
-        return K.int4_experts(
-            x, topk_w.contiguous(), topk_idx.contiguous(), (in_levels, in_scales),
-            (out_levels, out_scales), (sh_in_levels, sh_in_scales) if shared else None,
-            (sh_out_levels, sh_out_scales) if shared else None, d_hidden, group, act)
+        return K.int4_experts(x, topk_w.contiguous(), topk_idx.contiguous(), w_in, w_out, shared_in,
+                              shared_out, d_hidden, group, act)
 
 
 @_int4_experts.register_fake
-def _(x, topk_w, topk_idx, in_levels, in_scales, out_levels, out_scales, sh_in_levels, sh_in_scales,
-      sh_out_levels, sh_out_scales, d_hidden, group, act):
+def _(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out, d_hidden, group, act):
     return x.new_empty(x.shape)
 
 
@@ -235,9 +251,8 @@ def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, 
     if len({w.group for w in weights}) > 1:
         raise ValueError("the experts' weights have scale groups of different sizes")
     _check_call(x, (topk_w, topk_idx), weights)
-    sh = [v for w in shared for v in (w.levels, w.scales)] or [None] * 4
-    return _int4_experts(x, topk_w, topk_idx, w_in.levels, w_in.scales, w_out.levels, w_out.scales, *sh,
-                         h, w_in.group, act)
+    sh = [w.data for w in shared] or [None] * 2
+    return _int4_experts(x, topk_w, topk_idx, w_in.data, w_out.data, *sh, h, w_in.group, act)
 
 
 def _experts_fit(w_in, w_out, shared_in, shared_out):
@@ -246,16 +261,18 @@ def _experts_fit(w_in, w_out, shared_in, shared_out):
     if type(w_in) is not Int4Weight or type(w_out) is not Int4Weight:
         return None
     (e, d, h2), (e2, h, d2) = (w.shape if len(w.shape) == 3 else (0, 0, 0) for w in (w_in, w_out))
-    if h < 16 or h % 16 or h2 != 2 * h or e2 != e or d2 != d or w_in.group != w_out.group:
+    if (h < 16 or h % 16 or h2 != 2 * h or e2 != e or d2 != d or w_in.group != w_out.group
+            or w_in.dtype != w_out.dtype):
         return None
     if shared_in is None and shared_out is None:
-        sh = (None, None, None, None)
+        sh = (None, None)
     else:
         if type(shared_in) is not Int4Weight or type(shared_out) is not Int4Weight:
             return None
         s = shared_in.shape[0]
         if (shared_in.shape != (s, d, h2) or shared_out.shape != (s, h, d)
-                or not shared_in.group == shared_out.group == w_in.group):
+                or not shared_in.group == shared_out.group == w_in.group
+                or not shared_in.dtype == shared_out.dtype == w_in.dtype):
             return None
-        sh = (shared_in.levels, shared_in.scales, shared_out.levels, shared_out.scales)
-    return (w_in.levels, w_in.scales, w_out.levels, w_out.scales, *sh, d, h, w_in.group)
+        sh = (shared_in.data, shared_out.data)
+    return (w_in.data, w_out.data, *sh, w_in.dtype, d, h, w_in.group)

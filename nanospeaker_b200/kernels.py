@@ -878,15 +878,15 @@ def grouped_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor) -> to
     return dw
 
 
-def int4_mm(x: torch.Tensor, levels, scales, group: int, n_dim: int) -> torch.Tensor:
+def int4_mm(x: torch.Tensor, data: torch.Tensor, group: int, n_dim: int) -> torch.Tensor:
     """x [R, K] times one packed 4-bit matrix -> [R, n_dim]."""
-    _need_cuda(x, levels, scales)
+    _need_cuda(x, data)
     x = _rows8(x)
     r, k = x.shape
     y = torch.empty((r, n_dim), dtype=x.dtype, device=x.device)
     _lib.check(_lib.load().moe_b200_int4_mm(
-        x.data_ptr(), r, x.stride(0) if r > 1 else k, k, levels.data_ptr(), scales.data_ptr(), group,
-        n_dim, DTYPE_IDS.get(x.dtype, -1), y.data_ptr(), status_word(x.device).data_ptr(), _stream(x)),
+        x.data_ptr(), r, x.stride(0) if r > 1 else k, k, data.data_ptr(), group, n_dim,
+        DTYPE_IDS.get(x.dtype, -1), y.data_ptr(), status_word(x.device).data_ptr(), _stream(x)),
         "moe_b200_int4_mm")
     _count(1 if r else 0)
     return y
@@ -894,23 +894,21 @@ def int4_mm(x: torch.Tensor, levels, scales, group: int, n_dim: int) -> torch.Te
 
 def int4_experts(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out, d_hidden: int, group: int,
                  act: int) -> torch.Tensor:
-    """out [T, D] of the block's experts with packed 4-bit weights; each weight a (levels, scales) pair,
-    the shared ones None without shared experts."""
-    _need_cuda(x, topk_w, topk_idx, *w_in, *w_out)
+    """out [T, D] of the block's experts with packed 4-bit weights ([E, bytes] each, the shared ones None
+    without shared experts)."""
+    _need_cuda(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out)
     x = _rows8(x)
     t, d = x.shape
-    k, e = topk_idx.shape[1], w_in[0].shape[0]
-    s = 0 if shared_in is None else shared_in[0].shape[0]
-    none = (None, None)
+    k, e = topk_idx.shape[1], w_in.shape[0]
+    s = 0 if shared_in is None else shared_in.shape[0]
     lib = _lib.load()
     out = torch.empty((t, d), dtype=x.dtype, device=x.device)
     nbytes = lib.moe_b200_int4_experts_scratch_bytes(t, k, s, d, d_hidden)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    ptrs = [_lib.ptr(v) for pair in (shared_in or none, shared_out or none) for v in pair]
     _lib.check(lib.moe_b200_int4_experts(
         x.data_ptr(), t, x.stride(0) if t > 1 else d, d, d_hidden, topk_w.data_ptr(),
-        topk_idx.data_ptr(), k, e, w_in[0].data_ptr(), w_in[1].data_ptr(), w_out[0].data_ptr(),
-        w_out[1].data_ptr(), s, *ptrs, group, act, DTYPE_IDS.get(x.dtype, -1), out.data_ptr(),
+        topk_idx.data_ptr(), k, e, w_in.data_ptr(), w_out.data_ptr(), s, _lib.ptr(shared_in),
+        _lib.ptr(shared_out), group, act, DTYPE_IDS.get(x.dtype, -1), out.data_ptr(),
         scratch.data_ptr(), nbytes, status_word(x.device).data_ptr(), _stream(x)),
         "moe_b200_int4_experts")
     _count(3 if t else 0)

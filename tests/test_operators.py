@@ -155,27 +155,48 @@ def test_packing_returns_what_was_packed(shape, group):
     w = Int4Weight.from_levels(levels, scales, group)
     back, s = w.to_levels()
     assert torch.equal(back, levels) and torch.equal(s, scales)
-    assert w.levels.dtype == torch.int32 and w.levels.is_contiguous() and w.scales.is_contiguous()
+    assert w.data.dtype == torch.uint8 and w.data.is_contiguous()
     assert w.shape == shape and w.dtype == torch.bfloat16
 
 
-def test_packed_layout_is_the_documented_one():
-    """Nibble i of half b of word j of lane 4 * row + t, written out level by level."""
+@pytest.mark.parametrize("k,group", [(128, 64), (576, 128), (640, 32), (1024, 64)])
+def test_packed_layout_is_the_documented_one(lib, k, group):
+    """Chunk by chunk, strip by strip: nibble i of half b of word j of lane 4 * row + t, then the scales."""
     from nanospeaker_b200 import Int4Weight
-    levels = torch.randint(0, 16, (128, 32), dtype=torch.uint8)
-    w = Int4Weight.from_levels(levels, torch.ones(2, 32).half(), 64)
-    words = w.levels[0].to(torch.int64) & 0xFFFFFFFF
-    for strip in range(2):
-        for kb in range(2):
-            for lane in range(32):
-                row, t = lane // 4, lane % 4
-                for j in range(4):
-                    for i in range(4):
-                        for b in range(2):
-                            k = 64 * kb + 32 * (j // 2) + 8 * t + 4 * (j % 2) + 2 * (i // 2) + b
-                            n = 16 * strip + row + 8 * (i % 2)
-                            got = (int(words[strip, kb, lane, j]) >> (4 * i + 16 * b)) & 15
-                            assert got == int(levels[k, n])
+    levels = torch.randint(0, 16, (k, 32), dtype=torch.uint8)
+    scales = torch.rand(-(-k // group), 32).half()
+    w = Int4Weight.from_levels(levels, scales, group)
+    data = bytes(w.data[0].tolist())
+    assert len(data) == lib.moe_b200_int4_bytes(k, 32, group)
+    at, kb = 0, k // 64
+    for chunk in range(0, kb, 8):
+        blocks = range(chunk, min(kb, chunk + 8))
+        groups = range(chunk * 64 // group, -(-blocks.stop * 64 // group))
+        for strip in range(2):
+            for block in blocks:
+                for lane in range(32):
+                    row, t = lane // 4, lane % 4
+                    for j in range(4):
+                        word = int.from_bytes(data[at:at + 4], "little")
+                        at += 4
+                        for i in range(4):
+                            for b in range(2):
+                                into = 64 * block + 32 * (j // 2) + 8 * t + 4 * (j % 2) + 2 * (i // 2) + b
+                                assert (word >> (4 * i + 16 * b)) & 15 == \
+                                    int(levels[into, 16 * strip + row + 8 * (i % 2)])
+            for g in groups:
+                for row in range(8):
+                    for i in range(2):
+                        v = torch.frombuffer(bytearray(data[at:at + 2]), dtype=torch.float16)
+                        at += 2
+                        assert v == scales[g, 16 * strip + row + 8 * i]
+    assert at == len(data)
+
+
+def test_packed_bytes(lib):
+    assert lib.moe_b200_int4_bytes(4096, 4096, 128) == 4096 * 4096 // 2 + 4096 * 32 * 2
+    for k, n, group in ((60, 16, 64), (64, 0, 64), (64, 16, 96), (0, 16, 32)):
+        assert lib.moe_b200_int4_bytes(k, n, group) == 0
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -308,15 +329,15 @@ def test_entry_points_validate_before_any_launch(lib):
     need = lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 100000, 2)
     assert need > 0 and lib.moe_b200_grouped_wgrad_scratch_bytes(64, 32, 256, 2) == 0
     assert wg(rows=100000) == wg(rows=100000, sc=p, nb=need - 1) == -4
-    q = lambda x=p, rows=4, ld=64, k=64, lv=p, sc=p, grp=64, n=32, dt=0, y=p, st=p: \
-        lib.moe_b200_int4_mm(x, rows, ld, k, lv, sc, grp, n, dt, y, st, null)  # noqa: E731
+    q = lambda x=p, rows=4, ld=64, k=64, w=p, grp=64, n=32, dt=0, y=p, st=p: \
+        lib.moe_b200_int4_mm(x, rows, ld, k, w, grp, n, dt, y, st, null)  # noqa: E731
     assert q(rows=0) == 0
     assert q(rows=-1) == q(k=60) == q(n=0) == q(ld=56) == q(grp=16) == q(grp=96) == q(grp=256) == -1
     assert q(dt=2) == -5
-    assert q(x=null) == q(lv=null) == q(sc=null) == q(y=null) == q(st=null) == -2
-    assert q(x=odd) == q(lv=odd) == q(sc=odd) == -3
+    assert q(x=null) == q(w=null) == q(y=null) == q(st=null) == -2
+    assert q(x=odd) == q(w=odd) == -3
     ex = lambda t=4, d=64, h=32, k=2, e=4, s=0, w=p, idx=p, grp=64, act=0, dt=0, sc=p, nb=1 << 20, sh=null, o=p: \
-        lib.moe_b200_int4_experts(p, t, d, d, h, w, idx, k, e, p, p, p, p, s, sh, sh, sh, sh, grp, act,
+        lib.moe_b200_int4_experts(p, t, d, d, h, w, idx, k, e, p, p, s, sh, sh, grp, act,
                                   dt, o, sc, nb, p, null)  # noqa: E731
     assert ex(t=0) == 0
     assert ex(t=-1) == ex(d=60) == ex(h=24) == ex(k=0) == ex(e=0) == ex(s=-1) == ex(grp=48) == -1
