@@ -34,7 +34,7 @@ namespace q4 {
 constexpr int MAX_WARPS = 4;     // of a CTA that multiply (copy_warps more copy)
 constexpr int STRIPS = 2;        // strips of 16 outputs a warp computes
 constexpr int MAX_DEPTH = 6;     // stages of the ring
-constexpr int PAIR_WINDOW = 512;   // pairs whose expert ids are looked at in one go
+constexpr int PAIR_WINDOW = 1024;   // pairs whose expert ids are looked at in one go
 
 constexpr int CHUNK = 8;         // blocks of 64 inputs in a chunk
 
@@ -457,20 +457,28 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
         each([&](float& v, int o) { to[o] = v; });
       }
       compute_sync(n_warps * 32);
+      // a thread's two neighbouring results of a row, then of the rows behind it (wn is a power of two)
       constexpr int OUT = MODE == GLU ? 16 : STRIPS * 16;   // results of a pair of strips
-      const int n_out = OUT * p.wn;
-      for (int i = threadIdx.x; i < n_out * live; i += n_warps * 32) {
-        const int r = i / n_out, c = i - r * n_out, o = c % OUT;
-        const int col = blockIdx.x * n_out + c;
-        if (col >= p.n_dim) continue;
-        const float* v = red + (c / OUT * STRIPS * 16 + o) * RED + r;
-        const int64_t to = out_row(r0 + r) * p.ld_out + col;
-        if (MODE == GLU)
-          static_cast<T*>(p.out)[to] = Half16<T>::from_float(activation(p.act, v[0]) * v[16 * RED]);
-        else if (MODE == DENSE)
-          static_cast<T*>(p.out)[to] = Half16<T>::from_float(v[0]);
-        else
-          static_cast<float*>(p.out)[to] = v[0];
+      const int n_out = OUT * p.wn, log_two = 31 - __clz(n_out / 2), rows_each = (n_warps * 32) >> log_two;
+      const int c = (threadIdx.x & (n_out / 2 - 1)) * 2, col = blockIdx.x * n_out + c;
+      const float* v = red + (c / OUT * STRIPS * 16 + c % OUT) * RED;
+      if (col < p.n_dim) {
+        for (int r = threadIdx.x >> log_two; r < live; r += rows_each) {
+          const int64_t to = out_row(r0 + r) * p.ld_out + col;
+          float a = v[r], b = v[RED + r];
+          if (MODE == GLU) {
+            a = activation(p.act, a) * v[16 * RED + r];
+            b = activation(p.act, b) * v[17 * RED + r];
+          }
+          if (MODE == PAIRS) {   // (an even number of columns, in fp32)
+            *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to) = make_float2(a, b);
+          } else if (MODE == GLU || p.n_dim % 2 == 0) {
+            *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to) = Half16<T>::pack(a, b);
+          } else {
+            static_cast<T*>(p.out)[to] = Half16<T>::from_float(a);
+            if (col + 1 < p.n_dim) static_cast<T*>(p.out)[to + 1] = Half16<T>::from_float(b);
+          }
+        }
       }
       compute_sync(n_warps * 32);
     }
@@ -570,7 +578,8 @@ static bool set_warps(Args& a, int nt, bool glu, int64_t matrices, int slots, in
     Args b = a;
     b.wk = wk;
     b.kpb = (a.full_blocks + wk - 1) / wk;
-    b.wn = std::min(MAX_WARPS / wk, pairs);
+    b.wn = MAX_WARPS / wk;
+    while (b.wn / 2 >= pairs) b.wn /= 2;
     const int red = (wk + 1) / 2 * b.wn * STRIPS * 16 * (nt * 8 + 1) * int(sizeof(float));
     const int fit = (memory - red) / StageShape(a.full_blocks, b.wn * STRIPS, a.full, a.x_rows).bytes;
     b.depth = std::min(std::min(fit, a.n_stages), MAX_DEPTH);
@@ -686,7 +695,7 @@ int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, c
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
   if (rows == 0) return MOE_B200_OK;
   if (!x || !w || !y || !status) return MOE_B200_ERR_NULL;
-  if (!q4::aligned(x, 16) || !q4::aligned(w, 16) || !q4::aligned(y, 2)) return MOE_B200_ERR_ALIGN;
+  if (!q4::aligned(x, 16) || !q4::aligned(w, 16) || !q4::aligned(y, n_dim % 2 ? 2 : 4)) return MOE_B200_ERR_ALIGN;
   q4::Args a{};
   a.x = x;
   a.ld_x = ld_x;
