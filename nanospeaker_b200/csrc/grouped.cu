@@ -173,16 +173,7 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc2(tmem_slot, TMEM_COLS);
-    tmem_relinquish2();
-    pdl_trigger();
-  }
-  tc_fence_before();
-  cluster_sync_all();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  pdl_wait();
+  const uint32_t tmem_base = pair_start(tmem_slot, TMEM_COLS, warp);
 
   if (warp == 2) {
     const bool bad = load_run_starts(p.offsets, p.n_groups, p.rows, lane, table.start);
@@ -428,16 +419,7 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc2(tmem_slot, TMEM_COLS);
-    tmem_relinquish2();
-    pdl_trigger();
-  }
-  tc_fence_before();
-  cluster_sync_all();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  pdl_wait();
+  const uint32_t tmem_base = pair_start(tmem_slot, TMEM_COLS, warp);
 
   const int tiles = p.m_tiles * p.n_tiles;
   if (warp == 2) {

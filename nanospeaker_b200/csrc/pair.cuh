@@ -1,6 +1,7 @@
 // What kernels on CTA pairs (a cluster of two, tcgen05 cta_group::2) share: the pair's ranks and
 // addresses, TMEM held by both, MMAs issued by the leader for both, loads that signal the leader.
 #pragma once
+#include "pdl.cuh"
 #include "ptx.cuh"
 
 namespace moe {
@@ -96,6 +97,22 @@ __device__ __forceinline__ void tma_load_4d_2cta(void* dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar) & PEER_BIT_MASK), "r"(c0), "r"(c1),
       "r"(c2), "r"(c3)
       : "memory");
+}
+
+// How a kernel of pairs begins, behind the initialisation of its barriers: both CTAs take their TMEM (warp 1 holds
+// it), let the next kernel in, meet, and wait for the kernels before them. Returns the accumulators' address.
+__device__ __forceinline__ uint32_t pair_start(uint32_t* tmem_slot, uint32_t ncols, int warp) {
+  if (warp == 1) {
+    tmem_alloc2(tmem_slot, ncols);
+    tmem_relinquish2();
+    pdl_trigger();
+  }
+  tc_fence_before();
+  cluster_sync_all();     // both CTAs' barriers are initialised and both have their TMEM
+  tc_fence_after();
+  const uint32_t base = *tmem_slot;
+  pdl_wait();
+  return base;
 }
 
 }  // namespace moe

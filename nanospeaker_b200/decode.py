@@ -19,11 +19,17 @@ class StackedMoEDecoder:
     """`x + block(x)` over a list of MoE blocks (eval mode, CUDA, bf16), graph-replayed per batch
     size.
 
+    weights="int4" holds the experts' weights (not the router's) in 4 bits with a scale per `group`
+    inputs, a quarter of the bytes; they are rounded once, on the first step (`requantize` after the
+    blocks' weights have changed). Then blocks of any width that is a multiple of 16 and bf16 or fp16
+    activations are taken, without biases or a capacity, four launches a layer (`int4_experts`).
+
     step(x) runs the stack on x [T, d_model] and returns the result (a tensor owned by the runner:
     it is overwritten by the next step with the same T). The first call for a given T captures the
     graph; later calls copy x into the graph's input and replay."""
 
-    def __init__(self, blocks: Sequence[MoEBlock], combine: str = "store"):
+    def __init__(self, blocks: Sequence[MoEBlock], combine: str = "store", weights: str = "16bit",
+                 group: int = 64):
         # "store": per-pair rows summed in fp32 in pair order, so a replay reproduces the eager
         # stack bit for bit and a token's routing further down the stack cannot flip from run to
         # run; at decode sizes the separate combine launch costs next to nothing. "atomic" is the
@@ -32,6 +38,16 @@ class StackedMoEDecoder:
         self.blocks: List[MoEBlock] = list(blocks)
         if not self.blocks:
             raise ValueError("need at least one block")
+        if weights not in ("16bit", "int4"):
+            raise ValueError(f"weights are held in \"16bit\" or \"int4\", got {weights!r}")
+        if weights == "int4":
+            for b in self.blocks:
+                if (b._kernel_act is None or b.b_in is not None or b.b_sh_in is not None
+                        or b._capacity_setting not in (None, "auto") or b.d_hidden % 16 or b.d_model % 8):
+                    raise ValueError("4-bit experts: a named activation, no biases, no capacity, a width "
+                                     "that is a multiple of 16")
+        self.weights, self.group = weights, group
+        self._int4 = {}
         for b in self.blocks:
             b.eval()
         self._graphs = {}
@@ -92,6 +108,29 @@ class StackedMoEDecoder:
             return None
         return plan
 
+    def requantize(self) -> None:
+        """Round the experts' weights again on the next step (they have changed)."""
+        self._int4.clear()
+        self._graphs.clear()
+
+    def _int4_args(self, b: MoEBlock, x: torch.Tensor):
+        """(w_in, w_out, shared_in, shared_out) of a block in 4 bits for x's dtype, made on first use."""
+        from .int4 import quantize_int4
+        key = (id(b), x.dtype, x.device)
+        if key not in self._int4:
+            pack = lambda w: (None if w is None else  # noqa: E731
+                              quantize_int4(w.detach().to(x.device), self.group, x.dtype))
+            self._int4[key] = tuple(pack(w) for w in (b.W_in, b.W_out, b.W_sh_in, b.W_sh_out))
+        return self._int4[key]
+
+    def _eager_int4(self, x: torch.Tensor) -> torch.Tensor:
+        from .int4 import int4_experts
+        for b in self.blocks:
+            topk_w, topk_idx, _ = b.router(x)
+            w_in, w_out, sh_in, sh_out = self._int4_args(b, x)
+            x = x + int4_experts(x, topk_w, topk_idx, w_in, w_out, b._kernel_act, sh_in, sh_out)
+        return x
+
     @torch.no_grad()
     def eager(self, x: torch.Tensor) -> torch.Tensor:
         """x <- x + block(x) through the stack: one persistent kernel for blocks of one shape and up
@@ -102,6 +141,8 @@ class StackedMoEDecoder:
         from . import kernels as K
         from . import moe_kernel as MK
         x = x.contiguous()
+        if self.weights == "int4":
+            return self._eager_int4(x)
         plan = self._stack_plan(x) if x.dim() == 2 and MK._ONE_CALL else None
         if plan is not None:
             return K.stack_infer(plan[0], len(self.blocks), x, *plan[2])

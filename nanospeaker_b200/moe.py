@@ -15,7 +15,10 @@ Paths, in the order `forward` tries them:
                failing library raises; nothing is silently rerouted. An explicit capacity_factor
                (the reference's padded path, src/model/moe.py:225-283) runs on the same kernels:
                the dispatch drops the pairs over capacity instead of padding a batch.
-  2. torch     the per-expert loop in plain torch (src/model/moe.py:377-418) for everything the
+  2. grouped   with `block.grouped = True`, CUDA blocks of widths (or in fp16) that the kernels of 1.
+               decline: the experts' products as `grouped_mm` over the sorted pairs, dropless unless a
+               capacity is given; gather, GLU and sum are torch's. No host sync.
+  3. torch     the per-expert loop in plain torch (src/model/moe.py:377-418) for everything the
                kernels decline (CPU, fp32/fp64, custom activations), with or without a capacity.
 """
 import math
@@ -25,6 +28,7 @@ from torch import nn
 
 from . import moe_kernel as MK
 from .glu import glu_hidden_dim, make_glu
+from .grouped import GROUPED_DTYPES, MAX_GROUPS, grouped_mm
 from .moe_kernel import (KERNEL_ACTIVATIONS, fused_moe_block, fused_moe_forward,
                          kernel_supported)
 from .router import TopKRouter
@@ -70,6 +74,9 @@ class MoEBlock(nn.Module):
         # how the kernel path sums a token's per-pair rows: None = the library default
         # (moe_kernel.get_combine_mode()), or "atomic" / "store" for this block
         self.combine_mode = None
+        # Blocks that the kernels decline for their width or dtype run their experts' products as
+        # grouped_mm where this is set (off: the torch loop, as before it existed).
+        self.grouped = False
         # a registered name bound to its registered function, and known to the epilogues
         named = ACTIVATIONS.get(self.activation) is act_fn and self.activation in KERNEL_ACTIVATIONS
         self._kernel_act = self.activation if named else None
@@ -111,7 +118,7 @@ class MoEBlock(nn.Module):
         (src/model/moe.py:189-206)."""
         if self._capacity_setting != "auto":
             return self._capacity_setting
-        return None if self._kernel_ready() else AUTO_CAPACITY
+        return None if self._kernel_ready() or self._grouped_ok(self.W_in) else AUTO_CAPACITY
 
     def _use_kernel(self, x: torch.Tensor) -> bool:
         """The dropless kernel path (the gate of src/model/moe.py:331-343)."""
@@ -126,6 +133,11 @@ class MoEBlock(nn.Module):
         """Can x go to the forms without biases or a capacity: the whole-block op of traced calls, the
         graph pair, the decode stack?"""
         return self._use_kernel(x) and self.b_in is None and self.b_sh_in is None
+
+    def _grouped_ok(self, t: torch.Tensor) -> bool:
+        """Do the experts of tensors like t go through grouped_mm?"""
+        return (self.grouped and t.is_cuda and t.dtype in GROUPED_DTYPES and self.d_model % 8 == 0
+                and self.d_hidden % 8 == 0 and self.n_experts <= MAX_GROUPS)
 
     # ---------------------------------------------------------------------------- bookkeeping
     def _record(self, probs, counts, x):
@@ -193,6 +205,31 @@ class MoEBlock(nn.Module):
             out.index_add_(0, rows, y * pair_w[lo:lo + n, None])
         return out, counts
 
+    def _grouped_experts(self, x, topk_w, topk_idx, cap: int):
+        """The routed experts as two grouped products over the sorted pairs. Pairs over a capacity are
+        multiplied with the rest and left out of the sum. A token's rows are summed in fp32
+        in pair order: reproducible bit for bit."""
+        experts, order, token_idx, counts = self._plan(topk_idx)
+        offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+        at = torch.arange(order.numel(), device=x.device)
+        kept = None
+        if cap:
+            kept = torch.empty_like(at, dtype=torch.bool).index_copy_(0, order, at - offsets[experts] < cap)
+            self.dropped = (~kept).sum().detach()
+        offsets = offsets.to(torch.int32)
+        a = grouped_mm(x[token_idx], self.W_in.to(x.dtype), offsets)
+        if self.b_in is not None:
+            a = a + self.b_in.float()[experts].to(x.dtype)   # (its gradient is then summed in fp32)
+        gate, up = a.chunk(2, dim=-1)
+        y = grouped_mm(self.glu(gate, up), self.W_out.to(x.dtype), offsets)
+        if self.b_out is not None:
+            y = y + self.b_out.float()[experts].to(x.dtype)
+        rows = y[torch.empty_like(order).index_copy_(0, order, at)].view(*topk_idx.shape, self.d_model)
+        rows = rows.float() * topk_w[..., None].float()
+        if kept is not None:
+            rows = torch.where(kept.view(*topk_idx.shape, 1), rows, 0.0)
+        return rows.sum(1).to(x.dtype), counts
+
     # ------------------------------------------------------------------------------ forward
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1] != self.d_model:
@@ -255,7 +292,8 @@ class MoEBlock(nn.Module):
                 self.dropped = (counts - cap).clamp(min=0).sum().detach().long()
             return out.view(shape)
 
-        out, counts = self._torch_experts(x, topk_w, topk_idx, cap)
+        experts = self._grouped_experts if self._grouped_ok(x) else self._torch_experts
+        out, counts = experts(x, topk_w, topk_idx, cap)
         self._record(probs, counts, x)
         if self.n_shared:
             out = out + self._shared(x)

@@ -18,6 +18,7 @@ import torch.nn.functional as F
 
 from . import kernels as K
 from . import moe_kernel as MK
+from .dropout import DROPOUT_DTYPES, dropout_add
 from .moe import MoEBlock
 
 
@@ -71,12 +72,20 @@ class _FFNSublayerFn(torch.autograd.Function):
 
 class MoEFFNSublayer(nn.Module):
     """`x + ffn(norm_ffn(x))`, returning (out, aux_loss) like the tail of the reference's
-    Block.forward. `norm_gamma` is RMSNorm's scale (src/model/ln.py:29), `ffn` a MoEBlock."""
+    Block.forward. `norm_gamma` is RMSNorm's scale (src/model/ln.py:29), `ffn` a MoEBlock.
 
-    def __init__(self, ffn: MoEBlock, epsilon: float = 1e-6):
+    dropout: share of the block's output that is dropped in training mode before the residual is added,
+    `x + dropout(ffn(norm_ffn(x)))`. On the GPU the mask's state is drawn from torch's generator of the
+    device at every forward, so torch.manual_seed, activation checkpointing and graph replays treat it as
+    they treat torch's own dropout. (0, the default, keeps the fused node.)"""
+
+    def __init__(self, ffn: MoEBlock, epsilon: float = 1e-6, dropout: float = 0.0):
         super().__init__()
+        if not 0 <= dropout < 1:
+            raise ValueError(f"dropout ({dropout}) has to be in [0, 1).")
         self.ffn = ffn
         self.epsilon = epsilon
+        self.dropout = dropout
         self.norm_gamma = nn.Parameter(torch.ones(ffn.d_model))
 
     def _fused_ok(self, x: torch.Tensor) -> bool:
@@ -85,7 +94,19 @@ class MoEFFNSublayer(nn.Module):
         return (f._whole_block_ok(x) and not (f.training and f.router.noise_std)
                 and f.d_model % 8 == 0 and f.d_model <= 2048)
 
+    def _with_dropout(self, x: torch.Tensor):
+        """x + dropout(ffn(norm(x))): the residual is added where the mask is made."""
+        y = self.ffn(F.rms_norm(x, (x.shape[-1],), self.norm_gamma.to(x.dtype), self.epsilon))
+        if x.is_cuda and x.dtype in DROPOUT_DTYPES:
+            rng = torch.empty(2, dtype=torch.int64, device=x.device).random_()
+            out = dropout_add(y, x, self.dropout, rng)
+        else:
+            out = x + F.dropout(y, self.dropout)
+        return out, self.ffn.aux_loss
+
     def forward(self, x: torch.Tensor):
+        if self.training and self.dropout:
+            return self._with_dropout(x)
         shape = x.shape
         x2 = x if x.dim() == 2 else x.reshape(-1, shape[-1])
         f = self.ffn

@@ -2,6 +2,7 @@
 generator compiled for the host, the packed layout, and what is refused before anything is launched."""
 import ctypes
 import os
+import re
 import subprocess
 
 import pytest
@@ -111,6 +112,21 @@ def test_scratch_covers_every_split_run(lib, host):
             counts = torch.bincount(torch.multinomial(load, rows, True, generator=rng), minlength=groups)
             need = sum(host.chunks(int(c), ks) for c in counts if c > ks)
             assert need <= have
+
+
+def test_pair_kernels_begin_in_the_one_place():
+    """A kernel of CTA pairs lets the next one in when it holds its TMEM and reads nothing before its wait: the
+    order stands in pair_start, and the kernels here begin with it and nothing else of it."""
+    code = lambda f: re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, f)).read())  # noqa: E731
+    body = code("pair.cuh").split("pair_start(")[1].split("\n}\n")[0]
+    assert re.findall(r"\b(tmem_alloc|tmem_relinquish|pdl_trigger|cluster_sync_all|pdl_wait)2?\(", body) == [
+        "tmem_alloc", "tmem_relinquish", "pdl_trigger", "cluster_sync_all", "pdl_wait"]
+    kernels = [k.split("\n}\n")[0] for k in code("grouped.cu").split("__global__")[1:]]
+    pairs = [k for k in kernels if "tmem_dealloc2" in k]
+    assert len(pairs) == 2
+    for k in pairs:
+        assert k.count("pair_start(") == 1 and not re.search(r"tmem_alloc|pdl_trigger|pdl_wait", k)
+        assert "p.offsets" not in k.split("pair_start(")[0]
 
 
 # ------------------------------------------------------------------------------------ generator
