@@ -869,9 +869,10 @@ static int rows_product(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
   const int dev = current_device();
   // pairs of row tiles: at most one partly filled per run
   const int64_t pairs = std::min<int64_t>(rows, rows / (2 * BM) + n_groups);
-  // The wide tile reads less per product (measured in the comment at the kernel); the narrow one where the
-  // wide one would leave clusters without work.
-  const bool wide_tile = n_dim > 128 && pairs * ((n_dim + 255) / 256) >= sm_count(dev) / 2;
+  // The wide tile loads less per product (1293 rows x 76, 256 -> 576: 46 us against the narrow one's 57); the
+  // narrow one where the wide one would leave a quarter of the clusters without work (100 rows x 8, 1024 -> 1024:
+  // 7.5 us against 9.6; at 64 tiles for 74 clusters, 2048^3, the wide one's 15.3 against 17.5).
+  const bool wide_tile = n_dim > 128 && pairs * ((n_dim + 255) / 256) * 8 >= sm_count(dev) * 3;
   const int bn = wide_tile ? 256 : 128;
   RowsArgs a{};
   a.offsets = offsets;
