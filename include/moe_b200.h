@@ -693,7 +693,8 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
  * moe_b200_int4_bytes: bytes of one matrix (a multiple of 32); 0 for a bad shape.
  * x, y, topk_w: bf16 or fp16 (dtype), k_dim a multiple of 8; fp32 sums. Weights 16-byte aligned.
  *
- * moe_b200_int4_mm: y [rows, n_dim] = x [rows, k_dim] @ W.
+ * moe_b200_int4_mm: y [rows, n_dim] = x [rows, k_dim] @ W; up to 65535 * 8 rows (32 rows read the
+ * weight once).
  * moe_b200_int4_experts: out[t] = sum_j topk_w[t, j] * expert topk_idx[t, j] of x[t], plus the shared
  * experts of x[t]; an expert is (act(gate) * up) @ W_out with gate | up = x @ W_in, W_in
  * [d_model, 2 * d_hidden], d_hidden a multiple of 16; w_in and w_out are n_experts matrices one after

@@ -125,11 +125,15 @@ class StackedMoEDecoder:
 
     def _eager_int4(self, x: torch.Tensor) -> torch.Tensor:
         from .int4 import int4_experts
+        shape = x.shape
+        x = x.reshape(-1, shape[-1])
+        if x.shape[0] == 0:
+            return x.clone().view(shape)
         for b in self.blocks:
             topk_w, topk_idx, _ = b.router(x)
             w_in, w_out, sh_in, sh_out = self._int4_args(b, x)
             x = x + int4_experts(x, topk_w, topk_idx, w_in, w_out, b._kernel_act, sh_in, sh_out)
-        return x
+        return x.view(shape)
 
     @torch.no_grad()
     def eager(self, x: torch.Tensor) -> torch.Tensor:

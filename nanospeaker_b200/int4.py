@@ -126,7 +126,7 @@ def _check_group(group: int) -> None:
 
 def quantize_int4(w: torch.Tensor, group: int = 64, dtype: Optional[torch.dtype] = None) -> Int4Weight:
     """w [K, N] or [G, K, N] rounded to 4 bits: a group's scale is its largest magnitude / 7, in `dtype`
-    (default: w's, bf16 for fp32), its levels the nearest ones. Non-finite weights raise."""
+    (default: w's, bf16 for fp32), its levels the nearest ones. Weights that are not finite, or too large for the scales, raise."""
     dtype = dtype or (w.dtype if w.dtype in INT4_DTYPES else torch.bfloat16)
     if w.dim() not in (2, 3):
         raise ValueError(f"a weight is [K, N] or [G, K, N], got {tuple(w.shape)}")
@@ -141,6 +141,8 @@ def quantize_int4(w: torch.Tensor, group: int = 64, dtype: Optional[torch.dtype]
     padded = torch.nn.functional.pad(w, (0, 0, 0, groups * group - k))
     blocks = padded.view(*w.shape[:-2], groups, group, n)
     scales = (blocks.abs().amax(-2) / 7).to(dtype)
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError(f"weights too large for scales in {dtype}")
     s = scales.float().unsqueeze(-2)
     levels = torch.where(s > 0, blocks / s, 0.0).round().clamp(-8, 7) + 8
     levels = levels.to(torch.uint8).view(*w.shape[:-2], groups * group, n)[..., :k, :].contiguous()

@@ -560,3 +560,100 @@ def test_dropout_graph_replays_move_on():
         assert torch.equal(out, dropout_add(x, None, 0.5, torch.tensor([9, call], device="cuda")))
         seen.append(out.clone())
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+# ------------------------------------------------------------------------------ traced and captured
+def test_registered_ops_check_out():
+    """Schemas, fake kernels and autograd of the ops that traced calls see."""
+    off, r = runs([20, 0, 13])
+    ops = torch.ops.moe_b200
+    check = lambda op, args: torch.library.opcheck(  # noqa: E731
+        op, args, test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
+    x, w = randn(r, 64).requires_grad_(), randn(3, 64, 72, seed=1).requires_grad_()
+    check(ops.grouped_mm, (x, w, off))
+    check(ops.grouped_wgrad, (x.detach(), randn(r, 72), off))
+    rng = torch.tensor([1, 2], device="cuda")
+    check(ops.dropout_add, (x, randn(r, 64, seed=2).requires_grad_(), 0.3, rng))
+    check(ops.dropout_bwd, (x, 0.3, rng))
+    q = quantize_int4(randn(64, 40))
+    check(ops.int4_mm, (x.detach(), q.data, q.group, 40))
+    xx, tw, idx, p, _ = experts_case(6, 64, 16, 4, 2, 1, 64, torch.bfloat16)
+    check(ops.int4_experts, (xx, tw, idx, p["w_in"].data, p["w_out"].data, p["shared_in"].data,
+                             p["shared_out"].data, 16, 64, 0))
+
+
+def test_registered_ops_give_what_the_eager_calls_give():
+    """The two ways into the same kernels, gradients included."""
+    off, r = runs([20, 0, 13])
+    rng = torch.tensor([1, 2], device="cuda")
+    res = randn(r, 72, seed=4)
+    for layout in (lambda w: w, lambda w: w.transpose(1, 2).contiguous().transpose(1, 2)):
+        both = []
+        for mm, drop in ((grouped_mm, dropout_add),
+                         (torch.ops.moe_b200.grouped_mm, lambda *a: torch.ops.moe_b200.dropout_add(*a)[0])):
+            x, w = randn(r, 64).requires_grad_(), layout(randn(3, 64, 72, seed=1)).requires_grad_()
+            b = res.clone().requires_grad_()
+            out = drop(mm(x, w, off), b, 0.25, rng)
+            both.append((out.detach(), *torch.autograd.grad(out, (x, w, b), randn(r, 72, seed=2))))
+        assert all(torch.equal(a, b) for a, b in zip(*both))
+    q = quantize_int4(randn(64, 40))
+    assert torch.equal(int4_mm(x.detach(), q), torch.ops.moe_b200.int4_mm(x.detach(), q.data, q.group, 40))
+
+
+def test_second_gradients_of_grouped_products_are_refused():
+    off, r = runs([20, 13])
+    x, w = randn(r, 64).requires_grad_(), randn(2, 64, 72, seed=1).requires_grad_()
+    dx, = torch.autograd.grad(grouped_mm(x, w, off), x, randn(r, 72, seed=2), create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        dx.sum().backward()
+
+
+def test_training_step_in_a_graph():
+    """Forward and gradients captured and replayed on new inputs. (No eager graph of the same leaves may be
+    alive meanwhile: torch's engine then joins the leaves' stream to the capture, with any op, and the capture
+    fails with an error.)"""
+    off, r = runs([100, 0, 57])
+    x, w = randn(r, 64).requires_grad_(), randn(3, 64, 72, seed=1).requires_grad_()
+    dy, rng = randn(r, 72, seed=2), torch.tensor([3, 0], device="cuda")
+    step = lambda: torch.autograd.grad(dropout_add(grouped_mm(x, w, off), None, 0.5, rng), (x, w), dy)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        x.copy_(randn(r, 64, seed=7))
+        rng[1] = 5
+    graph.replay()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+
+
+def test_graphs_of_two_calls_share_nothing():
+    """Two captured graphs of split weight gradients and of experts, replayed in turn and at once on two
+    streams."""
+    off, r = runs([3000, 10])
+    x, y = randn(r, 64), randn(r, 40, seed=2)
+    e = experts_case(16, 64, 32, 8, 2, 1, 64, torch.bfloat16)
+    run = lambda: (kernels.grouped_wgrad(x, y, off),  # noqa: E731
+                   int4_experts(e[0], e[1], e[2], e[3]["w_in"], e[3]["w_out"], "silu", e[3]["shared_in"],
+                                e[3]["shared_out"]))
+    want = run()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run()
+        graphs.append((g, out))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -239,6 +239,14 @@ def test_quantising_zeros_and_what_is_not_finite():
             quantize_int4(w)
 
 
+def test_scales_that_overflow_are_refused():
+    from nanospeaker_b200 import quantize_int4
+    w = torch.full((64, 16), 1e6)
+    with pytest.raises(ValueError, match="too large"):
+        quantize_int4(w, 64, torch.float16)
+    assert torch.allclose(quantize_int4(w, 64, torch.bfloat16).dequantize(), w, rtol=2.0 ** -7)
+
+
 def test_weight_refusals():
     from nanospeaker_b200 import Int4Weight, quantize_int4
     q, s = torch.zeros(64, 16, dtype=torch.uint8), torch.ones(1, 16).half()
