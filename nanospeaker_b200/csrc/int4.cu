@@ -128,7 +128,8 @@ __device__ __forceinline__ void levels_of(uint32_t word, uint32_t* a) {
   }
 }
 
-__device__ __forceinline__ float activation(int act, float g) {
+// (Called, not copied to every place: these kernels are over before much code has been fetched.)
+__device__ __noinline__ float activation(int act, float g) {
   switch (act) {
     case ACT_SILU: return act_f<ACT_SILU>(g);
     case ACT_GELU: return act_f<ACT_GELU>(g);
@@ -162,11 +163,9 @@ struct StageShape {
 };
 
 // CTAs that an SM holds (their registers and shared memory are sized for it): many at a time, so that one's
-// start and end lie under the others' work. One row of 4096 x 16384: at 5 CTAs 15.2 us, at 4, with the
-// registers to have two blocks in the works, 12.7; 64 tokens of the experts, short strips: 19.6 at 5, 22.5 at 4.
-__host__ __device__ constexpr int ctas_per_sm(int nt, int mode) {
-  return nt == 1 ? (mode == 0 ? 4 : 5) : nt == 2 ? 3 : 2;
-}
+// start and end lie under the others' work, but with the registers for two blocks in the works. One row of 4096 x
+// 16384: at 5 CTAs 15.2 us, at 4 12.5; one token of the experts 11.2 and 10.2.
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
 __host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 
 // A CTA: wn pairs of strips of one matrix (GLU: a pair is a gate strip and its up strip), wk warps on each that
@@ -174,17 +173,18 @@ __host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 // copy. NT: tiles of 8 rows per pass; more rows of one expert take more passes, which copy the weights
 // again. FINE: scale groups of 32 inputs (two per block).
 template <typename T, int NT, bool FINE, int MODE>
-__global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm(NT, MODE)) int4_kernel(const Args p) {
-  constexpr int ROWS = NT * 8, RED = ROWS + 1;   // (odd: a column of sums meets every bank)
+__global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm(NT)) int4_kernel(const Args p) {
+  constexpr int ROWS = NT * 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_bar[MAX_DEPTH], empty_bar[MAX_DEPTH];
   __shared__ int list[MODE == DENSE ? 1 : PAIR_WINDOW];
+  __shared__ uint32_t found[MODE == DENSE ? 1 : PAIR_WINDOW / 32];
   __shared__ int warp_count[MAX_WARPS + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_warps = p.wk * p.wn;
   constexpr int COPY_WARPS = copy_warps(NT);
   const StageShape sh(p.full_blocks, p.wn * STRIPS, p.full, p.x_rows);
-  float* red = reinterpret_cast<float*>(smem + p.depth * sh.bytes);   // [ceil(wk / 2)][wn][STRIPS * 16][RED]
+  float4* red = reinterpret_cast<float4*>(smem + p.depth * sh.bytes);   // [wk / 2][wn][STRIPS * NT][32 lanes]
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.depth; ++i) {
@@ -282,29 +282,27 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
       const int all = n_warps + COPY_WARPS;
       const int share = ((n + all - 1) / all + 31) / 32 * 32;
       const int lo = warp * share, hi = min(n, lo + share);
-      constexpr int EACH = (PAIR_WINDOW / 2 + 31) / 32;   // (two warps at least)
-      uint32_t who[EACH];
       int count = 0;
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int at = lo + 32 * i;
-        who[i] = 0;
-        if (at < hi) who[i] = __ballot_sync(0xffffffffu, at + lane < hi && p.topk_idx[base + at + lane] == e);
-        count += __popc(who[i]);
+#pragma unroll 4
+      for (int at = lo; at < hi; at += 32) {
+        const uint32_t who = __ballot_sync(0xffffffffu, at + lane < hi && p.topk_idx[base + at + lane] == e);
+        if (lane == 0) found[at >> 5] = who;
+        count += __popc(who);
       }
       if (win > 0) __syncthreads();     // (the list of the window before has been used)
       if (lane == 0) warp_count[warp] = count;
       __syncthreads();
-      int at = 0;
+      int before = 0;
       for (int i = 0; i < all; ++i) {
-        at += i < warp ? warp_count[i] : 0;
+        before += i < warp ? warp_count[i] : 0;
         n_rows += warp_count[i];
       }
       if (count > 0) {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          if ((who[i] >> lane) & 1) list[at + __popc(who[i] & ((1u << lane) - 1))] = base + lo + 32 * i + lane;
-          at += __popc(who[i]);
+#pragma unroll 1
+        for (int at = lo; at < hi; at += 32) {
+          const uint32_t who = found[at >> 5];
+          if ((who >> lane) & 1) list[before + __popc(who & ((1u << lane) - 1))] = base + at + lane;
+          before += __popc(who);
         }
       }
       __syncthreads();
@@ -427,71 +425,91 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
         for (int i = 0; i < NT; ++i) x_at[i] += by;
       }
 
-      // The warps' sums meet in shared memory, the upper half's added to the lower half's until one is left.
-      auto red_at = [&](int k) { return red + ((k * p.wn + wn) * STRIPS * 16 + g) * RED + 2 * t; };
-      auto each = [&](auto f) {
+      // The warps' sums meet in shared memory, the upper half's added to the lower half's until one is left (wk is a
+      // power of two). A lane adds what the same lane of another warp has: any order of the values will do.
+      float4* mine4 = red + wn * (STRIPS * NT * 32) + lane;
+      for (int half = p.wk >> 1; half > 0; half >>= 1) {
+        float4* at4 = mine4 + (wk & (half - 1)) * p.wn * (STRIPS * NT * 32);
+        if (wk >= half && wk < 2 * half) {
 #pragma unroll
-        for (int s = 0; s < STRIPS; ++s)
+          for (int s = 0; s < STRIPS; ++s)
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f(acc[s][i][k], (s * 16 + (k >> 1) * 8) * RED + i * 8 + (k & 1));
-      };
-      int n = p.wk;
-      while (n > 1) {
-        const int half = (n + 1) >> 1;
-        if (wk >= half && wk < n) {
-          float* to = red_at(wk - half);
-          each([&](float& v, int o) { to[o] = v; });
+            for (int i = 0; i < NT; ++i)
+              at4[(s * NT + i) * 32] = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
         }
         compute_sync(n_warps * 32);
-        if (wk < n - half) {
-          const float* from = red_at(wk);
-          each([&](float& v, int o) { v += from[o]; });
+        if (wk < half) {
+#pragma unroll
+          for (int s = 0; s < STRIPS; ++s)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              const float4 v = at4[(s * NT + i) * 32];
+              acc[s][i][0] += v.x;
+              acc[s][i][1] += v.y;
+              acc[s][i][2] += v.z;
+              acc[s][i][3] += v.w;
+            }
         }
         compute_sync(n_warps * 32);
-        n = half;
       }
-      if (wk == 0) {
-        float* to = red_at(0);
-        each([&](float& v, int o) { to[o] = v; });
-      }
-      compute_sync(n_warps * 32);
-      // a thread's two neighbouring results of a row, then of the rows behind it (wn is a power of two)
-      constexpr int OUT = MODE == GLU ? 16 : STRIPS * 16;   // results of a pair of strips
-      const int n_out = OUT * p.wn, log_two = 31 - __clz(n_out / 2), rows_each = (n_warps * 32) >> log_two;
-      const int c = (threadIdx.x & (n_out / 2 - 1)) * 2, col = blockIdx.x * n_out + c;
-      const float* v = red + (c / OUT * STRIPS * 16 + c % OUT) * RED;
-      if (col < p.n_dim) {
-        for (int r = threadIdx.x >> log_two; r < live; r += rows_each) {
-          const int64_t to = out_row(r0 + r) * p.ld_out + col;
-          float a = v[r], b = v[RED + r];
-          if (MODE == GLU) {
-            a = activation(p.act, a) * v[16 * RED + r];
-            b = activation(p.act, b) * v[17 * RED + r];
-          }
-          if (MODE == PAIRS) {   // (an even number of columns, in fp32)
-            *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to) = make_float2(a, b);
-          } else if (MODE == GLU || p.n_dim % 2 == 0) {
-            *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to) = Half16<T>::pack(a, b);
-          } else {
-            static_cast<T*>(p.out)[to] = Half16<T>::from_float(a);
-            if (col + 1 < p.n_dim) static_cast<T*>(p.out)[to + 1] = Half16<T>::from_float(b);
-          }
+      // The sums are shared out again, a tile of 8 rows to each of the warps in turn. A lane has outputs g and g + 8
+      // of rows 2 t and 2 t + 1; with the lane of the next g it trades one row's for the other's, so that it stores
+      // two outputs side by side.
+      if (p.wk > 1) {
+        if (wk == 0) {
+#pragma unroll
+          for (int s = 0; s < STRIPS; ++s)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+              mine4[(s * NT + i) * 32] = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
         }
+        compute_sync(n_warps * 32);
       }
-      compute_sync(n_warps * 32);
+      const int pair = blockIdx.x * p.wn + wn;
+      const bool odd = g & 1;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        if (i >= tiles || (i & (p.wk - 1)) != wk) continue;
+        float v[STRIPS][4];
+#pragma unroll
+        for (int s = 0; s < STRIPS; ++s) {
+          if (p.wk > 1) *reinterpret_cast<float4*>(v[s]) = mine4[(s * NT + i) * 32];
+          else *reinterpret_cast<float4*>(v[s]) = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
+        }
+        if (MODE == GLU) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[0][k] = activation(p.act, v[0][k]) * v[1][k];
+        }
+        const int r = i * 8 + 2 * t + odd;
+        const int64_t to = r < live ? out_row(r0 + r) * p.ld_out : 0;
+#pragma unroll
+        for (int s = 0; s < (MODE == GLU ? 1 : STRIPS); ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float got = __shfl_xor_sync(0xffffffffu, v[s][2 * h + (odd ? 0 : 1)], 4);
+            const float a = odd ? got : v[s][2 * h], b = odd ? v[s][2 * h + 1] : got;
+            const int col = (MODE == GLU ? pair : pair * STRIPS + s) * 16 + h * 8 + (g & 6);
+            if (r >= live || col >= p.n_dim) continue;
+            if (MODE == PAIRS) {   // (an even number of columns, in fp32)
+              *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + col) = make_float2(a, b);
+            } else if (MODE == GLU || p.n_dim % 2 == 0) {
+              *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + col) = Half16<T>::pack(a, b);
+            } else {
+              static_cast<T*>(p.out)[to + col] = Half16<T>::from_float(a);
+              if (col + 1 < p.n_dim) static_cast<T*>(p.out)[to + col + 1] = Half16<T>::from_float(b);
+            }
+          }
+      }
+      if (p.wk > 1) compute_sync(n_warps * 32);
     }
   }
   // weights copied for rows that did not come: nobody leaves with a copy in flight
-  __shared__ int ahead;
-  if (copier == 0 && lane == 0) ahead = w_issued;
-  __syncthreads();
-  if (copier >= 0) {
-    while (x_issued < ahead && !dead) {
-      const int s = x_slot, use = x_issued / p.depth;
-      issue_stage(nullptr, 0);
-      for (int n = 0; n < 4096 && !mbar_try_wait(full_bar + s, use & 1); ++n) {
+  if (copier == 0) {
+    for (int i = x_issued; i < w_issued; ++i) {   // (only ever a pass's first stages, each slot's first use)
+      if (lane == 0)
+        mbar_expect_tx(full_bar + i, (MODE == GLU ? 2 : 1) * live_strips * (i == n_stages - 1 ? p.last : p.full));
+      for (int k = lane; k < 32 * COPY_WARPS; k += 32) mbar_arrive(full_bar + i);
+      for (int n = 0; n < 4096 && !mbar_try_wait(full_bar + i, 0); ++n) {
       }
     }
   }
@@ -580,7 +598,7 @@ static bool set_warps(Args& a, int nt, bool glu, int64_t matrices, int slots, in
     b.kpb = (a.full_blocks + wk - 1) / wk;
     b.wn = MAX_WARPS / wk;
     while (b.wn / 2 >= pairs) b.wn /= 2;
-    const int red = (wk + 1) / 2 * b.wn * STRIPS * 16 * (nt * 8 + 1) * int(sizeof(float));
+    const int red = wk / 2 * b.wn * STRIPS * nt * 32 * int(sizeof(float4));
     const int fit = (memory - red) / StageShape(a.full_blocks, b.wn * STRIPS, a.full, a.x_rows).bytes;
     b.depth = std::min(std::min(fit, a.n_stages), MAX_DEPTH);
     if (b.depth < std::min(2, a.n_stages) && a.wk > 0) break;   // (the ring of the last try is longer)
@@ -599,14 +617,14 @@ template <typename T, int NT, bool FINE, int MODE>
 static int launch(Args a, cudaStream_t st) {
   auto kern = int4_kernel<T, NT, FINE, MODE>;
   // shared memory of a CTA: an equal share for as many as the registers allow
-  constexpr int share = 227 * 1024 / ctas_per_sm(NT, MODE) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 4 * PAIR_WINDOW) - 256;
+  constexpr int share = 227 * 1024 / ctas_per_sm(NT) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 4 * PAIR_WINDOW) - 256;
   a.x_rows = MODE == DENSE ? std::min(a.rows, NT * 8) : NT * 8;
   a.row_chunks = std::max(1, (a.rows + NT * 8 - 1) / (NT * 8));
   const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
   if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
-  if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT, MODE), share)) return MOE_B200_ERR_UNSUPPORTED;
+  if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT), share)) return MOE_B200_ERR_UNSUPPORTED;
   const int smem = a.depth * StageShape(a.full_blocks, a.wn * STRIPS, a.full, a.x_rows).bytes +
-                   (a.wk + 1) / 2 * a.wn * STRIPS * 16 * (NT * 8 + 1) * int(sizeof(float));
+                   a.wk / 2 * a.wn * STRIPS * NT * 32 * int(sizeof(float4));
   static PerDevice<cudaError_t> ready;
   int dev = -1;
   const cudaError_t* ok = cudaGetDevice(&dev) != cudaSuccess ? nullptr : ready.get(dev, [&](int) {
