@@ -657,3 +657,64 @@ def test_graphs_of_two_calls_share_nothing():
     torch.cuda.synchronize()
     for _, out in graphs:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# --------------------------------------------------------------------------- places past 31 and 32 bits
+def test_grouped_results_past_two_to_the_31():
+    """More than 2^31 values in y and in dw: what lies at the ends is what a small call gives."""
+    r, n = 540_000, 4096
+    x, w = randn(r, 8), randn(2, 8, n, seed=1)
+    off = torch.tensor([0, r - 300, r], dtype=torch.int32, device="cuda")
+    y = grouped_mm(x, w, off)
+    assert y.numel() > 2 ** 31
+    tail = torch.tensor([0, 100, 400], dtype=torch.int32, device="cuda")
+    assert torch.equal(y[-400:], grouped_mm(x[-400:].contiguous(), w, tail))
+    del y
+    g, m, n = 260, 2048, 4096
+    a, b = randn(40, m), randn(40, n, seed=1)
+    off = torch.full((g + 1,), 40, dtype=torch.int32, device="cuda")
+    off[:g - 1] = 0
+    off[g - 1] = 25
+    dw = kernels.grouped_wgrad(a, b, off)
+    assert dw.numel() > 2 ** 31
+    small = kernels.grouped_wgrad(a, b, torch.tensor([0, 25, 40], dtype=torch.int32, device="cuda"))
+    assert torch.equal(dw[-2:], small) and not dw[0].any() and not dw[g // 2].any()
+
+
+def test_experts_past_two_to_the_32_levels():
+    """The last of 2300 experts, whose levels lie beyond 2^32, is the expert it is by itself."""
+    d, h, e = 1024, 1024, 2300
+    one_in, one_out = quantize_int4(randn(1, d, 2 * h)), quantize_int4(randn(1, h, d, seed=1))
+    many = [Int4Weight(torch.zeros(e, w.data.shape[1], dtype=torch.uint8, device="cuda"), (e, *w.shape[1:]), 64,
+                       torch.bfloat16) for w in (one_in, one_out)]
+    for big, w in zip(many, (one_in, one_out)):
+        big.data[-1] = w.data[0]
+    assert e * d * 2 * h > 2 ** 32
+    x, tw = randn(3, d), torch.ones(3, 1, device="cuda", dtype=torch.bfloat16)
+    idx = torch.full((3, 1), e - 1, device="cuda")
+    want = int4_experts(x, tw, torch.zeros_like(idx), one_in, one_out)
+    assert torch.equal(int4_experts(x, tw, idx, *many), want) and bool(want.any())
+
+
+def test_dropout_past_two_to_the_31_elements():
+    n = 2 ** 31 + 12_345
+    rng = torch.tensor([7, 9], device="cuda")
+    out = dropout_add(torch.ones(n, dtype=torch.float16, device="cuda"), None, 0.5, rng)
+    for at in (2 ** 31 - 8, n - 9):
+        for i in range(at, at + 8):
+            c, k = [(i // 4) & 0xFFFFFFFF, (i // 4) >> 32, 9, 0], [7, 0]
+            for _ in range(10):
+                a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+                c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+                k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+            assert float(out[i]) == (2.0 if c[i % 4] >= 2 ** 31 else 0.0)
+
+
+def test_int4_mm_many_rows():
+    """More rows than one grid line of passes, of which each is 32 rows."""
+    q, s = levels((64, 48), 64, torch.bfloat16)
+    w = Int4Weight.from_levels(q, s, 64)
+    x = randn(40_000, 64)
+    y = int4_mm(x, w)
+    ew = exact_weight(q, s, 64)
+    within(y, x.double() @ ew, 128, x.double().abs() @ ew.abs())
