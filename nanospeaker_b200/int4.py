@@ -27,10 +27,23 @@ class Int4Weight:
     shape     (K, N) or (G, K, N)
     group     inputs that share a scale: 32, 64 or 128 (the last group of a matrix may be short)
     dtype     of the scales, bf16 or fp16: that of the activations
-    data      uint8 [G, bytes of a matrix]"""
+    data      uint8 [G, bytes of a matrix] (G = 1 for a matrix), contiguous, on 16 bytes"""
 
     def __init__(self, data: torch.Tensor, shape, group: int, dtype: torch.dtype):
-        self.data, self.shape, self.group, self.dtype = data, tuple(shape), group, dtype
+        shape = tuple(shape)
+        if dtype not in INT4_DTYPES:
+            raise ValueError(f"scales are bf16 or fp16, got {dtype}")
+        _check_group(group)
+        if len(shape) not in (2, 3):
+            raise ValueError(f"a weight is [K, N] or [G, K, N], got {shape}")
+        _check_widths(*shape[-2:])
+        want = (shape[0] if len(shape) == 3 else 1, _matrix_bytes(*shape[-2:], group))
+        if data.dtype != torch.uint8 or tuple(data.shape) != want or not data.is_contiguous():
+            raise ValueError(f"a weight {shape} in groups of {group} is {want} bytes in one piece, got "
+                             f"{data.dtype} {tuple(data.shape)}")
+        if data.device.type != "meta" and data.data_ptr() % 16:
+            raise ValueError("packed weights have to start on 16 bytes")
+        self.data, self.shape, self.group, self.dtype = data, shape, group, dtype
 
     device = property(lambda self: self.data.device)
 
@@ -48,8 +61,9 @@ class Int4Weight:
             raise ValueError(f"scales are bf16 or fp16, got {scales.dtype}")
         _check_group(group)
         k, n = levels.shape[-2:]
-        if k < 8 or k % 8 or n < 1:
-            raise ValueError(f"a weight of {k} inputs and {n} outputs: inputs have to be a multiple of 8")
+        _check_widths(k, n)
+        if bool((levels > 15).any()):
+            raise ValueError("levels are 0 .. 15")
         if tuple(scales.shape) != (*levels.shape[:-2], -(-k // group), n):
             raise ValueError(f"levels {tuple(levels.shape)} in groups of {group} do not take scales "
                              f"{tuple(scales.shape)}")
@@ -122,6 +136,17 @@ def _chunks(kb: int, kg: int, group: int):
 def _check_group(group: int) -> None:
     if group not in GROUPS:
         raise ValueError(f"scale groups of {group} inputs: {GROUPS} are covered")
+
+
+def _check_widths(k: int, n: int) -> None:
+    if not (8 <= k < 2 ** 31 and 1 <= n < 2 ** 31) or k % 8:
+        raise ValueError(f"a weight of {k} inputs and {n} outputs: inputs have to be a multiple of 8")
+
+
+def _matrix_bytes(k: int, n: int, group: int) -> int:
+    """moe_b200_int4_bytes."""
+    kb = -(-k // BLOCK)
+    return -(-n // STRIP) * (kb * 512 + -(-kb * BLOCK // group) * 32)
 
 
 def quantize_int4(w: torch.Tensor, group: int = 64, dtype: Optional[torch.dtype] = None) -> Int4Weight:

@@ -266,6 +266,34 @@ def test_weight_refusals():
 
 
 # ------------------------------------------------------------------------------------- refusals
+def test_packed_weights_that_are_not_what_they_say_are_refused(lib):
+    from nanospeaker_b200 import Int4Weight, quantize_int4
+    from nanospeaker_b200.int4 import _matrix_bytes
+    for k, n, group in ((8, 1, 32), (136, 33, 128), (4096, 4096, 64), (520, 17, 128), (1000, 16, 32)):
+        assert _matrix_bytes(k, n, group) == lib.moe_b200_int4_bytes(k, n, group)
+    w = quantize_int4(torch.randn(3, 128, 48), 64)
+    again = Int4Weight(w.data, w.shape, w.group, w.dtype)
+    assert torch.equal(again.dequantize(), w.dequantize())
+    for data, shape, group, dtype, what in (
+            (w.data[:2], w.shape, 64, w.dtype, "in one piece"),
+            (w.data[:, :-32], w.shape, 64, w.dtype, "in one piece"),
+            (w.data, (3, 128, 64), 64, w.dtype, "in one piece"),
+            (w.data, w.shape, 32, w.dtype, "in one piece"),
+            (w.data.to(torch.int32), w.shape, 64, w.dtype, "in one piece"),
+            (w.data.t().contiguous().t(), w.shape, 64, w.dtype, "in one piece"),
+            (w.data, w.shape, 48, w.dtype, "scale groups"),
+            (w.data, w.shape, 64, torch.float32, "scales are"),
+            (w.data, (384, 3, 16, 8), 64, w.dtype, "a weight is"),
+            (w.data, (3, 130, 48), 64, w.dtype, "multiple of 8")):
+        with pytest.raises(ValueError, match=what):
+            Int4Weight(data, shape, group, dtype)
+    off = torch.empty(w.data.numel() + 1, dtype=torch.uint8)[1:].view(w.data.shape)
+    with pytest.raises(ValueError, match="16 bytes"):
+        Int4Weight(off, w.shape, 64, w.dtype)
+    with pytest.raises(ValueError, match="0 .. 15"):
+        Int4Weight.from_levels(torch.full((64, 16), 16, dtype=torch.uint8), torch.ones(1, 16, dtype=torch.bfloat16), 64)
+
+
 def test_grouped_refusals():
     from nanospeaker_b200 import grouped_mm
     x, w = torch.randn(6, 16).bfloat16(), torch.randn(2, 16, 24).bfloat16()
