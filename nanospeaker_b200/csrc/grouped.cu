@@ -36,6 +36,7 @@ constexpr int EPI_WARPS = 8;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int BAND = 8;   // row tiles of a band (tile_in_bands)
 constexpr int SHORT = 32; // rows of the smaller A box
+constexpr int MAX_ROWS = INT_MAX - 2 * BM;   // (a tile's rows behind the last one are still ints)
 // MN-major operands, as in gemm.cuh: 64 x 64 boxes
 constexpr uint32_t MN_LBO = 8192u, MN_SBO = 1024u, MN_KADV = 2048u;
 
@@ -981,7 +982,7 @@ int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
                         int32_t n_groups, int64_t w_group_stride, int64_t ld_w, int32_t n_inner,
                         int32_t n_dim, const int32_t* offsets, int32_t dtype, void* y, int32_t* status,
                         void* stream) {
-  if (rows < 0 || rows > INT_MAX || k_dim < 8 || k_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
+  if (rows < 0 || rows > grouped::MAX_ROWS || k_dim < 8 || k_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
       n_groups > RUNS_MAX_GROUPS || ld_x < k_dim || ld_x % 8 || w_group_stride % 8 || ld_w % 8 ||
       w_group_stride < 0 || ld_w < (n_inner ? n_dim : k_dim))
     return MOE_B200_ERR_SHAPE;
@@ -1011,7 +1012,7 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
                            int32_t n_dim, int64_t rows, const int32_t* offsets, int32_t n_groups,
                            int32_t dtype, void* dw, void* scratch, size_t scratch_bytes, int32_t* status,
                            void* stream) {
-  if (rows < 0 || rows > INT_MAX || m_dim < 8 || m_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
+  if (rows < 0 || rows > grouped::MAX_ROWS || m_dim < 8 || m_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
       n_groups > RUNS_MAX_GROUPS || ld_a < m_dim || ld_a % 8 || ld_b < n_dim || ld_b % 8)
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;

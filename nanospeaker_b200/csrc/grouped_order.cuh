@@ -39,7 +39,7 @@ MOE_ORDER_FN TileAt tile_in_bands(int l, int m_tiles, int n_tiles, int band) {
 
 // Chunks of at most ks rows that a run of `rows` rows is cut into: at least one, a run without rows
 // still has its (zero) result stored.
-MOE_ORDER_FN int run_chunks(int rows, int ks) { return rows <= ks ? 1 : (rows + ks - 1) / ks; }
+MOE_ORDER_FN int run_chunks(int rows, int ks) { return rows <= ks ? 1 : (rows - 1) / ks + 1; }
 
 // Rows per chunk for n_groups runs of `rows` rows in all whose result has `tiles` tiles each. The runs being
 // alike, `n` chunks each give rounds of all clusters that take (a 64-row step 0.5 us, a tile's end 2 us, all

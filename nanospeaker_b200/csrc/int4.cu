@@ -743,7 +743,8 @@ int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t
                           void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
   if (n_tokens < 0 || top_k < 1 || n_experts < 1 || n_shared < 0 || n_experts + int64_t(n_shared) > 65535 ||
       d_model < 8 || d_model % 8 || d_hidden < 16 || d_hidden % 16 || ld_x < d_model || ld_x % 8 ||
-      !q4::group_ok(group) || n_tokens * (int64_t(top_k) + n_shared) > 0x7fffffff)
+      !q4::group_ok(group) || n_tokens > 0x7fffffff ||
+      n_tokens * (int64_t(top_k) + n_shared) > 0x7fffffff - q4::PAIR_WINDOW)
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
   if (activation < MOE_B200_ACT_SILU || activation > MOE_B200_ACT_TANH) return MOE_B200_ERR_UNSUPPORTED;

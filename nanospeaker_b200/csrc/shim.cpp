@@ -872,6 +872,7 @@ OptTensor grouped_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, in
   if (x.dim() != 2 || w.dim() != 3 || offsets.dim() != 1 || x.size(1) != w.size(1) ||
       offsets.numel() != w.size(0) + 1 || !half16(x) || w.scalar_type() != x.scalar_type() ||
       offsets.scalar_type() != at::kInt || w.size(1) < 8 || w.size(2) < 8 || w.size(1) % 8 || w.size(2) % 8 ||
+      w.size(1) > INT32_MAX || w.size(2) > INT32_MAX ||
       w.size(0) < 1 || w.size(0) > max_groups || !x.is_cuda() || w.device() != x.device() ||
       offsets.device() != x.device())
     return {};
@@ -924,7 +925,7 @@ OptTensor int4_experts(const Tensor& x_in, const Tensor& topk_w, const Tensor& t
                        at::ScalarType dtype, int64_t d_model, int64_t d_hidden, int64_t group, int64_t act) {
   const auto device = x_in.device();
   if (x_in.dim() != 2 || topk_idx.dim() != 2 || topk_w.sizes() != topk_idx.sizes() ||
-      topk_idx.size(0) != x_in.size(0) || topk_idx.size(1) < 1 || !x_in.is_cuda() ||
+      topk_idx.size(0) != x_in.size(0) || topk_idx.size(1) < 1 || topk_idx.size(1) > INT32_MAX || !x_in.is_cuda() ||
       x_in.scalar_type() != dtype || x_in.size(1) != d_model || topk_w.scalar_type() != dtype ||
       topk_idx.scalar_type() != at::kLong || topk_w.device() != device || topk_idx.device() != device ||
       w_in.device() != device || w_out.device() != device ||

@@ -259,7 +259,7 @@ def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, 
     weights = (w_in, w_out, *shared)
     _check_types(x, *weights)
     if x.dim() != 2 or topk_idx.dim() != 2 or topk_w.shape != topk_idx.shape or \
-            topk_idx.shape[0] != x.shape[0] or topk_idx.shape[1] < 1:
+            topk_idx.shape[0] != x.shape[0] or not 1 <= topk_idx.shape[1] < 2 ** 31:
         raise ValueError(f"int4_experts takes x [T, D] with topk_w and topk_idx [T, k], got "
                          f"{tuple(x.shape)}, {tuple(topk_w.shape)} and {tuple(topk_idx.shape)}")
     if topk_w.dtype != x.dtype or topk_idx.dtype != torch.int64:

@@ -87,6 +87,12 @@ def test_chunks_of_a_run(host, rows, ks, want):
     assert host.chunks(rows, ks) == want
 
 
+def test_chunks_of_the_longest_run(host):
+    rows = (1 << 31) - 257
+    for ks in (256, 1 << 20, 96_745_344, rows - 1, rows):
+        assert host.chunks(rows, ks) == -(-rows // ks)
+
+
 def test_chunk_rows(host):
     """Runs are cut where there are too few tiles for the clusters, or where one is far longer than the
     rest."""
@@ -407,3 +413,19 @@ def test_entry_points_validate_before_any_launch(lib):
     assert dr(dt=3) == -5
     assert dr(x=null) == dr(rng=null) == dr(o=null) == -2
     assert dr(rng=odd) == dr(used=odd) == dr(x=odd, dt=2) == -3
+
+
+def test_sizes_whose_places_leave_31_bits_are_refused(lib):
+    buf = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 63) & ~63)
+    rows = (1 << 31) - 256
+    assert lib.moe_b200_grouped_mm(p, rows, 8, 8, p, 1, 64, 8, 1, 8, p, 0, p, p, None) == -1
+    assert lib.moe_b200_grouped_wgrad(p, 8, 8, p, 8, 8, rows, p, 1, 0, p, None, 0, p, None) == -1
+    for tokens, top_k in (((1 << 31) - 1023, 1), (1, (1 << 31) - 1023), ((1 << 33) + 1, 1)):
+        assert lib.moe_b200_int4_experts(p, tokens, 8, 8, 16, p, p, top_k, 4, p, p, 0, None, None, 64, 0, 0, p, p,
+                                         1 << 62, p, None) == -1
+    from nanospeaker_b200 import grouped_mm
+    x, w = torch.empty(4, 1 << 31, device="meta", dtype=torch.bfloat16), torch.empty(
+        2, 1 << 31, 8, device="meta", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="widths"):
+        grouped_mm(x, w, torch.empty(3, device="meta", dtype=torch.int32))
