@@ -97,7 +97,7 @@ class MoEFFNSublayer(nn.Module):
     def _with_dropout(self, x: torch.Tensor):
         """x + dropout(ffn(norm(x))): the residual is added where the mask is made."""
         y = self.ffn(F.rms_norm(x, (x.shape[-1],), self.norm_gamma.to(x.dtype), self.epsilon))
-        if x.is_cuda and x.dtype in DROPOUT_DTYPES:
+        if x.is_cuda and x.dtype == y.dtype and x.dtype in DROPOUT_DTYPES:   # (autocast's may differ)
             rng = torch.empty(2, dtype=torch.int64, device=x.device).random_()
             out = dropout_add(y, x, self.dropout, rng)
         else:

@@ -151,6 +151,36 @@ def test_sublayer_dropout_masks_and_gradients():
 
 
 @gpu
+@pytest.mark.parametrize("kernel,dtype", [(True, torch.bfloat16), (False, torch.bfloat16), (False, torch.float16)])
+def test_sublayer_dropout_under_autocast(kernel, dtype):
+    """The result has the type that the sublayer without dropout gives, and gradients flow. (In fp16 the shared
+    experts' bf16 products make the block's result fp32.)"""
+    ffn = block(64, 8, 96, 2, 1, dtype, kernel=kernel).cuda().train()
+    ffn.grouped = not kernel
+    x = torch.randn(40, 64, device="cuda").to(dtype).requires_grad_()
+    with torch.autocast("cuda", torch.bfloat16):
+        want, _ = MoEFFNSublayer(ffn).cuda()(x)
+        out, _ = MoEFFNSublayer(ffn, dropout=0.5).cuda()(x)
+    assert out.dtype == want.dtype and out.shape == want.shape
+    out.float().sum().backward()
+    assert bool(torch.isfinite(x.grad).all())
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(0, 64), (2, 0, 64), (1, 64), (3, 5, 64)])
+def test_wide_sublayer_and_block_of_few_rows_and_none(shape):
+    m = block(64, 8, 96, 2, dtype=torch.bfloat16).cuda().train()
+    m.grouped = True
+    sub = MoEFFNSublayer(m, dropout=0.5).to(torch.bfloat16).cuda()
+    x = torch.randn(shape, device="cuda").bfloat16().requires_grad_()
+    assert m(x).shape == sub(x)[0].shape == x.shape
+    if x.numel():
+        sub(x)[0].float().sum().backward()
+        assert bool(torch.isfinite(x.grad).all())
+    assert StackedMoEDecoder([m], weights="int4").eager(x.detach()).shape == x.shape
+
+
+@gpu
 def test_sublayer_dropout_under_activation_checkpointing():
     """The recomputed forward meets the same mask: gradients as without checkpointing."""
     from torch.utils.checkpoint import checkpoint
