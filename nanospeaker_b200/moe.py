@@ -17,7 +17,7 @@ Paths, in the order `forward` tries them:
                the dispatch drops the pairs over capacity instead of padding a batch.
   2. grouped   with `block.grouped = True`, CUDA blocks of widths (or in fp16) that the kernels of 1.
                decline: the experts' products as `grouped_mm` over the sorted pairs, dropless unless a
-               capacity is given; gather, GLU and sum are torch's. No host sync.
+               capacity is given (or "auto" with weights that are not 16-bit); gather, GLU and sum are torch's. No host sync.
   3. torch     the per-expert loop in plain torch (src/model/moe.py:377-418) for everything the
                kernels decline (CPU, fp32/fp64, custom activations), with or without a capacity.
 """
@@ -176,10 +176,11 @@ class MoEBlock(nn.Module):
 
     def _shared(self, x):
         """Sum of the always-on experts on every token (src/model/moe.py:310-329)."""
+        cast = (lambda t: t.to(x.dtype)) if self._grouped_ok(x) else (lambda t: t)   # (as the routed ones')
         total = None
         for s in range(self.n_shared):
-            y = self._mlp(x, self.W_sh_in[s], None if self.b_sh_in is None else self.b_sh_in[s],
-                          self.W_sh_out[s], None if self.b_sh_out is None else self.b_sh_out[s])
+            y = self._mlp(x, cast(self.W_sh_in[s]), None if self.b_sh_in is None else cast(self.b_sh_in[s]),
+                          cast(self.W_sh_out[s]), None if self.b_sh_out is None else cast(self.b_sh_out[s]))
             total = y if total is None else total + y
         return total
 

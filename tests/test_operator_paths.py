@@ -106,6 +106,21 @@ def test_block_of_any_width_matches_the_torch_loop(kw, dtype):
 
 
 @gpu
+def test_wide_block_with_fp32_weights_takes_16_bit_rows():
+    """Weights in fp32, cast where they are used: the result of the 16-bit block with the same values, and fp32
+    gradients."""
+    m = block(64, 8, 96, 2, 2, torch.bfloat16, bias=True).cuda().train()
+    full = block(64, 8, 96, 2, 2, bias=True).cuda().train()
+    full.load_state_dict({k: v.float() for k, v in m.state_dict().items()})
+    m.grouped = full.grouped = True
+    x = torch.randn(60, 64, device="cuda").bfloat16()
+    got, want = both(full, x, x), both(m, x, x)
+    assert torch.equal(got[0], want[0]) and got[0].dtype == torch.bfloat16
+    for a, b in zip(got[2:], want[2:]):
+        assert a.dtype == torch.float32 and rel_l2(a, b) < TOL[torch.bfloat16]
+
+
+@gpu
 def test_block_of_any_width_without_a_sync_and_in_a_graph():
     m = block(64, 8, 96, 2, dtype=torch.bfloat16).cuda().eval()
     m.grouped = True
