@@ -128,14 +128,19 @@ __device__ __forceinline__ void levels_of(uint32_t word, uint32_t* a) {
   }
 }
 
-// (Called, not copied to every place: these kernels are over before much code has been fetched.)
-__device__ __noinline__ float activation(int act, float g) {
+// Four at a time, side by side: one after another they were a tenth of a CTA's time. (Called, not copied to every
+// place: these kernels are over before much code has been fetched.)
+template <int ACT>
+__device__ __forceinline__ float4 act4(const float4& g) {
+  return make_float4(act_f<ACT>(g.x), act_f<ACT>(g.y), act_f<ACT>(g.z), act_f<ACT>(g.w));
+}
+__device__ __noinline__ float4 activation(int act, float4 g) {
   switch (act) {
-    case ACT_SILU: return act_f<ACT_SILU>(g);
-    case ACT_GELU: return act_f<ACT_GELU>(g);
-    case ACT_RELU: return act_f<ACT_RELU>(g);
-    case ACT_SIGMOID: return act_f<ACT_SIGMOID>(g);
-    default: return act_f<ACT_TANH>(g);
+    case ACT_SILU: return act4<ACT_SILU>(g);
+    case ACT_GELU: return act4<ACT_GELU>(g);
+    case ACT_RELU: return act4<ACT_RELU>(g);
+    case ACT_SIGMOID: return act4<ACT_SIGMOID>(g);
+    default: return act4<ACT_TANH>(g);
   }
 }
 
@@ -177,38 +182,53 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
   constexpr int ROWS = NT * 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_bar[MAX_DEPTH], empty_bar[MAX_DEPTH];
-  __shared__ int list[MODE == DENSE ? 1 : PAIR_WINDOW];
-  __shared__ uint32_t found[MODE == DENSE ? 1 : PAIR_WINDOW / 32];
-  __shared__ int warp_count[MAX_WARPS + 2];
+  __shared__ uint16_t list[MODE == DENSE ? 1 : PAIR_WINDOW];   // places in the window
+  __shared__ int n_found;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_warps = p.wk * p.wn;
   constexpr int COPY_WARPS = copy_warps(NT);
   const StageShape sh(p.full_blocks, p.wn * STRIPS, p.full, p.x_rows);
-  float4* red = reinterpret_cast<float4*>(smem + p.depth * sh.bytes);   // [wk / 2][wn][STRIPS * NT][32 lanes]
+  float4* red = reinterpret_cast<float4*>(smem + p.depth * sh.bytes);   // [wk - 1][wn][STRIPS * NT][32 lanes]
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.depth; ++i) {
       mbar_init(full_bar + i, 1 + 32 * COPY_WARPS);   // the weights' bytes, and every copying lane's rows
       mbar_init(empty_bar + i, n_warps);
     }
+    n_found = 0;
     fence_mbar_init();
   }
+  // The down projection's weights and ids are older than the kernel before it, whose result (the rows of
+  // x) it waits for further down: that kernel lets this one start when it has itself waited for all before it.
+  if (MODE == GLU) pdl_wait();
+  // The ids that this thread looks at first, asked for ahead of all else (LOOKS in flight, a CTA's width apart).
+  constexpr int LOOKS = 8;
+  int64_t seen[LOOKS];
+  auto look = [&](int base, int n, int from) {
+#pragma unroll
+    for (int i = 0; i < LOOKS; ++i) {
+      const int at = from + i * int(blockDim.x) + lane;
+      seen[i] = at < n ? p.topk_idx[base + at] : -1;
+    }
+  };
+  const bool all_rows = MODE == DENSE || int(blockIdx.y) >= p.routed.groups;
+  if (!all_rows) look(0, min(PAIR_WINDOW, p.n_pairs), warp * 32);
   __syncthreads();
 
   // which matrix, and which of its rows
-  const bool all_rows = MODE == DENSE || int(blockIdx.y) >= p.routed.groups;
   const int y = MODE == DENSE ? blockIdx.y : int(blockIdx.y) - p.routed.groups;
   const int chunk = all_rows ? y % p.row_chunks : 0;
   const int e = MODE == DENSE ? 0 : all_rows ? y / p.row_chunks : int(blockIdx.y);
   const int strip_step = MODE == GLU ? p.strips / 2 : 1;
   const int n_stages = p.n_stages;
   // the row of the result, and of x, that row r of this expert is
+  int win = 0;
   auto out_row = [&](int r) -> int64_t {
     if (MODE == DENSE) return r;
-    return all_rows ? int64_t(p.n_pairs) + int64_t(e) * p.rows + r : list[r];
+    return all_rows ? int64_t(p.n_pairs) + int64_t(e) * p.rows + r : win * PAIR_WINDOW + list[r];
   };
   auto x_row = [&](int r) -> int64_t {
-    return MODE == DENSE ? r : MODE == PAIRS ? out_row(r) : all_rows ? r : list[r] / p.top_k;
+    return MODE == DENSE ? r : MODE == PAIRS ? out_row(r) : all_rows ? r : (win * PAIR_WINDOW + list[r]) / p.top_k;
   };
 
   // ---- the copying warps' side. A pass is n_stages stages, the weights the same ones in each; the first of
@@ -264,9 +284,7 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
     }
   };
 
-  // The down projection's weights and ids are older than the kernel before it, whose result (the rows of
-  // x) it waits for behind this: that kernel lets this one start when it has itself waited for all before it.
-  if (MODE != PAIRS) pdl_wait();
+  if (MODE == DENSE) pdl_wait();
   pdl_trigger();
   if (copier == 0 && (p.eager || all_rows))
     for (int i = min(p.depth, n_stages); i > 0; --i) issue_weights();
@@ -274,38 +292,38 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
   const int windows = all_rows ? 1 : (p.n_pairs + PAIR_WINDOW - 1) / PAIR_WINDOW;
   bool waited = MODE != PAIRS;
   int slot = 0, phase = 0;
-  for (int win = 0; win < windows; ++win) {
+  for (; win < windows; ++win) {
     int first = chunk * ROWS, n_rows = all_rows ? min(p.rows, first + ROWS) : 0;
     if (!all_rows) {
-      // the pairs of this expert among the window's, in order: every warp looks at a share of them
+      // The pairs of this expert among the window's, in whatever order the warps come: rows do not mix, a row's
+      // result is the same in any place.
       const int base = win * PAIR_WINDOW, n = min(PAIR_WINDOW, p.n_pairs - base);
-      const int all = n_warps + COPY_WARPS;
-      const int share = ((n + all - 1) / all + 31) / 32 * 32;
-      const int lo = warp * share, hi = min(n, lo + share);
-      int count = 0;
-#pragma unroll 4
-      for (int at = lo; at < hi; at += 32) {
-        const uint32_t who = __ballot_sync(0xffffffffu, at + lane < hi && p.topk_idx[base + at + lane] == e);
-        if (lane == 0) found[at >> 5] = who;
-        count += __popc(who);
+      if (win > 0) {
+        __syncthreads();     // (the list of the window before has been used)
+        if (threadIdx.x == 0) n_found = 0;
+        __syncthreads();
       }
-      if (win > 0) __syncthreads();     // (the list of the window before has been used)
-      if (lane == 0) warp_count[warp] = count;
-      __syncthreads();
-      int before = 0;
-      for (int i = 0; i < all; ++i) {
-        before += i < warp ? warp_count[i] : 0;
-        n_rows += warp_count[i];
-      }
-      if (count > 0) {
-#pragma unroll 1
-        for (int at = lo; at < hi; at += 32) {
-          const uint32_t who = found[at >> 5];
-          if ((who >> lane) & 1) list[before + __popc(who & ((1u << lane) - 1))] = base + at + lane;
-          before += __popc(who);
+      for (int from = warp * 32; from < n; from += LOOKS * int(blockDim.x)) {
+        if (win > 0 || from != warp * 32) look(base, n, from);
+        uint32_t who[LOOKS];
+        int count = 0, at = 0;
+#pragma unroll
+        for (int i = 0; i < LOOKS; ++i) {
+          who[i] = __ballot_sync(0xffffffffu, seen[i] == e);
+          count += __popc(who[i]);
+        }
+        if (count == 0) continue;
+        if (lane == 0) at = atomicAdd(&n_found, count);
+        at = __shfl_sync(0xffffffffu, at, 0);
+#pragma unroll
+        for (int i = 0; i < LOOKS; ++i) {
+          if ((who[i] >> lane) & 1)
+            list[at + __popc(who[i] & ((1u << lane) - 1))] = uint16_t(from + i * int(blockDim.x) + lane);
+          at += __popc(who[i]);
         }
       }
       __syncthreads();
+      n_rows = n_found;
     }
     if (n_rows <= first) continue;
     if (!waited) {
@@ -368,42 +386,49 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
 #pragma unroll
             for (int k = 0; k < 4; ++k) levels_of<T>(q[k], a[s][k]);
           }
+          // Tiles whose products, independent of one another, are in the works together. Two where all tiles mostly have
+          // rows (64 rows x 4096^2: 13.3 us with one, 12.8 with two); an expert's last tile would often have no partner
+          // (200 tokens: 57.9 us with one, 58.7 with two).
+          constexpr int AT = MODE == DENSE && NT > 1 ? 2 : 1;
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            if (i > 0 && i >= tiles) break;
-            uint4 b0, b1;
-            ld_shared_v4(x_at[i] + j * 128, b0.x, b0.y, b0.z, b0.w);
-            ld_shared_v4(x_at[i] + j * 128 + other[i], b1.x, b1.y, b1.z, b1.w);
-            if (cut) {
-              const int k = kb * 64 + t * 8;
-              if (k >= p.k_dim) b0 = make_uint4(0, 0, 0, 0);
-              if (k + 32 >= p.k_dim) b1 = make_uint4(0, 0, 0, 0);
-            }
-            float c[STRIPS][4];
-            auto scale_in = [&](int h) {
+          for (int i0 = 0; i0 < NT; i0 += AT) {
+            if (i0 > 0 && i0 >= tiles) break;
+            uint4 b0[AT], b1[AT];
+            float c[AT][STRIPS][4] = {};
 #pragma unroll
-              for (int s = 0; s < STRIPS; ++s) {
-                const float2 f = Half16<T>::unpack(sc[s][h]);
-                acc[s][i][0] += f.x * c[s][0];
-                acc[s][i][1] += f.x * c[s][1];
-                acc[s][i][2] += f.y * c[s][2];
-                acc[s][i][3] += f.y * c[s][3];
+            for (int i = 0; i < AT; ++i) {
+              ld_shared_v4(x_at[i0 + i] + j * 128, b0[i].x, b0[i].y, b0[i].z, b0[i].w);
+              ld_shared_v4(x_at[i0 + i] + j * 128 + other[i0 + i], b1[i].x, b1[i].y, b1[i].z, b1[i].w);
+              if (cut) {
+                const int k = kb * 64 + t * 8;
+                if (k >= p.k_dim) b0[i] = make_uint4(0, 0, 0, 0);
+                if (k + 32 >= p.k_dim) b1[i] = make_uint4(0, 0, 0, 0);
               }
+            }
+            auto each = [&](auto f) {
+#pragma unroll
+              for (int i = 0; i < AT; ++i)
+#pragma unroll
+                for (int s = 0; s < STRIPS; ++s) f(i, s);
             };
-#pragma unroll
-            for (int s = 0; s < STRIPS; ++s) Mma<T>::first(c[s], a[s][0], b0.x, b0.y);
-#pragma unroll
-            for (int s = 0; s < STRIPS; ++s) Mma<T>::run(c[s], a[s][1], b0.z, b0.w);
+            auto scale_in = [&](int h) {
+              each([&](int i, int s) {
+                const float2 f = Half16<T>::unpack(sc[s][h]);
+                acc[s][i0 + i][0] += f.x * c[i][s][0];
+                acc[s][i0 + i][1] += f.x * c[i][s][1];
+                acc[s][i0 + i][2] += f.y * c[i][s][2];
+                acc[s][i0 + i][3] += f.y * c[i][s][3];
+              });
+            };
+            each([&](int i, int s) { Mma<T>::first(c[i][s], a[s][0], b0[i].x, b0[i].y); });
+            each([&](int i, int s) { Mma<T>::run(c[i][s], a[s][1], b0[i].z, b0[i].w); });
             if constexpr (FINE) {
               scale_in(0);
-#pragma unroll
-              for (int s = 0; s < STRIPS; ++s) Mma<T>::first(c[s], a[s][2], b1.x, b1.y);
+              each([&](int i, int s) { Mma<T>::first(c[i][s], a[s][2], b1[i].x, b1[i].y); });
             } else {
-#pragma unroll
-              for (int s = 0; s < STRIPS; ++s) Mma<T>::run(c[s], a[s][2], b1.x, b1.y);
+              each([&](int i, int s) { Mma<T>::run(c[i][s], a[s][2], b1[i].x, b1[i].y); });
             }
-#pragma unroll
-            for (int s = 0; s < STRIPS; ++s) Mma<T>::run(c[s], a[s][3], b1.z, b1.w);
+            each([&](int i, int s) { Mma<T>::run(c[i][s], a[s][3], b1[i].z, b1[i].w); });
             scale_in(FINE ? 1 : 0);
           }
         };
@@ -425,43 +450,22 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
         for (int i = 0; i < NT; ++i) x_at[i] += by;
       }
 
-      // The warps' sums meet in shared memory, the upper half's added to the lower half's until one is left (wk is a
-      // power of two). A lane adds what the same lane of another warp has: any order of the values will do.
-      float4* mine4 = red + wn * (STRIPS * NT * 32) + lane;
-      for (int half = p.wk >> 1; half > 0; half >>= 1) {
-        float4* at4 = mine4 + (wk & (half - 1)) * p.wn * (STRIPS * NT * 32);
-        if (wk >= half && wk < 2 * half) {
-#pragma unroll
-          for (int s = 0; s < STRIPS; ++s)
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-              at4[(s * NT + i) * 32] = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
-        }
-        compute_sync(n_warps * 32);
-        if (wk < half) {
-#pragma unroll
-          for (int s = 0; s < STRIPS; ++s)
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              const float4 v = at4[(s * NT + i) * 32];
-              acc[s][i][0] += v.x;
-              acc[s][i][1] += v.y;
-              acc[s][i][2] += v.z;
-              acc[s][i][3] += v.w;
-            }
-        }
-        compute_sync(n_warps * 32);
-      }
-      // The sums are shared out again, a tile of 8 rows to each of the warps in turn. A lane has outputs g and g + 8
-      // of rows 2 t and 2 t + 1; with the lane of the next g it trades one row's for the other's, so that it stores
-      // two outputs side by side.
+      // A tile of 8 rows is finished by one of the warps that share a strip's inputs, warp i % wk: the others leave
+      // it their sums in shared memory. A lane adds what the same lane of another warp has, of four warps 0 and 2, 1
+      // and 3, then both: whichever of them finishes, the bits are the same. It has outputs g and g + 8 of rows 2 t
+      // and 2 t + 1; with the lane of the next g it trades one row's for the other's, so that it stores two outputs
+      // side by side.
+      float4* sums = red + wn * (STRIPS * NT * 32) + lane;   // of the warp d - 1 places behind the tile's own
+      const int sums_step = p.wn * (STRIPS * NT * 32);
       if (p.wk > 1) {
-        if (wk == 0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const int d = (wk - i) & (p.wk - 1);
+          if (i >= tiles || d == 0) continue;
 #pragma unroll
           for (int s = 0; s < STRIPS; ++s)
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-              mine4[(s * NT + i) * 32] = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
+            sums[(d - 1) * sums_step + (s * NT + i) * 32] =
+                make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
         }
         compute_sync(n_warps * 32);
       }
@@ -470,35 +474,69 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         if (i >= tiles || (i & (p.wk - 1)) != wk) continue;
-        float v[STRIPS][4];
+        float4 v[STRIPS];
 #pragma unroll
-        for (int s = 0; s < STRIPS; ++s) {
-          if (p.wk > 1) *reinterpret_cast<float4*>(v[s]) = mine4[(s * NT + i) * 32];
-          else *reinterpret_cast<float4*>(v[s]) = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
+        for (int s = 0; s < STRIPS; ++s) v[s] = make_float4(acc[s][i][0], acc[s][i][1], acc[s][i][2], acc[s][i][3]);
+        const float4* from = sums + i * 32;
+        auto add = [](float4& x, const float4& y) {
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
+        };
+        if (p.wk == 2) {
+          float4 u[STRIPS];
+#pragma unroll
+          for (int s = 0; s < STRIPS; ++s) u[s] = from[s * (NT * 32)];
+#pragma unroll
+          for (int s = 0; s < STRIPS; ++s) add(v[s], u[s]);
+        } else if (p.wk == 4) {
+          float4 u[3][STRIPS];
+#pragma unroll
+          for (int d = 0; d < 3; ++d)
+#pragma unroll
+            for (int s = 0; s < STRIPS; ++s) u[d][s] = from[d * sums_step + s * (NT * 32)];
+#pragma unroll
+          for (int s = 0; s < STRIPS; ++s) {
+            add(v[s], u[1][s]);
+            add(u[0][s], u[2][s]);
+            add(v[s], u[0][s]);
+          }
         }
         if (MODE == GLU) {
+          const float4 f = activation(p.act, v[0]);
+          v[0] = make_float4(f.x * v[1].x, f.y * v[1].y, f.z * v[1].z, f.w * v[1].w);
+        }
+        constexpr int OUTS = MODE == GLU ? 1 : STRIPS;
+        float2 o[OUTS][2];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[0][k] = activation(p.act, v[0][k]) * v[1][k];
+        for (int s = 0; s < OUTS; ++s) {
+          const float x = __shfl_xor_sync(0xffffffffu, odd ? v[s].x : v[s].y, 4);
+          const float y = __shfl_xor_sync(0xffffffffu, odd ? v[s].z : v[s].w, 4);
+          o[s][0] = odd ? make_float2(x, v[s].y) : make_float2(v[s].x, x);
+          o[s][1] = odd ? make_float2(y, v[s].w) : make_float2(v[s].z, y);
         }
         const int r = i * 8 + 2 * t + odd;
-        const int64_t to = r < live ? out_row(r0 + r) * p.ld_out : 0;
+        if (r < live) {
+          const int col = pair * (16 * OUTS) + (g & 6);
+          const int64_t to = out_row(r0 + r) * p.ld_out + col;
 #pragma unroll
-        for (int s = 0; s < (MODE == GLU ? 1 : STRIPS); ++s)
+          for (int s = 0; s < OUTS; ++s)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float got = __shfl_xor_sync(0xffffffffu, v[s][2 * h + (odd ? 0 : 1)], 4);
-            const float a = odd ? got : v[s][2 * h], b = odd ? v[s][2 * h + 1] : got;
-            const int col = (MODE == GLU ? pair : pair * STRIPS + s) * 16 + h * 8 + (g & 6);
-            if (r >= live || col >= p.n_dim) continue;
-            if (MODE == PAIRS) {   // (an even number of columns, in fp32)
-              *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + col) = make_float2(a, b);
-            } else if (MODE == GLU || p.n_dim % 2 == 0) {
-              *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + col) = Half16<T>::pack(a, b);
-            } else {
-              static_cast<T*>(p.out)[to + col] = Half16<T>::from_float(a);
-              if (col + 1 < p.n_dim) static_cast<T*>(p.out)[to + col + 1] = Half16<T>::from_float(b);
+            for (int h = 0; h < 2; ++h) {
+              const int at = s * 16 + h * 8;
+              if (col + at >= p.n_dim) continue;
+              const float2 f = o[s][h];
+              if (MODE == PAIRS) {   // (an even number of columns, in fp32)
+                *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + at) = f;
+              } else if (MODE == GLU || p.n_dim % 2 == 0) {
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + at) = Half16<T>::pack(f.x, f.y);
+              } else {
+                static_cast<T*>(p.out)[to + at] = Half16<T>::from_float(f.x);
+                if (col + at + 1 < p.n_dim) static_cast<T*>(p.out)[to + at + 1] = Half16<T>::from_float(f.y);
+              }
             }
-          }
+        }
       }
       if (p.wk > 1) compute_sync(n_warps * 32);
     }
@@ -598,7 +636,7 @@ static bool set_warps(Args& a, int nt, bool glu, int64_t matrices, int slots, in
     b.kpb = (a.full_blocks + wk - 1) / wk;
     b.wn = MAX_WARPS / wk;
     while (b.wn / 2 >= pairs) b.wn /= 2;
-    const int red = wk / 2 * b.wn * STRIPS * nt * 32 * int(sizeof(float4));
+    const int red = (wk - 1) * b.wn * STRIPS * nt * 32 * int(sizeof(float4));
     const int fit = (memory - red) / StageShape(a.full_blocks, b.wn * STRIPS, a.full, a.x_rows).bytes;
     b.depth = std::min(std::min(fit, a.n_stages), MAX_DEPTH);
     if (b.depth < std::min(2, a.n_stages) && a.wk > 0) break;   // (the ring of the last try is longer)
@@ -617,14 +655,14 @@ template <typename T, int NT, bool FINE, int MODE>
 static int launch(Args a, cudaStream_t st) {
   auto kern = int4_kernel<T, NT, FINE, MODE>;
   // shared memory of a CTA: an equal share for as many as the registers allow
-  constexpr int share = 227 * 1024 / ctas_per_sm(NT) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 4 * PAIR_WINDOW) - 256;
+  constexpr int share = 227 * 1024 / ctas_per_sm(NT) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 2 * PAIR_WINDOW) - 256;
   a.x_rows = MODE == DENSE ? std::min(a.rows, NT * 8) : NT * 8;
   a.row_chunks = std::max(1, (a.rows + NT * 8 - 1) / (NT * 8));
   const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
   if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
   if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT), share)) return MOE_B200_ERR_UNSUPPORTED;
   const int smem = a.depth * StageShape(a.full_blocks, a.wn * STRIPS, a.full, a.x_rows).bytes +
-                   a.wk / 2 * a.wn * STRIPS * NT * 32 * int(sizeof(float4));
+                   (a.wk - 1) * a.wn * STRIPS * NT * 32 * int(sizeof(float4));
   static PerDevice<cudaError_t> ready;
   int dev = -1;
   const cudaError_t* ok = cudaGetDevice(&dev) != cudaSuccess ? nullptr : ready.get(dev, [&](int) {

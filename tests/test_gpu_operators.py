@@ -400,6 +400,21 @@ def test_int4_experts_activations(act):
                            int4_experts(x, tw, idx, p["w_in"], p["w_out"], "silu"))
 
 
+@pytest.mark.parametrize("t,e", [(30, 1), (30, 2), (8, 1), (64, 2), (200, 8), (1300, 3)])
+def test_int4_experts_place_of_a_row_changes_nothing(t, e):
+    """Tokens in another order, and again: bit for bit the same rows, in whatever place of a tile or pass they come."""
+    d, h = 1024, 64
+    w_in, w_out = quantize_int4(randn(e, d, 2 * h)), quantize_int4(randn(e, h, d, seed=1))
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, idx = randn(t, d, seed=2), torch.randint(0, e, (t, 1), device="cuda", generator=gen)
+    tw = torch.rand(t, 1, device="cuda", generator=gen).to(torch.bfloat16)
+    want = int4_experts(x, tw, idx, w_in, w_out)
+    for seed in range(3):
+        order = torch.randperm(t, device="cuda", generator=gen)
+        assert torch.equal(int4_experts(x[order], tw[order], idx[order], w_in, w_out), want[order])
+        assert torch.equal(int4_experts(x, tw, idx, w_in, w_out), want)
+
+
 def test_int4_experts_windows_of_pairs():
     """More pairs than one look at the expert ids takes, all on one expert or spread."""
     x, tw, idx, packed, plain = experts_case(1500, 64, 16, 5, 3, 1, 64, torch.bfloat16)
@@ -682,17 +697,17 @@ def test_grouped_results_past_two_to_the_31():
 
 
 def test_experts_past_two_to_the_32_levels():
-    """The last of 2300 experts, whose levels lie beyond 2^32, is the expert it is by itself."""
+    """The last of 2300 experts, whose levels lie beyond 2^32, is what the same weights are in the first place."""
     d, h, e = 1024, 1024, 2300
     one_in, one_out = quantize_int4(randn(1, d, 2 * h)), quantize_int4(randn(1, h, d, seed=1))
     many = [Int4Weight(torch.zeros(e, w.data.shape[1], dtype=torch.uint8, device="cuda"), (e, *w.shape[1:]), 64,
                        torch.bfloat16) for w in (one_in, one_out)]
     for big, w in zip(many, (one_in, one_out)):
-        big.data[-1] = w.data[0]
+        big.data[0] = big.data[-1] = w.data[0]
     assert e * d * 2 * h > 2 ** 32
     x, tw = randn(3, d), torch.ones(3, 1, device="cuda", dtype=torch.bfloat16)
     idx = torch.full((3, 1), e - 1, device="cuda")
-    want = int4_experts(x, tw, torch.zeros_like(idx), one_in, one_out)
+    want = int4_experts(x, tw, torch.zeros_like(idx), *many)
     assert torch.equal(int4_experts(x, tw, idx, *many), want) and bool(want.any())
 
 
