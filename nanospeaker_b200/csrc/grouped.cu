@@ -90,20 +90,17 @@ __device__ __forceinline__ void drain_ring(uint64_t* full_bar, uint32_t it) {
     }
 }
 
-// N chunks of 32 accumulator columns from column `col` of the result on, those that start below n_dim: each is
-// read from TMEM while the one before it is stored.
+// N chunks of 32 accumulator columns from column `col` of the result on, those that start below n_dim. (A loop: its
+// code is fetched once; the next chunk's read under this one's stores gained nothing, other warps fill the wait.)
 template <int N, typename Store>
 __device__ __forceinline__ void store_columns(uint32_t taddr, int col, int n_dim, Store store) {
   const int n = min(N, (n_dim - col + 31) / 32);
-  if (n <= 0) return;
-  float v[2][32];
-  tmem_ld32(taddr, v[0]);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (i >= n) break;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    float v[32];
+    tmem_ld32(taddr + i * 32, v);
     tmem_ld_wait();
-    if (i + 1 < n) tmem_ld32(taddr + (i + 1) * 32, v[(i + 1) & 1]);
-    store(col + i * 32, v[i & 1]);
+    store(col + i * 32, v);
   }
 }
 

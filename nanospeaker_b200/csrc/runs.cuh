@@ -14,47 +14,45 @@ struct RunTable {
   int first[RUNS_MAX_GROUPS + 1];   // first work unit of every run, then their number
 };
 
-__device__ __forceinline__ int warp_prefix_sum(int v, int lane) {   // inclusive
-#pragma unroll
+// An exclusive prefix sum (or maximum, from 0 on) over the warp. As a loop: a kernel's first work waits for its
+// code more than for anything else (the table of 76 runs in straight lines took 6000 cycles the first time and 600
+// the second; as it stands, 2000).
+template <bool MAX>
+__device__ __forceinline__ int warp_prefix(int v, int lane, int* all) {
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    if (lane >= o) v = MAX ? max(v, u) : v + u;
   }
-  return v;
+  *all = __shfl_sync(0xffffffffu, v, 31);
+  const int before = __shfl_up_sync(0xffffffffu, v, 1);
+  return lane ? before : 0;
 }
-__device__ __forceinline__ int warp_prefix_max(int v, int lane) {   // inclusive
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v = max(v, u);
-  }
-  return v;
-}
+
+constexpr int RUNS_PER_LANE = 4;
 
 // Starts that decrease or leave [0, rows] cannot reach memory: a start is taken into that range and is at
 // least every earlier one. True when any had to be changed (the caller reports it).
 __device__ __forceinline__ bool load_run_starts(const int32_t* offsets, int n_groups, int rows, int lane,
                                                 int* start) {
-  constexpr int AT_ONCE = 4;   // loads in flight: this is a kernel's first work
   int high = 0;
   bool changed = false;
-  for (int base = 0; base <= n_groups; base += 32 * AT_ONCE) {
-    int raw[AT_ONCE];
+#pragma unroll 1
+  for (int base = lane * RUNS_PER_LANE; base - lane * RUNS_PER_LANE <= n_groups; base += 32 * RUNS_PER_LANE) {
+    int raw[RUNS_PER_LANE], v[RUNS_PER_LANE];
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const int g = base + 32 * i + lane;
-      raw[i] = g <= n_groups ? ld_prev(offsets + g) : 0;
-    }
+    for (int i = 0; i < RUNS_PER_LANE; ++i) raw[i] = ld_prev(offsets + min(base + i, n_groups));
+    int own = 0, all;
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const int g = base + 32 * i + lane;
-      const int v = max(high, warp_prefix_max(min(max(raw[i], 0), rows), lane));
-      if (g <= n_groups) {
-        start[g] = v;
-        changed |= v != raw[i];
-      }
-      high = __shfl_sync(0xffffffffu, v, 31);   // (behind the last start the lanes repeat the highest)
+    for (int i = 0; i < RUNS_PER_LANE; ++i) v[i] = own = max(own, min(raw[i], rows));
+    const int before = max(high, warp_prefix<true>(own, lane, &all));
+#pragma unroll
+    for (int i = 0; i < RUNS_PER_LANE; ++i) {
+      v[i] = max(v[i], before);
+      changed |= v[i] != raw[i];
+      start[min(base + i, n_groups)] = v[i];   // (behind the last start: that one again)
     }
+    high = max(high, all);
   }
   __syncwarp();
   return __any_sync(0xffffffffu, changed);
@@ -65,12 +63,20 @@ template <typename UnitsOf>
 __device__ __forceinline__ int count_run_units(const int* start, int n_groups, int lane, int* first,
                                                UnitsOf units_of) {
   int before = 0;
-  for (int base = 0; base < n_groups; base += 32) {
-    const int g = base + lane;
-    const int own = g < n_groups ? units_of(start[g + 1] - start[g]) : 0;
-    const int upto = warp_prefix_sum(own, lane);
-    if (g < n_groups) first[g] = before + upto - own;
-    before += __shfl_sync(0xffffffffu, upto, 31);
+#pragma unroll 1
+  for (int base = lane * RUNS_PER_LANE; base - lane * RUNS_PER_LANE < n_groups; base += 32 * RUNS_PER_LANE) {
+    int own = 0, all, v[RUNS_PER_LANE];
+#pragma unroll
+    for (int i = 0; i < RUNS_PER_LANE; ++i) {
+      const int g = min(base + i, n_groups - 1);
+      v[i] = own;
+      own += base + i < n_groups ? units_of(start[g + 1] - start[g]) : 0;
+    }
+    const int upto = before + warp_prefix<false>(own, lane, &all);
+#pragma unroll
+    for (int i = 0; i < RUNS_PER_LANE; ++i)
+      if (base + i < n_groups) first[base + i] = upto + v[i];
+    before += all;
   }
   if (lane == 0) first[n_groups] = before;
   __syncwarp();
