@@ -23,6 +23,7 @@
 
 #include "../../include/moe_b200.h"
 #include "act.cuh"
+#include "grouped_order.cuh"
 #include "half16.cuh"
 #include "pdl.cuh"
 #include "per_device.cuh"
@@ -64,6 +65,7 @@ struct Args {
   // GLU / PAIRS: row p of the result is pair p of topk_idx, row n_pairs + s * rows + t token t of shared expert s
   const int64_t* topk_idx;
   int32_t n_pairs, top_k;
+  uint32_t top_k_inv, row_chunks_inv;   // (quotient)
   int32_t row_chunks;          // CTAs that share the rows of a matrix all rows go to (DENSE, shared experts)
   int32_t eager;               // copy before it is known whether the expert has rows
   int32_t act;
@@ -235,8 +237,8 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
 
   // which matrix, and which of its rows
   const int y = MODE == DENSE ? blockIdx.y : int(blockIdx.y) - p.routed.groups;
-  const int chunk = all_rows ? y % p.row_chunks : 0;
-  const int e = MODE == DENSE ? 0 : all_rows ? y / p.row_chunks : int(blockIdx.y);
+  const int e = MODE == DENSE ? 0 : all_rows ? quotient(y, p.row_chunks, p.row_chunks_inv) : int(blockIdx.y);
+  const int chunk = all_rows ? y - e * p.row_chunks : 0;
   const int strip_step = MODE == GLU ? p.strips / 2 : 1;
   const int n_stages = p.n_stages;
   // the row of the result, and of x, that row r of this expert is
@@ -246,7 +248,8 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
     return all_rows ? int64_t(p.n_pairs) + int64_t(e) * p.rows + r : win * PAIR_WINDOW + list[r];
   };
   auto x_row = [&](int r) -> int64_t {
-    return MODE == DENSE ? r : MODE == PAIRS ? out_row(r) : all_rows ? r : (win * PAIR_WINDOW + list[r]) / p.top_k;
+    if (MODE == PAIRS) return out_row(r);
+    return all_rows ? r : quotient(win * PAIR_WINDOW + list[r], p.top_k, p.top_k_inv);
   };
 
   // ---- the copying warps' side. A pass is n_stages stages, the weights the same ones in each; the first of
@@ -450,11 +453,20 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
             scale_in(FINE ? 1 : 0);
           }
         };
-        if (MODE == DENSE && p.kpb == 2 && lb0 + 2 <= blocks && (kb + 2) * 64 <= p.k_dim) {   // (long strips: two side by side)
+        // Two blocks side by side where that pays: in long strips as the one way there is (one row 12.1 us, with the
+        // loop 13.0, as a loop of two 12.9), in experts of few rows as a loop of two (64 tokens 15.1 us, one by one 15.4;
+        // of many rows 53.7 and 52.9).
+        if (MODE == DENSE && p.kpb == 2 && lb0 + 2 <= blocks && (kb + 2) * 64 <= p.k_dim) {
           block(0, false);
           block(1, false);
         } else {
-          for (int j = 0; j < p.kpb && lb0 + j < blocks; ++j, ++kb) block(j, (kb + 1) * 64 > p.k_dim);
+          int j = 0;
+          if (MODE != DENSE && NT == 1)
+            for (; j + 2 <= p.kpb && lb0 + j + 2 <= blocks && (kb + 2) * 64 <= p.k_dim; j += 2, kb += 2) {
+              block(j, false);
+              block(j + 1, false);
+            }
+          for (; j < p.kpb && lb0 + j < blocks; ++j, ++kb) block(j, (kb + 1) * 64 > p.k_dim);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty_bar + slot);
@@ -676,6 +688,7 @@ static int launch(Args a, cudaStream_t st) {
   constexpr int share = 227 * 1024 / ctas_per_sm(NT) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 2 * PAIR_WINDOW) - 256;
   a.x_rows = MODE == DENSE ? std::min(a.rows, NT * 8) : NT * 8;
   a.row_chunks = std::max(1, (a.rows + NT * 8 - 1) / (NT * 8));
+  a.row_chunks_inv = quotient_inverse(a.row_chunks);
   const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
   if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
   if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT), share)) return MOE_B200_ERR_UNSUPPORTED;
@@ -723,6 +736,7 @@ static int experts(const void* x, int64_t ld_x, int64_t n_tokens, int32_t d, int
   a.topk_idx = topk_idx;
   a.n_pairs = n_pairs;
   a.top_k = top_k;
+  a.top_k_inv = quotient_inverse(top_k);
   a.eager = n_pairs >= in.groups;   // (then most experts have rows)
   a.act = act;
   a.out = scratch;
