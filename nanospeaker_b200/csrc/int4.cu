@@ -783,6 +783,7 @@ int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, c
       !q4::group_ok(group))
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
+  if (rows > 65535 * 32) return MOE_B200_ERR_UNSUPPORTED;   // (a grid of 32 rows each)
   if (rows == 0) return MOE_B200_OK;
   if (!x || !w || !y || !status) return MOE_B200_ERR_NULL;
   if (!q4::aligned(x, 16) || !q4::aligned(w, 16) || !q4::aligned(y, n_dim % 2 ? 2 : 4)) return MOE_B200_ERR_ALIGN;

@@ -205,8 +205,8 @@ def _(x, data, group, n_dim):
 def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     """x [..., K] times a weight [K, N] held in 4 bits -> [..., N], in x's dtype (that of the scales).
 
-    Made for few rows: up to 32 read the weight once, more read it once per 32. fp32 sums, rounded
-    once; bitwise reproducible."""
+    Made for few rows: up to 32 read the weight once, more read it once per 32 (65535 * 32 rows at
+    most). fp32 sums, rounded once; bitwise reproducible."""
     if type(weight) is Int4Weight and native_ok(x):
         out = K.shim().int4_mm(x, weight.data, weight.dtype, weight.shape, weight.group)
         if out is not None:

@@ -424,6 +424,8 @@ def test_sizes_whose_places_leave_31_bits_are_refused(lib):
     for tokens, top_k in (((1 << 31) - 1023, 1), (1, (1 << 31) - 1023), ((1 << 33) + 1, 1)):
         assert lib.moe_b200_int4_experts(p, tokens, 8, 8, 16, p, p, top_k, 4, p, p, 0, None, None, 64, 0, 0, p, p,
                                          1 << 62, p, None) == -1
+    for many in (65535 * 32 + 1, (1 << 31) - 1):
+        assert lib.moe_b200_int4_mm(p, many, 8, 8, p, 64, 8, 0, p, p, None) == -5
     from nanospeaker_b200 import grouped_mm
     x, w = torch.empty(4, 1 << 31, device="meta", dtype=torch.bfloat16), torch.empty(
         2, 1 << 31, 8, device="meta", dtype=torch.bfloat16)
