@@ -4,7 +4,8 @@
 //   moe_b200_int4_experts  the block's GLU experts (routed by top-k ids, and shared ones) for a batch that
 //                          generates: up + GLU -> down -> weighted sum, three launches
 //
-// What bounds them is the weights' bytes, so a weight is read once and used for up to 32 rows from registers.
+// What they cannot do without is the weights' bytes, so a weight is read once and used for up to 32 rows from
+// registers; what bounds them is the latency of a CTA's start and of its instructions.
 // The layout (nanospeaker_b200/int4.py packs it) is the matrix instruction's: a lane's 16 bytes are its A
 // fragments (16 outputs x 16 inputs each) of 64 inputs, and the inputs are numbered within those 64 so that
 // the B fragments of a row of x are two 16-byte pieces of it. Levels become 16-bit floats exactly (a byte
@@ -187,8 +188,12 @@ struct StageShape {
 
 // CTAs that an SM holds (their registers and shared memory are sized for it): many at a time, so that one's
 // start and end lie under the others' work, but with the registers for two blocks in the works. One row of 4096 x
-// 16384: at 5 CTAs 15.2 us, at 4 12.5; one token of the experts 11.2 and 10.2.
-__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
+// 16384: at 5 CTAs 14.4 us, at 4 12.1, at 3 15.6. The up projection at 3 (its longer ring holds a pass; one token
+// of the experts 8.4 us, 64 14.2) rather than 4 (8.8, 15.1), the down projection, short strips, at 4 rather than 3
+// (64 tokens 14.8). 32 rows at 3: 21.8 us in place of 12.3.
+__host__ __device__ constexpr int ctas_per_sm(int nt, int mode) {
+  return nt == 1 ? (mode == GLU ? 3 : 4) : nt == 2 ? 3 : 2;
+}
 __host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 
 // A CTA: wn pairs of strips of one matrix (GLU: a pair is a gate strip and its up strip), wk warps on each that
@@ -196,7 +201,7 @@ __host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 // copy. NT: tiles of 8 rows per pass; more rows of one expert take more passes, which copy the weights
 // again. FINE: scale groups of 32 inputs (two per block).
 template <typename T, int NT, bool FINE, int MODE>
-__global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm(NT)) int4_kernel(const Args p) {
+__global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm(NT, MODE)) int4_kernel(const Args p) {
   constexpr int ROWS = NT * 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_bar[MAX_DEPTH], empty_bar[MAX_DEPTH];
@@ -266,7 +271,8 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
   auto issue_weights = [&] {   // (the slot is free)
     const int piece = w_stage == n_stages - 1 ? p.last : p.full;
     if (lane < (MODE == GLU ? 2 : 1)) {
-      const uint8_t* from = matrix + int64_t(w_stage) * p.strips * p.full + int64_t(first_strip + lane * strip_step) * piece;
+      const uint8_t* from = matrix + int64_t(w_stage) * p.strips * p.full +
+                            int64_t(first_strip + lane * strip_step) * piece;
       bulk_load(ring + w_slot * sh.bytes + lane * p.wn * p.full, from, live_strips * piece, full_bar + w_slot);
     }
     ++w_issued;
@@ -407,9 +413,9 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
 #pragma unroll
             for (int k = 0; k < 4; ++k) levels_of<T>(q[k], a[s][k]);
           }
-          // Tiles whose products, independent of one another, are in the works together. Two where all tiles mostly have
-          // rows (64 rows x 4096^2: 13.3 us with one, 12.8 with two); an expert's last tile would often have no partner
-          // (200 tokens: 57.9 us with one, 58.7 with two).
+          // Tiles whose products, independent of one another, are in the works together. Two where all tiles mostly
+          // have rows (64 rows x 4096^2: 13.3 us with one, 12.8 with two); an expert's last tile would often have no
+          // partner (200 tokens: 57.9 us with one, 58.7 with two).
           constexpr int AT = MODE == DENSE && NT > 1 ? 2 : 1;
 #pragma unroll
           for (int i0 = 0; i0 < NT; i0 += AT) {
@@ -454,8 +460,8 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
           }
         };
         // Two blocks side by side where that pays: in long strips as the one way there is (one row 12.1 us, with the
-        // loop 13.0, as a loop of two 12.9), in experts of few rows as a loop of two (64 tokens 15.1 us, one by one 15.4;
-        // of many rows 53.7 and 52.9).
+        // loop 13.0, as a loop of two 12.9), in experts of few rows as a loop of two (64 tokens 15.1 us, one by one
+        // 15.4; of many rows 53.7 and 52.9).
         if (MODE == DENSE && p.kpb == 2 && lb0 + 2 <= blocks && (kb + 2) * 64 <= p.k_dim) {
           block(0, false);
           block(1, false);
@@ -685,13 +691,14 @@ template <typename T, int NT, bool FINE, int MODE>
 static int launch(Args a, cudaStream_t st) {
   auto kern = int4_kernel<T, NT, FINE, MODE>;
   // shared memory of a CTA: an equal share for as many as the registers allow
-  constexpr int share = 227 * 1024 / ctas_per_sm(NT) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 2 * PAIR_WINDOW) - 256;
+  constexpr int share =
+      227 * 1024 / ctas_per_sm(NT, MODE) / 1024 * 1024 - 1024 - (MODE == DENSE ? 0 : 2 * PAIR_WINDOW) - 256;
   a.x_rows = MODE == DENSE ? std::min(a.rows, NT * 8) : NT * 8;
   a.row_chunks = std::max(1, (a.rows + NT * 8 - 1) / (NT * 8));
   a.row_chunks_inv = quotient_inverse(a.row_chunks);
   const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
   if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
-  if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT), share)) return MOE_B200_ERR_UNSUPPORTED;
+  if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT, MODE), share)) return MOE_B200_ERR_UNSUPPORTED;
   const int smem = a.depth * StageShape(a.full_blocks, a.wn * STRIPS, a.full, a.x_rows).bytes +
                    (a.wk - 1) * a.wn * STRIPS * NT * 32 * int(sizeof(float4));
   static PerDevice<cudaError_t> ready;
@@ -700,8 +707,8 @@ static int launch(Args a, cudaStream_t st) {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, share);
   });
   if (ok == nullptr || *ok != cudaSuccess || smem > share) return MOE_B200_ERR_CUDA;
-  return launch_pdl(kern, dim3(ctas_for(a, MODE == GLU), unsigned(ys)), dim3((a.wk * a.wn + copy_warps(NT)) * 32), size_t(smem), st,
-                    a) == cudaSuccess
+  return launch_pdl(kern, dim3(ctas_for(a, MODE == GLU), unsigned(ys)),
+                    dim3((a.wk * a.wn + copy_warps(NT)) * 32), size_t(smem), st, a) == cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
 }
