@@ -733,3 +733,31 @@ def test_int4_mm_many_rows():
     y = int4_mm(x, w)
     ew = exact_weight(q, s, 64)
     within(y, x.double() @ ew, 128, x.double().abs() @ ew.abs())
+
+
+# --------------------------------------------------------------------------- two calls at once
+def test_calls_on_two_streams_at_once():
+    """The operators on two streams that do not wait for one another, fifty times: what each gives alone."""
+    x, w = randn(900, 256), randn(6, 256, 192, seed=1)
+    off = torch.tensor([0, 300, 300, 305, 705, 800, 900], dtype=torch.int32, device="cuda")
+    dy = randn(900, 192, seed=2)
+    d, h, e = 576, 128, 16
+    w_in, w_out = quantize_int4(randn(e, d, 2 * h)), quantize_int4(randn(e, h, d, seed=1))
+    t, tw = randn(40, d, seed=3), torch.full((40, 4), 0.25, device="cuda", dtype=torch.bfloat16)
+    idx = torch.rand(40, e, device="cuda").topk(4).indices
+    rng = torch.tensor([3, 4], device="cuda")
+    calls = [lambda: grouped_mm(x, w, off), lambda: kernels.grouped_wgrad(x, dy, off),
+             lambda: int4_experts(t, tw, idx, w_in, w_out), lambda: dropout_add(x, None, 0.5, rng)]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(50):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append([c() for c in (calls if i % 4 < 2 else calls[::-1])])
+    torch.cuda.synchronize()
+    for i, outs in enumerate(got):
+        for a, b in zip(outs if i % 4 < 2 else outs[::-1], want):
+            assert torch.equal(a, b)
+    kernels.check_status("cuda")
