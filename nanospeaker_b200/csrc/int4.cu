@@ -10,8 +10,11 @@
 // fragments (16 outputs x 16 inputs each) of 64 inputs, and the inputs are numbered within those 64 so that
 // the B fragments of a row of x are two 16-byte pieces of it. Levels become 16-bit floats exactly (a byte
 // operation and a subtraction per two), products are summed in fp32 over one scale group at a time, and the
-// scale is applied to that sum: no rounding but the final one (and the GLU's result, which is held in the
-// activations' type between the two products).
+// scale is applied to that sum: no rounding but the final one. The GLU's result has to be an operand of the matrix
+// instruction again: it is held as two bf16 numbers, its upper half and what is left (2^-15 of the value at most is
+// lost, and fp32's range kept), and the down projection multiplies its levels, exact in bf16 too, with both. Held in
+// the activations' type it cost as much again as the rounding of the result (relative error against 64 bits: bf16
+// 0.0024 to 0.0027 in place of 0.0017, fp16 0.00029 in place of 0.00021).
 //
 // A chunk of 512 inputs of neighbouring strips (16 outputs each), levels and scales together, is one contiguous
 // piece: it comes to shared memory by one bulk copy (which costs the SM's copy engine some 50 cycles however
@@ -21,6 +24,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/moe_b200.h"
 #include "act.cuh"
@@ -47,20 +51,23 @@ struct Stack {
 };
 
 enum Mode { DENSE = 0, GLU = 1, PAIRS = 2 };
+// Numbers that a value of x is held in: the GLU's result, which the down projection reads, is two bf16 values.
+__host__ __device__ constexpr int parts_of(int mode) { return mode == PAIRS ? 2 : 1; }
 
 struct Args {
-  const void* x;
+  const void* x;               // PAIRS: [k_dim upper halves | k_dim rests] a row
   int64_t ld_x;
   Stack routed, shared;
   int32_t k_dim, n_dim;        // valid inputs and outputs (GLU: outputs = the hidden width)
   int32_t kblocks, strips;     // of both stacks
   int32_t group_shift;         // scale group = 32 << group_shift inputs
-  int32_t n_stages, depth;     // chunks of a strip = stages of a pass; stages of the ring
-  int32_t full_blocks, last_blocks;   // blocks of a chunk, of the last one
-  int32_t full, last;          // bytes of a strip's piece of a chunk
+  int32_t n_stages, depth;     // stages of a pass over a strip, each a chunk (halves: half of one); of the ring
+  int32_t full_blocks, last_blocks;   // blocks of a stage, of the last one
+  int32_t full, last;          // bytes of a strip's piece of a stage
+  int32_t halves, chunk;       // bytes of a strip's piece of a whole chunk
   int64_t matrix;              // bytes of a matrix
   int32_t wk, wn, kpb;         // warps that share a strip's inputs, pairs of strips per CTA, blocks of a warp
-                               // in a chunk
+                               // in a stage
   int32_t x_rows;              // rows of x that a stage has room for
   int32_t rows;                // DENSE: rows of x; else tokens
   // GLU / PAIRS: row p of the result is pair p of topk_idx, row n_pairs + s * rows + t token t of shared expert s
@@ -70,7 +77,7 @@ struct Args {
   int32_t row_chunks;          // CTAs that share the rows of a matrix all rows go to (DENSE, shared experts)
   int32_t eager;               // copy before it is known whether the expert has rows
   int32_t act;
-  void* out;                   // DENSE [rows, n_dim], GLU [n_pairs + S * rows, n_dim] of T; PAIRS fp32
+  void* out;                   // DENSE [rows, n_dim] of T, GLU [n_pairs + S * rows, 2, n_dim] bf16; PAIRS fp32
   int64_t ld_out;
   int32_t* status;
 };
@@ -163,6 +170,15 @@ __device__ __noinline__ float4 activation(int act, float4 g) {
   }
 }
 
+// Two values as pairs of bf16: their upper halves (cut, so that nothing finite becomes an infinity) and the rests,
+// rounded (of an infinity nothing: it would be infinity less infinity).
+__device__ __forceinline__ void split(const float2& v, uint32_t& upper, uint32_t& rest) {
+  const uint32_t x = __float_as_uint(v.x), y = __float_as_uint(v.y);
+  upper = __byte_perm(x, y, 0x7632);
+  auto left = [](float f, uint32_t bits) { return isinf(f) ? 0.f : f - __uint_as_float(bits & 0xFFFF0000u); };
+  rest = Half16<__nv_bfloat16>::pack(left(v.x, x), left(v.y, y));
+}
+
 __device__ __forceinline__ uint32_t ld_shared_b32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
@@ -177,22 +193,29 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// A stage of the ring, a chunk of up to `blocks` blocks: the strips' pieces, then the rows of x. A row's 16-byte
+// Bytes of a strip's piece of `blocks` blocks: levels, and scales of groups of 32 << group_shift inputs.
+__host__ __device__ constexpr int piece_bytes(int blocks, int group_shift) {
+  return blocks * 512 + (((2 * blocks - 1) >> group_shift) + 1) * 32;
+}
+
+// A stage of the ring, up to `blocks` blocks: the strips' pieces, then the rows of x. A row's 16-byte
 // piece c lies at c, in odd rows at c ^ 4: the two rows that a quarter of a warp reads at a time then lie in
-// different banks.
+// different banks. A row of two parts has the second one behind the first.
 struct StageShape {
   int x, row, bytes;
-  __host__ __device__ StageShape(int blocks, int strips, int piece, int rows)
-      : x((strips * piece + 127) / 128 * 128), row(blocks * 128), bytes((x + rows * row + 127) / 128 * 128) {}
+  __host__ __device__ StageShape(int blocks, int strips, int piece, int rows, int parts)
+      : x((strips * piece + 127) / 128 * 128), row(blocks * 128 * parts), bytes((x + rows * row + 127) / 128 * 128) {}
 };
 
 // CTAs that an SM holds (their registers and shared memory are sized for it): many at a time, so that one's
 // start and end lie under the others' work, but with the registers for two blocks in the works. One row of 4096 x
 // 16384: at 5 CTAs 14.4 us, at 4 12.1, at 3 15.6. The up projection at 3 (its longer ring holds a pass; one token
 // of the experts 8.4 us, 64 14.2) rather than 4 (8.8, 15.1), the down projection, short strips, at 4 rather than 3
-// (64 tokens 14.8). 32 rows at 3: 21.8 us in place of 12.3.
+// (64 tokens 14.8 and 15.4, though it leaves 24 to 60 bytes of a thread's registers in memory). Two tiles: dense at
+// 3, the experts at 2 (64 tokens of the wide block 30.9 us, at 3, with 56 to 220 bytes in memory, 42.5). Four tiles at
+// 2: at 3 32 rows took 21.8 us in place of 12.3.
 __host__ __device__ constexpr int ctas_per_sm(int nt, int mode) {
-  return nt == 1 ? (mode == GLU ? 3 : 4) : nt == 2 ? 3 : 2;
+  return nt == 1 ? (mode == GLU ? 3 : 4) : nt == 2 && mode == DENSE ? 3 : 2;
 }
 __host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 
@@ -202,7 +225,8 @@ __host__ __device__ constexpr int copy_warps(int nt) { return nt == 1 ? 1 : 2; }
 // again. FINE: scale groups of 32 inputs (two per block).
 template <typename T, int NT, bool FINE, int MODE>
 __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm(NT, MODE)) int4_kernel(const Args p) {
-  constexpr int ROWS = NT * 8;
+  constexpr int ROWS = NT * 8, PARTS = parts_of(MODE);
+  using X = std::conditional_t<MODE == PAIRS, __nv_bfloat16, T>;   // what the rows of x are held in
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_bar[MAX_DEPTH], empty_bar[MAX_DEPTH];
   __shared__ uint16_t list[MODE == DENSE ? 1 : PAIR_WINDOW];   // places in the window
@@ -210,7 +234,7 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_warps = p.wk * p.wn;
   constexpr int COPY_WARPS = copy_warps(NT);
-  const StageShape sh(p.full_blocks, p.wn * STRIPS, p.full, p.x_rows);
+  const StageShape sh(p.full_blocks, p.wn * STRIPS, p.full, p.x_rows, PARTS);
   float4* red = reinterpret_cast<float4*>(smem + p.depth * sh.bytes);   // [wk - 1][wn][STRIPS * NT][32 lanes]
 
   if (threadIdx.x == 0) {
@@ -269,8 +293,22 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
   int x_issued = 0, x_stage = 0, x_slot = 0, x_phase = 1;   // (phase: of the slot's release before)
   bool dead = false;
   auto issue_weights = [&] {   // (the slot is free)
-    const int piece = w_stage == n_stages - 1 ? p.last : p.full;
-    if (lane < (MODE == GLU ? 2 : 1)) {
+    const bool last = w_stage == n_stages - 1;
+    const int piece = last ? p.last : p.full;
+    if (MODE == PAIRS && p.halves) {   // (a strip's levels and its scales lie apart)
+      if (lane < 2 * live_strips) {
+        const int at = w_stage >> 1, half = w_stage & 1, blocks = min(CHUNK, p.kblocks - at * CHUNK);
+        const int strip = lane >> 1, levels = (last ? p.last_blocks : p.full_blocks) * 512;
+        const uint8_t* from = matrix + int64_t(at) * p.strips * p.chunk +
+                              int64_t(first_strip + strip) * piece_bytes(blocks, p.group_shift);
+        const uint32_t to = ring + w_slot * sh.bytes + strip * piece;
+        if (lane & 1)
+          bulk_load(to + levels, from + blocks * 512 + half * (CHUNK >> p.group_shift) * 32, piece - levels,
+                    full_bar + w_slot);
+        else
+          bulk_load(to, from + half * (CHUNK / 2 * 512), levels, full_bar + w_slot);
+      }
+    } else if (lane < (MODE == GLU ? 2 : 1)) {
       const uint8_t* from = matrix + int64_t(w_stage) * p.strips * p.full +
                             int64_t(first_strip + lane * strip_step) * piece;
       bulk_load(ring + w_slot * sh.bytes + lane * p.wn * p.full, from, live_strips * piece, full_bar + w_slot);
@@ -280,7 +318,7 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
     if (++w_slot == p.depth) w_slot = 0;
   };
   // `row`: lane r's row r of x; rows 0: the stage's weights alone
-  auto issue_stage = [&](const T* row, int rows) {
+  auto issue_stage = [&](const X* row, int rows) {
     if (x_issued >= p.depth) {
       if (!mbar_wait(empty_bar + x_slot, x_phase, p.status)) dead = true;
       dead = __any_sync(0xffffffffu, dead);
@@ -296,11 +334,14 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
     const int pieces = min(p.full_blocks * 8, (p.k_dim - at) / 8);
     const uint32_t to = ring + x_slot * sh.bytes + sh.x;
     for (int r = copier; r < rows; r += COPY_WARPS) {
-      const T* from = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r)) + at;
+      const X* from = reinterpret_cast<const X*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r)) + at;
 #pragma unroll
-      for (int h = 0; h < CHUNK * 8 / 32; ++h)
-        if (lane + 32 * h < pieces)
-          cp_async_16(to + r * sh.row + (((lane + 32 * h) ^ ((r & 1) << 2)) << 4), from + (lane + 32 * h) * 8, 16);
+      for (int part = 0; part < PARTS; ++part, from += p.k_dim)
+#pragma unroll
+        for (int h = 0; h < CHUNK * 8 / 32; ++h)
+          if (lane + 32 * h < pieces)
+            cp_async_16(to + r * sh.row + part * (p.full_blocks * 128) + (((lane + 32 * h) ^ ((r & 1) << 2)) << 4),
+                        from + (lane + 32 * h) * 8, 16);
     }
     cp_async_arrive(full_bar + x_slot);
     ++x_issued;
@@ -360,7 +401,7 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
     if (copier >= 0) {
       for (int r0 = first; r0 < n_rows && !dead; r0 += ROWS) {
         const int rows = min(ROWS, n_rows - r0);
-        const T* row = static_cast<const T*>(p.x) + (lane < rows ? x_row(r0 + lane) * p.ld_x : 0);
+        const X* row = static_cast<const X*>(p.x) + (lane < rows ? x_row(r0 + lane) * p.ld_x : 0);
         for (int i = 0; i < n_stages && !dead; ++i) issue_stage(row, rows);
       }
       if (dead && lane == 0) atomicExch(p.status, ST_WAIT_TIMEOUT);
@@ -411,7 +452,7 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
 #pragma unroll
             for (int h = 0; h < (FINE ? 2 : 1); ++h) sc[s][h] = ld_shared_b32(s_of + s * strip + h * 32);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) levels_of<T>(q[k], a[s][k]);
+            for (int k = 0; k < 4; ++k) levels_of<X>(q[k], a[s][k]);
           }
           // Tiles whose products, independent of one another, are in the works together. Two where all tiles mostly
           // have rows (64 rows x 4096^2: 13.3 us with one, 12.8 with two); an expert's last tile would often have no
@@ -420,18 +461,22 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
 #pragma unroll
           for (int i0 = 0; i0 < NT; i0 += AT) {
             if (i0 > 0 && i0 >= tiles) break;
-            uint4 b0[AT], b1[AT];
+            uint4 x[2][PARTS][AT];   // a lane's pieces of the block's first and second half
             float c[AT][STRIPS][4] = {};
 #pragma unroll
-            for (int i = 0; i < AT; ++i) {
-              ld_shared_v4(x_at[i0 + i] + j * 128, b0[i].x, b0[i].y, b0[i].z, b0[i].w);
-              ld_shared_v4(x_at[i0 + i] + j * 128 + other[i0 + i], b1[i].x, b1[i].y, b1[i].z, b1[i].w);
-              if (cut) {
-                const int k = kb * 64 + t * 8;
-                if (k >= p.k_dim) b0[i] = make_uint4(0, 0, 0, 0);
-                if (k + 32 >= p.k_dim) b1[i] = make_uint4(0, 0, 0, 0);
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+              for (int i = 0; i < AT; ++i) {
+                const uint32_t at = x_at[i0 + i] + j * 128 + part * (p.full_blocks * 128);
+                uint4 &u = x[0][part][i], &v = x[1][part][i];
+                ld_shared_v4(at, u.x, u.y, u.z, u.w);
+                ld_shared_v4(at + other[i0 + i], v.x, v.y, v.z, v.w);
+                if (cut) {
+                  const int k = kb * 64 + t * 8;
+                  if (k >= p.k_dim) u = make_uint4(0, 0, 0, 0);
+                  if (k + 32 >= p.k_dim) v = make_uint4(0, 0, 0, 0);
+                }
               }
-            }
             auto each = [&](auto f) {
 #pragma unroll
               for (int i = 0; i < AT; ++i)
@@ -447,15 +492,18 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
                 acc[s][i0 + i][3] += f.y * c[i][s][3];
               });
             };
-            each([&](int i, int s) { Mma<T>::first(c[i][s], a[s][0], b0[i].x, b0[i].y); });
-            each([&](int i, int s) { Mma<T>::run(c[i][s], a[s][1], b0[i].z, b0[i].w); });
-            if constexpr (FINE) {
-              scale_in(0);
-              each([&](int i, int s) { Mma<T>::first(c[i][s], a[s][2], b1[i].x, b1[i].y); });
-            } else {
-              each([&](int i, int s) { Mma<T>::run(c[i][s], a[s][2], b1[i].x, b1[i].y); });
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (FINE && k == 2) scale_in(0);
+#pragma unroll
+              for (int part = 0; part < PARTS; ++part)
+                each([&](int i, int s) {
+                  const uint4& v = x[k / 2][part][i];
+                  const uint32_t lo = k % 2 ? v.z : v.x, hi = k % 2 ? v.w : v.y;
+                  if (part == 0 && (k == 0 || (FINE && k == 2))) Mma<X>::first(c[i][s], a[s][k], lo, hi);
+                  else Mma<X>::run(c[i][s], a[s][k], lo, hi);
+                });
             }
-            each([&](int i, int s) { Mma<T>::run(c[i][s], a[s][3], b1[i].z, b1[i].w); });
             scale_in(FINE ? 1 : 0);
           }
         };
@@ -565,7 +613,10 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
               const float2 f = o[s][h];
               if (MODE == PAIRS) {   // (an even number of columns, in fp32)
                 *reinterpret_cast<float2*>(static_cast<float*>(p.out) + to + at) = f;
-              } else if (MODE == GLU || p.n_dim % 2 == 0) {
+              } else if (MODE == GLU) {
+                __nv_bfloat16* h = static_cast<__nv_bfloat16*>(p.out) + to + at;
+                split(f, *reinterpret_cast<uint32_t*>(h), *reinterpret_cast<uint32_t*>(h + p.n_dim));
+              } else if (p.n_dim % 2 == 0) {
                 *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + to + at) = Half16<T>::pack(f.x, f.y);
               } else {
                 static_cast<T*>(p.out)[to + at] = Half16<T>::from_float(f.x);
@@ -647,24 +698,31 @@ __global__ void __launch_bounds__(128)
   if (!waited) pdl_wait();
 }
 
-static void set_shape(Args& a, int32_t k_dim, int32_t n_dim, int32_t n_cols, int32_t group) {
+static void set_shape(Args& a, int mode, int32_t k_dim, int32_t n_dim, int32_t n_cols, int32_t group) {
   a.k_dim = k_dim;
   a.n_dim = n_dim;
   a.kblocks = (k_dim + 63) / 64;
   a.strips = (n_cols + 15) / 16;
   a.group_shift = group == 32 ? 0 : group == 64 ? 1 : 2;
-  a.n_stages = (a.kblocks + CHUNK - 1) / CHUNK;
-  a.full_blocks = std::min(CHUNK, a.kblocks);
-  a.last_blocks = a.kblocks - (a.n_stages - 1) * CHUNK;
-  auto piece = [&](int blocks) { return blocks * 512 + (((2 * blocks - 1) >> a.group_shift) + 1) * 32; };
-  a.full = piece(a.full_blocks);
-  a.last = piece(a.last_blocks);
+  auto stages = [&](int blocks) {
+    a.n_stages = (a.kblocks + blocks - 1) / blocks;
+    a.full_blocks = std::min(blocks, a.kblocks);
+    a.last_blocks = a.kblocks - (a.n_stages - 1) * blocks;
+    a.full = piece_bytes(a.full_blocks, a.group_shift);
+    a.last = piece_bytes(a.last_blocks, a.group_shift);
+  };
+  stages(CHUNK);
+  a.chunk = a.full;
   a.matrix = int64_t(a.strips) * (int64_t(a.n_stages - 1) * a.full + a.last);
+  // Rows in two parts fill a stage of whole chunks: of 32 rows one such stage fits, which is then copied and
+  // multiplied in turns (200 tokens of the wide block 70.2 us; with halves, two of which are in the ring, 57.6).
+  a.halves = mode == PAIRS && a.kblocks > CHUNK / 2;
+  if (a.halves) stages(CHUNK / 2);
 }
 // How a CTA's warps divide the work: on a strip's inputs where it has that many blocks; on more strips, which
 // share the rows of x, where the grid is more than the SMs hold at a time. False: no stage fits `memory`.
-static bool set_warps(Args& a, int nt, bool glu, int64_t matrices, int slots, int memory) {
-  const int pairs = glu ? a.strips / 2 : (a.strips + 1) / 2;
+static bool set_warps(Args& a, int nt, int mode, int64_t matrices, int slots, int memory) {
+  const int pairs = mode == GLU ? a.strips / 2 : (a.strips + 1) / 2;
   for (int wk = 4; wk > 0; wk /= 2) {
     if (wk > a.kblocks && wk > 1) continue;
     Args b = a;
@@ -672,13 +730,18 @@ static bool set_warps(Args& a, int nt, bool glu, int64_t matrices, int slots, in
     b.kpb = (a.full_blocks + wk - 1) / wk;
     b.wn = MAX_WARPS / wk;
     while (b.wn / 2 >= pairs) b.wn /= 2;
+    const int64_t ctas = (pairs + b.wn - 1) / b.wn * matrices;
     const int red = (wk - 1) * b.wn * STRIPS * nt * 32 * int(sizeof(float4));
-    const int fit = (memory - red) / StageShape(a.full_blocks, b.wn * STRIPS, a.full, a.x_rows).bytes;
+    const int fit = (memory - red) / StageShape(a.full_blocks, b.wn * STRIPS, a.full, a.x_rows, parts_of(mode)).bytes;
     b.depth = std::min(std::min(fit, a.n_stages), MAX_DEPTH);
     if (b.depth < std::min(2, a.n_stages) && a.wk > 0) break;   // (the ring of the last try is longer)
     if (b.depth < 1) return false;
+    // A warp alone on its strips pays where the rows come in one pass (200 tokens of the wide block 57.6 us, with two
+    // warps 60.1); in several passes only where the SMs stay full (256 tokens, two of eight experts of 1536 x 1024:
+    // 79.7 us on 192 CTAs, 66.7 on 384).
+    if (wk == 1 && a.wk > 0 && mode == PAIRS && a.n_pairs > a.routed.groups * nt * 8 && ctas < slots) break;
     a = b;
-    if ((pairs + b.wn - 1) / b.wn * matrices <= slots) break;
+    if (ctas <= slots) break;
   }
   return true;
 }
@@ -698,8 +761,8 @@ static int launch(Args a, cudaStream_t st) {
   a.row_chunks_inv = quotient_inverse(a.row_chunks);
   const int64_t ys = MODE == DENSE ? a.row_chunks : a.routed.groups + int64_t(a.shared.groups) * a.row_chunks;
   if (ys > 65535) return MOE_B200_ERR_UNSUPPORTED;
-  if (!set_warps(a, NT, MODE == GLU, ys, 148 * ctas_per_sm(NT, MODE), share)) return MOE_B200_ERR_UNSUPPORTED;
-  const int smem = a.depth * StageShape(a.full_blocks, a.wn * STRIPS, a.full, a.x_rows).bytes +
+  if (!set_warps(a, NT, MODE, ys, 148 * ctas_per_sm(NT, MODE), share)) return MOE_B200_ERR_UNSUPPORTED;
+  const int smem = a.depth * StageShape(a.full_blocks, a.wn * STRIPS, a.full, a.x_rows, parts_of(MODE)).bytes +
                    (a.wk - 1) * a.wn * STRIPS * NT * 32 * int(sizeof(float4));
   static PerDevice<cudaError_t> ready;
   int dev = -1;
@@ -738,7 +801,7 @@ static int experts(const void* x, int64_t ld_x, int64_t n_tokens, int32_t d, int
   a.ld_x = ld_x;
   a.routed = in;
   a.shared = in_sh;
-  set_shape(a, d, h, 2 * h, group);
+  set_shape(a, GLU, d, h, 2 * h, group);
   a.rows = int32_t(n_tokens);
   a.topk_idx = topk_idx;
   a.n_pairs = n_pairs;
@@ -747,15 +810,15 @@ static int experts(const void* x, int64_t ld_x, int64_t n_tokens, int32_t d, int
   a.eager = n_pairs >= in.groups;   // (then most experts have rows)
   a.act = act;
   a.out = scratch;
-  a.ld_out = h;
+  a.ld_out = 2 * int64_t(h);
   a.status = status;
   int rc = launch_for<T, GLU>(a, rows, st);
   if (rc != MOE_B200_OK) return rc;
   a.x = scratch;
-  a.ld_x = h;
+  a.ld_x = 2 * int64_t(h);
   a.routed = down;
   a.shared = down_sh;
-  set_shape(a, h, d, d, group);
+  set_shape(a, PAIRS, h, d, d, group);
   a.out = y;
   a.ld_out = d;
   rc = launch_for<T, PAIRS>(a, rows, st);
@@ -780,7 +843,7 @@ extern "C" {
 size_t moe_b200_int4_bytes(int32_t k_dim, int32_t n_dim, int32_t group) {
   if (k_dim < 8 || k_dim % 8 || n_dim < 1 || !q4::group_ok(group)) return 0;
   q4::Args a{};
-  q4::set_shape(a, k_dim, n_dim, n_dim, group);
+  q4::set_shape(a, q4::DENSE, k_dim, n_dim, n_dim, group);
   return size_t(a.matrix);
 }
 
@@ -798,7 +861,7 @@ int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, c
   a.x = x;
   a.ld_x = ld_x;
   a.routed = {static_cast<const uint8_t*>(w), 1};
-  q4::set_shape(a, k_dim, n_dim, n_dim, group);
+  q4::set_shape(a, q4::DENSE, k_dim, n_dim, n_dim, group);
   a.rows = int32_t(rows);
   a.out = y;
   a.ld_out = n_dim;
@@ -808,12 +871,15 @@ int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, c
                                 : q4::launch_for<__half, q4::DENSE>(a, rows, st);
 }
 
+static size_t int4_hidden_bytes(int64_t n_tokens, int32_t top_k, int32_t n_shared, int32_t d_hidden) {
+  return (size_t(n_tokens) * (size_t(top_k) + size_t(n_shared)) * size_t(d_hidden) * 4 + 255) / 256 * 256;
+}
+
 size_t moe_b200_int4_experts_scratch_bytes(int64_t n_tokens, int32_t top_k, int32_t n_shared, int32_t d_model,
                                            int32_t d_hidden) {
   if (n_tokens < 0 || top_k < 0 || n_shared < 0 || d_model < 1 || d_hidden < 1) return 0;
-  const size_t rows = size_t(n_tokens) * size_t(top_k + n_shared);
-  const size_t hid = (rows * size_t(d_hidden) * 2 + 255) / 256 * 256;
-  return hid + rows * size_t(d_model) * sizeof(float);
+  return int4_hidden_bytes(n_tokens, top_k, n_shared, d_hidden) +
+         size_t(n_tokens) * (size_t(top_k) + size_t(n_shared)) * size_t(d_model) * sizeof(float);
 }
 
 int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t d_model, int32_t d_hidden,
@@ -837,7 +903,7 @@ int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t
     return MOE_B200_ERR_ALIGN;
   const size_t need = moe_b200_int4_experts_scratch_bytes(n_tokens, top_k, n_shared, d_model, d_hidden);
   if (!scratch || scratch_bytes < need) return MOE_B200_ERR_SCRATCH;
-  const size_t hid = (size_t(n_tokens) * size_t(top_k + n_shared) * size_t(d_hidden) * 2 + 255) / 256 * 256;
+  const size_t hid = int4_hidden_bytes(n_tokens, top_k, n_shared, d_hidden);
   auto stack = [](const void* w, int32_t n) { return q4::Stack{static_cast<const uint8_t*>(w), n}; };
   const q4::Stack in = stack(w_in, n_experts), down = stack(w_out, n_experts);
   const q4::Stack in_sh = stack(w_sh_in, n_shared), down_sh = stack(w_sh_out, n_shared);

@@ -246,8 +246,8 @@ def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, 
     shared_*  the same for the always-on experts, [S, D, 2H] and [S, H, D]
 
     No dispatch comes before it and nothing synchronises: made for batches that generate. An id outside
-    [0, E) adds nothing and is reported by `kernels.check_status`. fp32 sums; the GLU's result is held in
-    x's dtype; bitwise reproducible."""
+    [0, E) adds nothing and is reported by `kernels.check_status`. fp32 sums; the GLU's result keeps
+    fp32's range and 16 bits or more; one rounding to x's dtype at the end; bitwise reproducible."""
     act = _act_id(activation)
     if native_ok(x):
         plain = _experts_fit(w_in, w_out, shared_in, shared_out)

@@ -1,0 +1,85 @@
+"""The operators beside the block where the larger tests' bounds are too wide to see: inputs chosen so that all
+sums but the one under test are exact, calls behind a reported one, and what is refused on the GPU."""
+import pytest
+import torch
+
+from nanospeaker_b200 import Int4Weight, int4_experts, kernels
+
+pytestmark = pytest.mark.gpu
+
+HALF = (torch.bfloat16, torch.float16)
+
+
+def whole(lo, hi, *shape, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randint(lo, hi + 1, shape, generator=g, device="cuda")
+
+
+# --------------------------------------------------------------------------- 4-bit experts: the hidden values
+def whole_experts(t, d, h, e, group, dtype, reach=2):
+    """Whole numbers throughout, rows of -reach .. reach: gates and hidden values (relu) are exact in fp32. Returns
+    the call's arguments, the hidden values of every token and w_out's rows that they meet, in 64 bits."""
+    x = whole(-reach, reach, t, d)
+    q_in, q_out = whole(0, 15, e, d, 2 * h, seed=1), whole(0, 15, e, h, d, seed=2)
+    s_in = torch.ones(e, -(-d // group), 2 * h, dtype=dtype, device="cuda")
+    s_out = torch.full((e, -(-h // group), d), 2.0 ** -14, dtype=dtype, device="cuda")
+    idx = whole(0, e - 1, t, 1, seed=3)
+    pack = lambda q, s: Int4Weight.from_levels(q.to(torch.uint8), s, group)  # noqa: E731
+    args = (x.to(dtype), torch.ones(t, 1, dtype=dtype, device="cuda"), idx, pack(q_in, s_in), pack(q_out, s_out))
+    hid = torch.empty(t, h, dtype=torch.float64, device="cuda")
+    down = torch.empty(t, h, d, dtype=torch.float64, device="cuda")
+    for i in range(e):
+        tok = (idx[:, 0] == i).nonzero()[:, 0]
+        gate, up = (x[tok].double() @ (q_in[i] - 8).double()).chunk(2, 1)
+        hid[tok] = gate.clamp(min=0) * up
+        down[tok] = (q_out[i] - 8).double() * 2.0 ** -14
+    return args, hid, down
+
+
+def hidden_bound(args, hid, down):
+    """(distance of the call's result from 64 bits, its bound, the result in 64 bits). The hidden value loses at most
+    2^-15 of itself (its upper half is cut at 2^-7 of it, the rest rounded at 2^-8 of that); the second product's
+    sum, two parts of h values and a scale per group, is off by 4 h 2^-23 of its magnitude; then one rounding."""
+    assert bool((hid.abs() <= 2 ** 24).all())
+    h, f = hid.shape[1], torch.finfo(args[0].dtype)
+    exact = torch.einsum("th,thd->td", hid, down)
+    magnitude = torch.einsum("th,thd->td", hid.abs(), down.abs())
+    a = (4 * h * 2.0 ** -23 + 2.0 ** -15) * magnitude
+    out = int4_experts(*args, "relu").double()
+    kernels.check_status("cuda")
+    return (out - exact).abs(), f.eps / 2 * (exact.abs() + a) + a + f.smallest_normal * f.eps, exact
+
+
+@pytest.mark.parametrize("t,e", [(1, 1), (5, 2), (24, 2), (100, 3), (300, 4)])
+@pytest.mark.parametrize("d,h,group", [(64, 16, 32), (64, 128, 64), (72, 272, 128), (64, 528, 64), (64, 720, 32)])
+@pytest.mark.parametrize("dtype", HALF)
+def test_int4_experts_hidden_values_are_not_held_in_the_type(t, e, d, h, group, dtype):
+    """Bits below the type's: a bf16 hidden value does not hold the bound (in fp16 its 2^-11, summed up with
+    either sign, may)."""
+    args, hid, down = whole_experts(t, d, h, e, group, dtype)
+    off, bound, exact = hidden_bound(args, hid, down)
+    assert bool((off <= bound).all())
+    if dtype == torch.bfloat16 and t * h >= 1000:
+        held = torch.einsum("th,thd->td", hid.to(dtype).double(), down).to(dtype).double()
+        assert not bool(((held - exact).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("t,h", [(5, 128), (60, 528), (300, 64)])
+@pytest.mark.parametrize("dtype", HALF)
+def test_int4_experts_hidden_values_past_the_types_range(t, h, dtype):
+    """Hidden values that fp16 does not reach, results that it does."""
+    args, hid, down = whole_experts(t, 64, h, 2, 64, dtype, reach=8)
+    assert float(hid.abs().max()) > 65504
+    off, bound, exact = hidden_bound(args, hid, down)
+    assert float(exact.abs().max()) < 65504 and bool((off <= bound).all())
+
+
+def test_int4_experts_what_is_not_finite_stays_with_its_token():
+    args, _, _ = whole_experts(40, 64, 128, 3, 64, torch.float16)
+    want = int4_experts(*args, "relu")
+    x = args[0].clone()
+    x[7, 3], x[20, 60] = float("inf"), float("nan")
+    out = int4_experts(x, *args[1:], "relu")
+    keep = [i for i in range(40) if i not in (7, 20)]
+    assert torch.equal(out[keep], want[keep])
+    assert not torch.isfinite(out[7]).all() and torch.isnan(out[20]).any()
