@@ -15,8 +15,10 @@
  *   - Return value: MOE_B200_OK or a negative MOE_B200_ERR_* (see moe_b200_error_string).
  *   - `status` is a device int32 word the kernels set non-zero when they notice a problem while
  *     running (a bounded wait that ran out = 1, an expert id out of range = 2, run starts that
- *     decrease or leave the rows = 3). The host reads it
- *     whenever it wants to pay for the synchronisation.
+ *     decrease or leave the rows = 3). The host reads it whenever it wants to pay for the
+ *     synchronisation. Codes 2 and 3 report an input and change no result, of this call or a later
+ *     one; behind a 1 waits give up early, and results are not to be used, until the host has set the
+ *     word back to 0.
  *   - "slot order": pairs (token, expert) sorted by expert, every expert's run padded to a
  *     multiple of 128 rows; pad slots hold the sentinel n_pairs in sorted_ids and zero rows in
  *     every slot-ordered activation buffer. l_cap = moe_b200_l_cap(n_pairs, n_experts) rows.

@@ -1,14 +1,12 @@
-// The gate activations the epilogues implement, as compile-time variants (ids as in the C ABI), and
-// the status codes a kernel can leave.
+// The gate activations the epilogues implement, as compile-time variants (ids as in the C ABI).
 #pragma once
 #include <cuda_runtime.h>
+
+#include "status.cuh"
 
 namespace moe {
 
 enum Act { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3, ACT_TANH = 4 };
-
-// Status codes a kernel can leave in the status word (0 = fine).
-enum DevStatus { ST_OK = 0, ST_WAIT_TIMEOUT = 1, ST_BAD_EXPERT = 2, ST_BAD_OFFSETS = 3 };
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float g) {

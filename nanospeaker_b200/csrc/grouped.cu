@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
 
   if (warp == 2) {
     const bool bad = load_run_starts(p.offsets, p.n_groups, p.rows, lane, table.start);
-    if (bad && blockIdx.x == 0 && lane == 0) atomicExch(p.status, ST_BAD_OFFSETS);
+    if (bad && blockIdx.x == 0 && lane == 0) report_input(p.status, ST_BAD_OFFSETS);
     const int nc = p.n_chunks;
     count_run_units(table.start, p.n_groups, lane, table.first,
                     [nc](int rows) { return ((rows + 2 * BM - 1) / (2 * BM)) * nc; });
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
   const int tiles = p.m_tiles * p.n_tiles;
   if (warp == 2) {
     const bool bad = load_run_starts(p.offsets, p.n_groups, p.rows, lane, table.start);
-    if (bad && blockIdx.x == 0 && lane == 0) atomicExch(p.status, ST_BAD_OFFSETS);
+    if (bad && blockIdx.x == 0 && lane == 0) report_input(p.status, ST_BAD_OFFSETS);
     const int ks = p.ks;
     count_run_units(table.start, p.n_groups, lane, table.first, [=](int rows) { return run_chunks(rows, ks); });
     count_run_units(table.start, p.n_groups, lane, split_first,

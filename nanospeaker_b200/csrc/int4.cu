@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(128)
     int4_sum_kernel(const float* y, const T* topk_w, const int64_t* topk_idx, int32_t n_tokens, int32_t top_k,
                     int32_t n_experts, int32_t n_shared, int32_t d, T* out, int32_t* status) {
   pdl_trigger();
-  bool waited = false;
+  bool waited = false, bad = false;
   const int64_t n_pairs = int64_t(n_tokens) * top_k, n4 = int64_t(n_tokens) * (d / 4);
   for (int64_t i = int64_t(blockIdx.x) * 128 + threadIdx.x; i < n4; i += int64_t(gridDim.x) * 128) {
     const int64_t tok = i / (d / 4);
@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(128)
           const int64_t e = ld_prev(topk_idx + tok * top_k + j0 + j);
           w[j] = Half16<T>::to_float(ld_prev(topk_w + tok * top_k + j0 + j));
           there[j] = e >= 0 && e < n_experts;
-          if (!there[j] && c == 0) atomicExch(status, ST_BAD_EXPERT);
+          bad |= !there[j] && c == 0;
         }
       }
       if (!waited) {
@@ -696,6 +696,7 @@ __global__ void __launch_bounds__(128)
         make_uint2(Half16<T>::pack(a.x, a.y), Half16<T>::pack(a.z, a.w));
   }
   if (!waited) pdl_wait();
+  if (bad) report_input(status, ST_BAD_EXPERT);   // (nothing is written ahead of the wait)
 }
 
 static void set_shape(Args& a, int mode, int32_t k_dim, int32_t n_dim, int32_t n_cols, int32_t group) {

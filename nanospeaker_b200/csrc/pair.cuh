@@ -44,7 +44,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     if (ok) return true;
-    if ((it & 1023u) == 1023u && *status != 0) return false;
+    if ((it & 1023u) == 1023u && status_ends_waits(*status)) return false;
   }
   return false;
 }

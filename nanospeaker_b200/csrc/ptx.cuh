@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "status.cuh"
+
 namespace moe {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -55,13 +57,13 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 #ifndef MOE_WAIT_LIMIT
 #define MOE_WAIT_LIMIT (1u << 22)
 #endif
-// `status` is the global status word: once any CTA has flagged a problem there, every other wait
-// gives up at its next check instead of running out its own limit.
+// `status` is the global status word: once a wait of any CTA has run out, every other one gives up at its
+// next check instead of running out its own limit.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
                                           const volatile int32_t* status) {
   for (uint32_t it = 0; it < MOE_WAIT_LIMIT; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 1023u) == 1023u && *status != 0) return false;
+    if ((it & 1023u) == 1023u && status_ends_waits(*status)) return false;
   }
   return false;
 }

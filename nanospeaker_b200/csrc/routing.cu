@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(DISPATCH_THREADS)
       if (e >= 0 && e < n_experts)
         atomicAdd(&hist[int(e)], 1);
       else
-        atomicExch(status, ST_BAD_EXPERT);
+        report_input(status, ST_BAD_EXPERT);
     }
   }
   // sentinel fill: each block paints an equal slice of [0, l_cap)

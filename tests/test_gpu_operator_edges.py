@@ -3,7 +3,7 @@ sums but the one under test are exact, calls behind a reported one, and what is 
 import pytest
 import torch
 
-from nanospeaker_b200 import Int4Weight, int4_experts, kernels
+from nanospeaker_b200 import Int4Weight, grouped_mm, int4_experts, kernels
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,44 @@ def test_int4_experts_what_is_not_finite_stays_with_its_token():
     keep = [i for i in range(40) if i not in (7, 20)]
     assert torch.equal(out[keep], want[keep])
     assert not torch.isfinite(out[7]).all() and torch.isnan(out[20]).any()
+
+
+# --------------------------------------------------------------------------- behind a reported input
+def test_reported_inputs_stop_no_call():
+    """A weight gradient of several ms in which one warp waits for the single ragged run end nearly throughout
+    (longer than a wait looks away from the status word): the same bits behind a reported expert id or run start, and
+    the report stays what it was."""
+    runs, each, m, n = 16, 32768, 2048, 4096
+    rows = runs * each - 31
+    a = torch.randn(rows, m, device="cuda", dtype=torch.bfloat16)
+    b = torch.randn(rows, n, device="cuda", dtype=torch.bfloat16)
+    off = (torch.arange(runs + 1, device="cuda") * each).clamp(max=rows).int()
+    kernels.check_status("cuda")
+    want = kernels.grouped_wgrad(a, b, off)
+    kernels.check_status("cuda")
+    word = kernels.status_word("cuda")
+    for code in (2, 3):
+        word.fill_(code)
+        assert torch.equal(kernels.grouped_wgrad(a, b, off), want)
+        assert int(word) == code
+        word.zero_()
+    # starts that decrease, reported by the call itself: taken into range, and the rest is right
+    bad = off.clone()
+    bad[3] = bad[4] + 5
+    good = bad.cummax(0).values
+    got = kernels.grouped_wgrad(a, b, bad)
+    with pytest.raises(RuntimeError, match="runs decrease or leave"):
+        kernels.check_status("cuda")
+    assert torch.equal(got, kernels.grouped_wgrad(a, b, good))
+    kernels.check_status("cuda")
+
+
+def test_a_report_is_not_replaced_by_a_later_one():
+    args, _, _ = whole_experts(3, 64, 16, 2, 32, torch.bfloat16)
+    x, w = torch.randn(8, 16, device="cuda").half(), torch.randn(2, 16, 16, device="cuda").half()
+    args[2][1, 0] = 7
+    int4_experts(*args, "relu")
+    grouped_mm(x, w, torch.tensor([0, 9, 8], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="expert id"):
+        kernels.check_status("cuda")
+    kernels.check_status("cuda")

@@ -65,3 +65,16 @@ def test_a_group_goes_on_or_leaves_as_one(harness, when, go):
     *got, reads_behind = map(int, out.stdout.split())
     assert got == [go] * 4            # (an abort raised behind the barrier counts at the next wait)
     assert reads_behind == 0
+
+
+def test_waits_end_early_for_waits_that_ran_out_and_not_for_reported_inputs(tmp_path):
+    """csrc/status.cuh: an expert id or a run start out of range, reported by this call or an earlier one, stops
+    nobody."""
+    (tmp_path / "main.cpp").write_text('#include "status.cuh"\n#include <cstdio>\nint main() {\n'
+                                       "  for (int code = -1; code < 5; ++code)\n"
+                                       '    std::printf("%d ", moe::status_ends_waits(code));\n}\n')
+    subprocess.run([shutil.which("g++") or "c++", "-std=c++17", "-I",
+                    os.path.join(ROOT, "nanospeaker_b200", "csrc"), str(tmp_path / "main.cpp"), "-o",
+                    str(tmp_path / "main")], check=True)
+    out = subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True).stdout
+    assert out.split() == ["0", "0", "1", "0", "0", "0"]
