@@ -78,3 +78,30 @@ def test_waits_end_early_for_waits_that_ran_out_and_not_for_reported_inputs(tmp_
                     str(tmp_path / "main")], check=True)
     out = subprocess.run([str(tmp_path / "main")], check=True, capture_output=True, text=True).stdout
     assert out.split() == ["0", "0", "1", "0", "0", "0"]
+
+
+def test_unseen_uses_are_the_copies_that_may_be_in_flight(tmp_path):
+    """csrc/ring.cuh against the ring itself: a reader that gives up at use `first` has seen all before; a writer that
+    waits for a stage to be freed can have started `stages` more. Each with the parity of the phase that it ends
+    (a barrier's phases count from 0, one per use of its stage)."""
+    (tmp_path / "main.cpp").write_text(
+        '#include "ring.cuh"\n#include <cstdio>\n#include <cstdlib>\nint main(int, char** v) {\n'
+        "  moe::unseen_uses(std::atoi(v[1]), std::atoi(v[2]), [](uint32_t s, uint32_t p) {\n"
+        '    std::printf("%u.%u ", s, p);\n  });\n}\n')
+    exe = str(tmp_path / "main")
+    subprocess.run([shutil.which("g++") or "c++", "-std=c++17", "-I",
+                    os.path.join(ROOT, "nanospeaker_b200", "csrc"), str(tmp_path / "main.cpp"), "-o", exe], check=True)
+    for stages in (1, 2, 3, 6):
+        for first in range(20):
+            freed, started, phase, flying = set(range(stages)), 0, [-1] * stages, {}
+            while started % stages in freed:          # the writer: a stage's first use needs no one
+                at = started % stages
+                if started < first:                   # (seen, and given back)
+                    phase[at] += 1
+                else:
+                    freed.discard(at)
+                    phase[at] += 1
+                    flying[at] = phase[at] & 1
+                started += 1
+            out = subprocess.run([exe, str(first), str(stages)], check=True, capture_output=True, text=True).stdout
+            assert dict(map(int, w.split(".")) for w in out.split()) == flying and len(out.split()) == stages
