@@ -81,15 +81,6 @@ __device__ __forceinline__ void store32(T* row, int64_t ld, int col, int n_dim, 
   }
 }
 
-// A producer that gave up waits (with a limit) for the copies it has in flight: the last uses of the ring's
-// stages. `it` counts the stages it has issued.
-template <int STAGES>
-__device__ __forceinline__ void drain_ring(uint64_t* full_bar, uint32_t it) {
-  for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-    for (int n = 0; n < 4096 && !mbar_try_wait(full_bar + i % STAGES, (i / STAGES) & 1); ++n) {
-    }
-}
-
 // N chunks of 32 accumulator columns from column `col` of the result on, those that start below n_dim. (A loop: its
 // code is fetched once; the next chunk's read under this one's stores gained nothing, other warps fill the wait.)
 template <int N, typename Store>
@@ -237,8 +228,6 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
           }
         }
       }
-      // (the leader's barriers count both CTAs' bytes, and the pair leaves together)
-      if (*abort_flag && rank == 0) drain_ring<STAGES>(full_bar, it);
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -276,6 +265,9 @@ __global__ void __launch_bounds__(64 + EPI_WARPS * 32, 1)
         }
         umma_commit_2cta(tfull_bar + b, 3);
       }
+      // (whoever gave up, nobody reads on from here; the leader's barriers count both CTAs' bytes, and the pair leaves
+      // together)
+      if (*abort_flag) mbar_drain(full_bar, it, STAGES);
     }
   } else {
     const int ew = warp - 2;
@@ -555,10 +547,6 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
             tma_load_3d(sB + i * 64 * BK * 2, &tmB, landed_bar + b, nb + 64 * i, row, 0);
         }
       }
-      if (*abort_flag) {   // (the leader's barriers count both CTAs' bytes, and the pair leaves together)
-        if (rank == 0) drain_ring<STAGES>(full_bar, it);
-        drain_ring<2>(landed_bar, uint32_t(tails));
-      }
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -611,6 +599,9 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
         }
         umma_commit_2cta(tfull_bar + b, 3);
       }
+      // (whoever gave up, nobody reads on from here; the leader's barriers count both CTAs' bytes, and the pair leaves
+      // together)
+      if (*abort_flag) mbar_drain(full_bar, it, STAGES);
     }
   } else if (warp == 2 + EPI_WARPS) {
     int tails = 0;
@@ -626,6 +617,7 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
           *abort_flag = 1;
           atomicExch(p.status, ST_WAIT_TIMEOUT);
         }
+        mbar_drain(landed_bar, tails - 1, 2);
         break;
       }
       // a 64 x 64 box keeps its row r in bytes r * 128 .. r * 128 + 127, in whatever order

@@ -33,7 +33,6 @@
 #include "pdl.cuh"
 #include "per_device.cuh"
 #include "ptx.cuh"
-#include "ring.cuh"
 
 namespace moe {
 namespace q4 {
@@ -178,15 +177,6 @@ __device__ __forceinline__ void split(const float2& v, uint32_t& upper, uint32_t
   upper = __byte_perm(x, y, 0x7632);
   auto left = [](float f, uint32_t bits) { return isinf(f) ? 0.f : f - __uint_as_float(bits & 0xFFFF0000u); };
   rest = Half16<__nv_bfloat16>::pack(left(v.x, x), left(v.y, y));
-}
-
-// A wait for a stage ran out: the copies that may be on their way, rows and weights, get some more time (8 ms a
-// stage) before anybody leaves. (Called, for it is hardly ever wanted.)
-__device__ __noinline__ void drain(uint64_t* full_bar, int first, int depth) {
-  unseen_uses(uint32_t(first), uint32_t(depth), [&](uint32_t stage, uint32_t parity) {
-    for (int n = 0; n < 4096 && !mbar_try_wait(full_bar + stage, parity); ++n) {
-    }
-  });
 }
 
 __device__ __forceinline__ uint32_t ld_shared_b32(uint32_t addr) {
@@ -441,7 +431,7 @@ __global__ void __launch_bounds__((MAX_WARPS + copy_warps(NT)) * 32, ctas_per_sm
         if (!dead && !mbar_wait(full_bar + slot, phase, p.status)) {
           dead = true;
           atomicExch(p.status, ST_WAIT_TIMEOUT);
-          drain(full_bar, phase * p.depth + slot, p.depth);
+          mbar_drain(full_bar, phase * p.depth + slot, p.depth);
         }
         // this warp's blocks of the chunk, and where its strips' pieces are
         const bool last = st == n_stages - 1;

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "ring.cuh"
 #include "status.cuh"
 
 namespace moe {
@@ -66,6 +67,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
     if ((it & 1023u) == 1023u && status_ends_waits(*status)) return false;
   }
   return false;
+}
+
+// The reader of a ring gives up at use `first`: the copies that may be on their way get some more time (8 ms a stage)
+// before anybody leaves. (Called, for it is hardly ever wanted.)
+template <typename = void>
+__device__ __noinline__ void mbar_drain(uint64_t* full_bar, uint32_t first, uint32_t stages) {
+  unseen_uses(first, stages, [&](uint32_t stage, uint32_t parity) {
+    for (int n = 0; n < 4096 && !mbar_try_wait(full_bar + stage, parity); ++n) {
+    }
+  });
 }
 
 // ------------------------------------------------------------- cp.async (gathered rows)
