@@ -928,23 +928,23 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   const int dev = current_device();
   const int bn = wgrad_bn(n_dim);
   const int64_t tiles = wgrad_tiles(m_dim, n_dim);
-  const int64_t ks = wgrad_chunk(rows, n_groups, tiles);
+  const int64_t ks = std::min<int64_t>(wgrad_chunk(rows, n_groups, tiles), INT_MAX / 2);
+  const int64_t units = (rows / ks + n_groups) * tiles;
+  if (units > INT_MAX) return MOE_B200_ERR_UNSUPPORTED;
   WgradArgs p{};
   p.offsets = offsets;
   p.n_groups = n_groups;
   p.rows = int32_t(rows);
-  p.ks = int32_t(std::min<int64_t>(ks, INT_MAX / 2));
+  p.ks = int32_t(ks);
   p.m_dim = m_dim;
   p.n_dim = n_dim;
   p.m_tiles = (m_dim + 2 * BM - 1) / (2 * BM);
   p.n_tiles = (n_dim + bn - 1) / bn;
-  p.tiles_inv = quotient_inverse(uint32_t(p.m_tiles * p.n_tiles));
+  p.tiles_inv = quotient_inverse(uint32_t(tiles));
   p.out = dw;
   p.wide = n_dim % 16 == 0 && reinterpret_cast<uintptr_t>(dw) % 32 == 0;
   p.partials = partials;
   p.status = status;
-  const int64_t units = (rows / p.ks + n_groups) * tiles;
-  if (units > INT_MAX) return MOE_B200_ERR_UNSUPPORTED;
   CUtensorMap tmA, tmB;
   if (!map_mn(&tmA, a, rows, ld_a, m_dim, BM / 64, &p.a_fused) ||
       !map_mn(&tmB, b, rows, ld_b, n_dim, bn / 128, &p.b_fused))
@@ -992,6 +992,7 @@ int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
 size_t moe_b200_grouped_wgrad_scratch_bytes(int32_t m_dim, int32_t n_dim, int64_t rows, int32_t n_groups) {
   if (m_dim < 8 || n_dim < 8 || rows < 0 || n_groups < 1) return 0;
   const int64_t tiles = grouped::wgrad_tiles(m_dim, n_dim);
+  if (tiles > INT_MAX) return 0;   // (refused)
   const int64_t ks = grouped::wgrad_chunk(rows, n_groups, tiles);
   return size_t(grouped::split_chunks(rows, ks, n_groups)) * size_t(tiles) * 2 * grouped::BM *
          size_t(grouped::wgrad_bn(n_dim)) * sizeof(float);
@@ -1005,6 +1006,7 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
       n_groups > RUNS_MAX_GROUPS || ld_a < m_dim || ld_a % 8 || ld_b < n_dim || ld_b % 8)
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
+  if (grouped::wgrad_tiles(m_dim, n_dim) > INT_MAX) return MOE_B200_ERR_UNSUPPORTED;
   if (!dw || !status) return MOE_B200_ERR_NULL;
   if (!grouped::aligned(dw, 16)) return MOE_B200_ERR_ALIGN;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -431,3 +431,14 @@ def test_sizes_whose_places_leave_31_bits_are_refused(lib):
         2, 1 << 31, 8, device="meta", dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="widths"):
         grouped_mm(x, w, torch.empty(3, device="meta", dtype=torch.int32))
+
+
+def test_products_of_more_tiles_than_31_bits_count_are_refused(lib):
+    """One row and two widths of 2^24, nothing to split: 2^32 tiles, which 32 bits take for none."""
+    buf = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 63) & ~63)
+    for m, n, groups in ((1 << 24, 1 << 24, 1), (1 << 30, 1 << 30, 1024), (1 << 19, 1 << 19, 1024)):
+        assert lib.moe_b200_grouped_wgrad(p, m, m, p, n, n, 1, p, groups, 0, p, None, 0, p, None) == -5
+        assert lib.moe_b200_grouped_wgrad(p, m, m, p, n, n, (1 << 31) - 257, p, groups, 0, p, None, 1 << 62, p,
+                                          None) in (-4, -5)
+    assert lib.moe_b200_grouped_wgrad_scratch_bytes(1 << 24, 1 << 24, 1 << 30, 1) == 0
