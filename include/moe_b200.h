@@ -662,8 +662,8 @@ int moe_b200_stack_infer(const void* plan, int32_t n_layers, const void* x, void
 
 /* ---- Products grouped by expert over ragged runs --------------------------------------------------
  * offsets [n_groups + 1]: rows offsets[g] .. offsets[g + 1] belong to group g, back to back, of any
- * length (also none); n_groups <= 1024, rows < 2^31 - 256. Starts that decrease or leave [0, rows] are taken into range
- * and reported through status. dtype MOE_B200_BF16 or MOE_B200_FP16; widths and strides are
+ * length (also none); n_groups <= 1024, rows and widths < 2^31 - 256. Starts that decrease or leave
+ * [0, rows] are taken into range and reported through status. dtype MOE_B200_BF16 or MOE_B200_FP16; widths and strides are
  * multiples of 8 elements; fp32 sums, rounded once.
  *
  * moe_b200_grouped_mm: y [rows, n_dim] = x[r] @ w[g(r)], x [rows, k_dim] with ld_x elements between
@@ -693,7 +693,8 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
  *     16 * strip + g + 8 * (i % 2), and behind them
  *   [scale groups of the chunk][8][2] scales in the activations' type: outputs g and g + 8.
  * moe_b200_int4_bytes: bytes of one matrix (a multiple of 32); 0 for a bad shape.
- * x, y, topk_w: bf16 or fp16 (dtype), k_dim a multiple of 8; fp32 sums. Weights 16-byte aligned.
+ * x, y, topk_w: bf16 or fp16 (dtype), k_dim a multiple of 8, widths (2 * d_hidden too) < 2^31 - 256;
+ * fp32 sums. Weights 16-byte aligned.
  *
  * moe_b200_int4_mm: y [rows, n_dim] = x [rows, k_dim] @ W; up to 65535 * 32 rows (32 rows read the
  * weight once).

@@ -36,7 +36,8 @@ constexpr int EPI_WARPS = 8;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int BAND = 8;   // row tiles of a band (tile_in_bands)
 constexpr int SHORT = 32; // rows of the smaller A box
-constexpr int MAX_ROWS = INT_MAX - 2 * BM;   // (a tile's rows behind the last one are still ints)
+constexpr int MAX_UNITS = INT_MAX - 1024;   // (the unit a cluster takes behind the last one, too)
+constexpr int MAX_DIM = INT_MAX - 2 * BM;   // of rows and widths: what a tile has behind the last one is still an int
 // MN-major operands, as in gemm.cuh: 64 x 64 boxes
 constexpr uint32_t MN_LBO = 8192u, MN_SBO = 1024u, MN_KADV = 2048u;
 
@@ -876,7 +877,7 @@ static int rows_product(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
   a.out = y;
   a.wide = n_dim % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 32 == 0;
   a.status = status;
-  if (pairs * a.n_chunks > INT_MAX) return MOE_B200_ERR_UNSUPPORTED;
+  if (pairs * a.n_chunks > MAX_UNITS) return MOE_B200_ERR_UNSUPPORTED;
   CUtensorMap tmA, tmShort, tmB;
   if (!map_x(&tmA, x, rows, ld_x, k_dim, BM) || !map_x(&tmShort, x, rows, ld_x, k_dim, SHORT))
     return MOE_B200_ERR_TMA;
@@ -930,7 +931,7 @@ static int wgrad_product(const void* a, int64_t ld_a, int32_t m_dim, const void*
   const int64_t tiles = wgrad_tiles(m_dim, n_dim);
   const int64_t ks = std::min<int64_t>(wgrad_chunk(rows, n_groups, tiles), INT_MAX / 2);
   const int64_t units = (rows / ks + n_groups) * tiles;
-  if (units > INT_MAX) return MOE_B200_ERR_UNSUPPORTED;
+  if (units > MAX_UNITS) return MOE_B200_ERR_UNSUPPORTED;
   WgradArgs p{};
   p.offsets = offsets;
   p.n_groups = n_groups;
@@ -971,7 +972,7 @@ int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
                         int32_t n_groups, int64_t w_group_stride, int64_t ld_w, int32_t n_inner,
                         int32_t n_dim, const int32_t* offsets, int32_t dtype, void* y, int32_t* status,
                         void* stream) {
-  if (rows < 0 || rows > grouped::MAX_ROWS || k_dim < 8 || k_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
+  if (rows < 0 || rows > grouped::MAX_DIM || k_dim > grouped::MAX_DIM || n_dim > grouped::MAX_DIM || k_dim < 8 || k_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
       n_groups > RUNS_MAX_GROUPS || ld_x < k_dim || ld_x % 8 || w_group_stride % 8 || ld_w % 8 ||
       w_group_stride < 0 || ld_w < (n_inner ? n_dim : k_dim))
     return MOE_B200_ERR_SHAPE;
@@ -990,7 +991,7 @@ int moe_b200_grouped_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim
 }
 
 size_t moe_b200_grouped_wgrad_scratch_bytes(int32_t m_dim, int32_t n_dim, int64_t rows, int32_t n_groups) {
-  if (m_dim < 8 || n_dim < 8 || rows < 0 || n_groups < 1) return 0;
+  if (m_dim < 8 || n_dim < 8 || m_dim > grouped::MAX_DIM || n_dim > grouped::MAX_DIM || rows < 0 || n_groups < 1) return 0;
   const int64_t tiles = grouped::wgrad_tiles(m_dim, n_dim);
   if (tiles > INT_MAX) return 0;   // (refused)
   const int64_t ks = grouped::wgrad_chunk(rows, n_groups, tiles);
@@ -1002,7 +1003,7 @@ int moe_b200_grouped_wgrad(const void* a, int64_t ld_a, int32_t m_dim, const voi
                            int32_t n_dim, int64_t rows, const int32_t* offsets, int32_t n_groups,
                            int32_t dtype, void* dw, void* scratch, size_t scratch_bytes, int32_t* status,
                            void* stream) {
-  if (rows < 0 || rows > grouped::MAX_ROWS || m_dim < 8 || m_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
+  if (rows < 0 || rows > grouped::MAX_DIM || m_dim > grouped::MAX_DIM || n_dim > grouped::MAX_DIM || m_dim < 8 || m_dim % 8 || n_dim < 8 || n_dim % 8 || n_groups < 1 ||
       n_groups > RUNS_MAX_GROUPS || ld_a < m_dim || ld_a % 8 || ld_b < n_dim || ld_b % 8)
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;

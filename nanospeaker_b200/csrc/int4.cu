@@ -43,6 +43,7 @@ constexpr int MAX_DEPTH = 6;     // stages of the ring
 constexpr int PAIR_WINDOW = 1024;   // pairs whose expert ids are looked at in one go
 
 constexpr int CHUNK = 8;         // blocks of 64 inputs in a chunk
+constexpr int MAX_WIDTH = 0x7fffffff - 256;   // what a block or a CTA's strips have behind the last is still an int
 
 // A stack of matrices in the packed layout (include/moe_b200.h).
 struct Stack {
@@ -843,7 +844,8 @@ using namespace moe;
 extern "C" {
 
 size_t moe_b200_int4_bytes(int32_t k_dim, int32_t n_dim, int32_t group) {
-  if (k_dim < 8 || k_dim % 8 || n_dim < 1 || !q4::group_ok(group)) return 0;
+  if (k_dim < 8 || k_dim % 8 || k_dim > q4::MAX_WIDTH || n_dim < 1 || n_dim > q4::MAX_WIDTH || !q4::group_ok(group))
+    return 0;
   q4::Args a{};
   q4::set_shape(a, q4::DENSE, k_dim, n_dim, n_dim, group);
   return size_t(a.matrix);
@@ -851,7 +853,8 @@ size_t moe_b200_int4_bytes(int32_t k_dim, int32_t n_dim, int32_t group) {
 
 int moe_b200_int4_mm(const void* x, int64_t rows, int64_t ld_x, int32_t k_dim, const void* w, int32_t group,
                      int32_t n_dim, int32_t dtype, void* y, int32_t* status, void* stream) {
-  if (rows < 0 || rows > 0x7fffffff || k_dim < 8 || k_dim % 8 || n_dim < 1 || ld_x < k_dim || ld_x % 8 ||
+  if (rows < 0 || rows > 0x7fffffff || k_dim < 8 || k_dim % 8 || k_dim > q4::MAX_WIDTH || n_dim < 1 ||
+      n_dim > q4::MAX_WIDTH || ld_x < k_dim || ld_x % 8 ||
       !q4::group_ok(group))
     return MOE_B200_ERR_SHAPE;
   if (dtype != MOE_B200_BF16 && dtype != MOE_B200_FP16) return MOE_B200_ERR_UNSUPPORTED;
@@ -890,7 +893,8 @@ int moe_b200_int4_experts(const void* x, int64_t n_tokens, int64_t ld_x, int32_t
                           const void* w_sh_out, int32_t group, int32_t activation, int32_t dtype, void* out,
                           void* scratch, size_t scratch_bytes, int32_t* status, void* stream) {
   if (n_tokens < 0 || top_k < 1 || n_experts < 1 || n_shared < 0 || n_experts + int64_t(n_shared) > 65535 ||
-      d_model < 8 || d_model % 8 || d_hidden < 16 || d_hidden % 16 || ld_x < d_model || ld_x % 8 ||
+      d_model < 8 || d_model % 8 || d_model > q4::MAX_WIDTH || d_hidden < 16 || d_hidden % 16 ||
+      d_hidden > q4::MAX_WIDTH / 2 || ld_x < d_model || ld_x % 8 ||
       !q4::group_ok(group) || n_tokens > 0x7fffffff ||
       n_tokens * (int64_t(top_k) + n_shared) > 0x7fffffff - q4::PAIR_WINDOW)
     return MOE_B200_ERR_SHAPE;

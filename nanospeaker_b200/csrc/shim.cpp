@@ -872,7 +872,7 @@ OptTensor grouped_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, in
   if (x.dim() != 2 || w.dim() != 3 || offsets.dim() != 1 || x.size(1) != w.size(1) ||
       offsets.numel() != w.size(0) + 1 || !half16(x) || w.scalar_type() != x.scalar_type() ||
       offsets.scalar_type() != at::kInt || w.size(1) < 8 || w.size(2) < 8 || w.size(1) % 8 || w.size(2) % 8 ||
-      w.size(1) > INT32_MAX || w.size(2) > INT32_MAX ||
+      w.size(1) > INT32_MAX - 256 || w.size(2) > INT32_MAX - 256 ||
       w.size(0) < 1 || w.size(0) > max_groups || !x.is_cuda() || w.device() != x.device() ||
       offsets.device() != x.device())
     return {};

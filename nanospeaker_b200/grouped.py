@@ -13,6 +13,7 @@ from . import kernels as K
 from .moe_kernel import native_ok
 
 MAX_GROUPS = 1024
+MAX_WIDTH = 2 ** 31 - 257
 GROUPED_DTYPES = (torch.bfloat16, torch.float16)
 
 
@@ -28,8 +29,8 @@ def _check(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> None:
                          f"{w.dtype}")
     if offsets.dtype != torch.int32:
         raise ValueError(f"offsets are int32, got {offsets.dtype}")
-    if not (8 <= w.shape[1] < 2 ** 31 and 8 <= w.shape[2] < 2 ** 31) or w.shape[1] % 8 or w.shape[2] % 8:
-        raise ValueError(f"the widths of w {tuple(w.shape)} have to be multiples of 8")
+    if not (8 <= w.shape[1] <= MAX_WIDTH and 8 <= w.shape[2] <= MAX_WIDTH) or w.shape[1] % 8 or w.shape[2] % 8:
+        raise ValueError(f"the widths of w {tuple(w.shape)} have to be multiples of 8, below 2^31 - 256")
     if not 1 <= w.shape[0] <= MAX_GROUPS:
         raise ValueError(f"{w.shape[0]} groups: 1 to {MAX_GROUPS} are covered")
     if not (x.is_cuda and x.device == w.device == offsets.device):

@@ -17,6 +17,7 @@ from .moe_kernel import _act_id, native_ok
 
 INT4_DTYPES = (torch.bfloat16, torch.float16)
 GROUPS = (32, 64, 128)      # inputs that share a scale
+MAX_WIDTH = 2 ** 31 - 257
 BLOCK, CHUNK, STRIP = 64, 8, 16   # inputs of a block, blocks of a chunk, outputs of a strip
 
 
@@ -139,8 +140,9 @@ def _check_group(group: int) -> None:
 
 
 def _check_widths(k: int, n: int) -> None:
-    if not (8 <= k < 2 ** 31 and 1 <= n < 2 ** 31) or k % 8:
-        raise ValueError(f"a weight of {k} inputs and {n} outputs: inputs have to be a multiple of 8")
+    if not (8 <= k <= MAX_WIDTH and 1 <= n <= MAX_WIDTH) or k % 8:
+        raise ValueError(f"a weight of {k} inputs and {n} outputs: inputs have to be a multiple of 8, both below "
+                         "2^31 - 256")
 
 
 def _matrix_bytes(k: int, n: int, group: int) -> int:

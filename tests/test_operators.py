@@ -442,3 +442,28 @@ def test_products_of_more_tiles_than_31_bits_count_are_refused(lib):
         assert lib.moe_b200_grouped_wgrad(p, m, m, p, n, n, (1 << 31) - 257, p, groups, 0, p, None, 1 << 62, p,
                                           None) in (-4, -5)
     assert lib.moe_b200_grouped_wgrad_scratch_bytes(1 << 24, 1 << 24, 1 << 30, 1) == 0
+
+
+def test_widths_whose_last_tile_leaves_31_bits_are_refused(lib):
+    """Widths just below 2^31: what is rounded up to whole tiles or strips would be negative."""
+    buf = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 63) & ~63)
+    wide = (1 << 31) - 8
+    mm = lambda k, n: lib.moe_b200_grouped_mm(p, 1, k, k, p, 1, k * n, n, 1, n, p, 0, p, p, None)  # noqa: E731
+    wg = lambda m, n: lib.moe_b200_grouped_wgrad(p, m, m, p, n, n, 1, p, 1, 0, p, None, 0, p, None)  # noqa: E731
+    assert mm(wide, 8) == mm(8, wide) == wg(wide, 8) == wg(8, wide) == -1
+    assert lib.moe_b200_grouped_wgrad_scratch_bytes(wide, 8, 1 << 20, 1) == 0
+    odd = (1 << 31) - 1
+    q = lambda k, n: lib.moe_b200_int4_mm(p, 1, k, k, p, 64, n, 0, p, p, None)  # noqa: E731
+    assert q(wide, 8) == q(8, odd) == -1
+    assert lib.moe_b200_int4_bytes(wide, 8, 64) == lib.moe_b200_int4_bytes(8, odd, 64) == 0
+    assert lib.moe_b200_int4_bytes(8, (1 << 31) - 257, 128) == (((1 << 31) - 257 + 15) // 16) * (512 + 32)
+    for d, h in ((wide, 16), (64, 1 << 30), (64, (1 << 31) - 16)):
+        assert lib.moe_b200_int4_experts(p, 1, d, d, h, p, p, 1, 4, p, p, 0, None, None, 64, 0, 0, p, p, 1 << 62, p,
+                                         None) == -1
+    from nanospeaker_b200 import Int4Weight, grouped_mm
+    meta = lambda *s: torch.empty(*s, device="meta", dtype=torch.bfloat16)  # noqa: E731
+    off = torch.empty(2, device="meta", dtype=torch.int32)
+    _refused(grouped_mm, "widths", meta(1, wide), meta(1, wide, 8), off)
+    _refused(grouped_mm, "widths", meta(1, 8), meta(1, 8, wide), off)
+    _refused(Int4Weight, "outputs", torch.empty(1, 64, device="meta", dtype=torch.uint8), (8, odd), 64, torch.bfloat16)
