@@ -821,6 +821,28 @@ def ep_pull_vec(v_ptrs, pair_rank, pair_row, n_tokens: int, k_all: int, top_k: i
 DTYPE_IDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+def _fits(ok: bool, call: str, *tensors) -> None:
+    """The kernels take lengths from one operand and trust the others to have them."""
+    if not ok or len({t.device for t in tensors if t is not None}) > 1:
+        raise ValueError(f"{call}: operands that do not fit together, "
+                         f"{[None if t is None else (tuple(t.shape), t.dtype, str(t.device)) for t in tensors]}")
+
+
+def _is_offsets(t: torch.Tensor, n: int) -> bool:
+    return t.dtype == torch.int32 and tuple(t.shape) == (n,) and t.is_contiguous()
+
+
+def _is_packed(t: Optional[torch.Tensor], count: int, k: int, n: int, group: int) -> bool:
+    """Is t `count` packed 4-bit matrices [k, n]?"""
+    size = _lib.load().moe_b200_int4_bytes(k, n, group) if max(k, n) < 2 ** 31 else 0
+    return (t is not None and size > 0 and t.dtype == torch.uint8 and tuple(t.shape) == (count, size)
+            and t.is_contiguous())
+
+
+def _is_state(t: Optional[torch.Tensor]) -> bool:
+    return t is None or (t.dtype == torch.int64 and tuple(t.shape) == (2,) and t.is_contiguous())
+
+
 def _rows8(t: torch.Tensor) -> torch.Tensor:
     """t [rows, cols] as the kernels read it in place: unit column stride, row starts on 16 bytes;
     otherwise a contiguous copy."""
@@ -844,6 +866,8 @@ def _stack8(w: torch.Tensor):
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """y [R, N]: rows offsets[g] .. offsets[g + 1] of x [R, K] times w[g], w [G, K, N] with either of its
     inner axes contiguous; rows of no run are zero. bf16 or fp16, K and N multiples of 8."""
+    _fits(x.dim() == 2 and w.dim() == 3 and x.shape[1] == w.shape[1] and w.dtype == x.dtype
+          and _is_offsets(offsets, w.shape[0] + 1), "grouped_mm", x, w, offsets)
     _need_cuda(x, w, offsets)
     x, (w, n_inner) = _rows8(x), _stack8(w)
     g, k, n = w.shape
@@ -862,6 +886,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch
 def grouped_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """dw [G, M, N]: the sum over each run's rows of a[r]^T b[r] (a [R, M], b [R, N]); zero without
     rows."""
+    _fits(a.dim() == b.dim() == 2 and a.shape[0] == b.shape[0] and b.dtype == a.dtype and offsets.dim() == 1
+          and offsets.numel() > 1 and _is_offsets(offsets, offsets.numel()), "grouped_wgrad", a, b, offsets)
     _need_cuda(a, b, offsets)
     a, b = _rows8(a), _rows8(b)
     r, m = a.shape
@@ -880,6 +906,7 @@ def grouped_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor) -> to
 
 def int4_mm(x: torch.Tensor, data: torch.Tensor, group: int, n_dim: int) -> torch.Tensor:
     """x [R, K] times one packed 4-bit matrix -> [R, n_dim]."""
+    _fits(x.dim() == 2 and _is_packed(data, 1, x.shape[1], n_dim, group), "int4_mm", x, data)
     _need_cuda(x, data)
     x = _rows8(x)
     r, k = x.shape
@@ -896,11 +923,20 @@ def int4_experts(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out, d_hidd
                  act: int) -> torch.Tensor:
     """out [T, D] of the block's experts with packed 4-bit weights ([E, bytes] each, the shared ones None
     without shared experts)."""
+    s = 0 if shared_in is None else shared_in.shape[0]
+    _fits(x.dim() == topk_idx.dim() == 2 and topk_idx.shape[0] == x.shape[0] and topk_w.shape == topk_idx.shape
+          and topk_w.dtype == x.dtype and topk_idx.dtype == torch.int64 and topk_w.is_contiguous()
+          and topk_idx.is_contiguous() and (shared_in is None) == (shared_out is None)
+          and all(_is_packed(t, n, *kn, group)
+                  for t, n, kn in ((w_in, w_in.shape[0], (x.shape[1], 2 * d_hidden)),
+                                   (w_out, w_in.shape[0], (d_hidden, x.shape[1])),
+                                   (shared_in, s, (x.shape[1], 2 * d_hidden)),
+                                   (shared_out, s, (d_hidden, x.shape[1]))) if n or t is not None),
+          "int4_experts", x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out)
     _need_cuda(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out)
     x = _rows8(x)
     t, d = x.shape
     k, e = topk_idx.shape[1], w_in.shape[0]
-    s = 0 if shared_in is None else shared_in.shape[0]
     lib = _lib.load()
     out = torch.empty((t, d), dtype=x.dtype, device=x.device)
     nbytes = lib.moe_b200_int4_experts_scratch_bytes(t, k, s, d, d_hidden)
@@ -918,6 +954,8 @@ def int4_experts(x, topk_w, topk_idx, w_in, w_out, shared_in, shared_out, d_hidd
 def dropout(x: torch.Tensor, residual: Optional[torch.Tensor], p: float, rng: torch.Tensor,
             used: Optional[torch.Tensor] = None) -> torch.Tensor:
     """residual + dropout(x) (fresh, contiguous); used (int64 [2]) receives the state it was made with."""
+    _fits((residual is None or (residual.shape == x.shape and residual.dtype == x.dtype)) and rng is not None
+          and _is_state(rng) and _is_state(used), "dropout", x, residual, rng, used)
     _need_cuda(x, residual, rng, used)
     x = x.contiguous()
     residual = None if residual is None else residual.contiguous()

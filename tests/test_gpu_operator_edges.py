@@ -124,3 +124,12 @@ def test_a_report_is_not_replaced_by_a_later_one():
     with pytest.raises(RuntimeError, match="expert id"):
         kernels.check_status("cuda")
     kernels.check_status("cuda")
+
+
+# --------------------------------------------------------------------------- refusals
+def test_low_level_entries_refuse_operands_that_do_not_fit():
+    from test_operators import low_level_calls
+    for call, args in low_level_calls("cuda"):
+        with pytest.raises((ValueError, RuntimeError), match="do not fit together"):
+            call(*args)
+    kernels.check_status("cuda")

@@ -467,3 +467,51 @@ def test_widths_whose_last_tile_leaves_31_bits_are_refused(lib):
     _refused(grouped_mm, "widths", meta(1, wide), meta(1, wide, 8), off)
     _refused(grouped_mm, "widths", meta(1, 8), meta(1, 8, wide), off)
     _refused(Int4Weight, "outputs", torch.empty(1, 64, device="meta", dtype=torch.uint8), (8, odd), 64, torch.bfloat16)
+
+
+def low_level_calls(device):
+    """Every low-level entry, by its function or its registered op, with one operand that does not have the length
+    that another gives it."""
+    from nanospeaker_b200 import kernels as K
+    from nanospeaker_b200 import quantize_int4
+    half = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=device)  # noqa: E731
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=device)  # noqa: E731
+    x, w, idx = half(6, 64), half(2, 64, 24), torch.zeros(6, 2, dtype=torch.int64, device=device)
+    one = quantize_int4(torch.zeros(64, 32)).data.to(device)
+    w_in = quantize_int4(torch.zeros(4, 64, 64)).data.to(device)
+    w_out = quantize_int4(torch.zeros(4, 32, 64)).data.to(device)
+    sh_in, sh_out = w_in[:1], w_out[:1]
+    rng = torch.zeros(2, dtype=torch.int64, device=device)
+    ops = torch.ops.moe_b200
+    for mm in (K.grouped_mm, ops.grouped_mm):
+        yield from ((mm, a) for a in ((half(1, 32), w, i32(3)), (x, w, i32(2)), (x, w, i32(3).long()),
+                                      (x, w.half(), i32(3)), (x[0], w, i32(3))))
+    yield K.grouped_mm, (x, w, i32(6)[::2])
+    yield K.grouped_mm, (x, w.to("meta"), i32(3))
+    for wg in (K.grouped_wgrad, ops.grouped_wgrad):
+        yield from ((wg, a) for a in ((x, half(5, 24), i32(3)), (x, half(7, 24), i32(3)), (x, half(6, 24).half(), i32(3)),
+                                      (x, half(6, 24), i32(3).long()), (x, half(6, 24), i32(1))))
+    for mm in (K.int4_mm, ops.int4_mm):
+        yield from ((mm, a) for a in ((x, one, 64, 48), (x, one, 32, 32), (half(6, 128), one, 64, 32), (x, one, 48, 32),
+                                      (x, one[:, :-32], 64, 32), (x, one.view(torch.int8), 64, 32),
+                                      (x[0], one, 64, 32)))
+    for ex in (K.int4_experts, ops.int4_experts):
+        good = [x, half(6, 2), idx, w_in, w_out, sh_in, sh_out, 32, 64, 0]
+        for at, other in ((0, half(5, 64)), (0, half(6, 128)), (1, half(6, 1)), (1, half(6, 2).half()), (2, idx.int()),
+                          (3, w_in[:3]), (4, w_out[:3]), (5, None), (6, None), (5, w_in[:2]), (7, 48), (8, 32)):
+            yield ex, (*good[:at], other, *good[at + 1:])
+    yield from ((K.dropout, a) for a in ((x, half(6, 32), 0.1, rng), (x, x.half(), 0.1, rng), (x, None, 0.1, rng[:1]),
+                                         (x, None, 0.1, rng.int()), (x, None, 0.1, rng, rng[:1])))
+    yield ops.dropout_add, (x, half(6, 32), 0.1, rng)
+    yield ops.dropout_bwd, (x, 0.1, rng[:1])
+
+
+def test_low_level_entries_refuse_operands_that_do_not_fit():
+    """Before the device is looked at: what they would read past the end of is never reached."""
+    n = 0
+    for call, args in low_level_calls("cpu"):
+        if not isinstance(call, torch._ops.OpOverloadPacket):     # (the ops take CUDA tensors alone)
+            with pytest.raises(ValueError, match="do not fit together"):
+                call(*args)
+            n += 1
+    assert n > 30
