@@ -429,11 +429,16 @@ template <typename... T>
 bool any_grad(const T&... t) {
   return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
 }
-// The nodes here have no forward-mode derivative; an operand's would be dropped without a word.
+// The nodes here have no forward-mode derivative; an operand's would be dropped without a word. (Looked at whether or
+// not a gradient is wanted: an operand with a tangent mostly requires none.)
+template <typename... T>
+void refuse_forward_mode_of(const char* whose, const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!((t.defined() && t._fw_grad(0).defined()) || ...), whose,
+                              " does not support forward mode AD");
+}
 template <typename... T>
 void refuse_forward_mode(const T&... t) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!((t.defined() && t._fw_grad(0).defined()) || ...),
-                              "the MoE block does not support forward mode AD");
+  refuse_forward_mode_of("the MoE block", t...);
 }
 template <typename N>
 std::shared_ptr<N> new_node() {
@@ -483,11 +488,11 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> block(
   const Options o{top_k, activation, capacity, normalize, full_softmax, store, mm_logits,
                   one_stream, aux_coef};
   check_operands(p, o);
+  refuse_forward_mode(p.x, p.router_w, p.w_in, p.w_out, p.w_sh_in, p.w_sh_out, p.b_in, p.b_out,
+                      p.b_sh_in, p.b_sh_out, p.residual);
   std::shared_ptr<MoEBlockBackward> node;
   if (any_grad(p.x, p.router_w, p.w_in, p.w_out, p.w_sh_in, p.w_sh_out, p.b_in, p.b_out, p.b_sh_in,
                p.b_sh_out, p.residual)) {
-    refuse_forward_mode(p.x, p.router_w, p.w_in, p.w_out, p.w_sh_in, p.w_sh_out, p.b_in, p.b_out,
-                        p.b_sh_in, p.b_sh_out, p.residual);
     node = new_node<MoEBlockBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(
         p.x, p.router_w, p.w_in, p.w_out, p.w_sh_in, p.w_sh_out, p.b_in, p.b_out, p.b_sh_in,
@@ -876,10 +881,9 @@ OptTensor grouped_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, in
       w.size(0) < 1 || w.size(0) > max_groups || !x.is_cuda() || w.device() != x.device() ||
       offsets.device() != x.device())
     return {};
+  refuse_forward_mode_of("grouped_mm", x, w);
   std::shared_ptr<GroupedMMBackward> node;
   if (any_grad(x, w)) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined() && !w._fw_grad(0).defined(),
-                                "grouped_mm does not support forward mode AD");
     node = new_node<GroupedMMBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(x, w));
   }
@@ -904,6 +908,7 @@ OptTensor int4_mm(const Tensor& x, const Tensor& data, at::ScalarType dtype, con
   if (shape.size() != 2 || x.dim() < 1 || x.size(-1) != shape[0] || !x.is_cuda() || x.scalar_type() != dtype ||
       data.device() != x.device() || any_grad(x))
     return {};
+  refuse_forward_mode_of("int4_mm", x);
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard on(x.device());
   const Tensor flat = rows8(x.dim() == 2 ? x : x.reshape({-1, shape[0]}));
@@ -931,6 +936,7 @@ OptTensor int4_experts(const Tensor& x_in, const Tensor& topk_w, const Tensor& t
       w_in.device() != device || w_out.device() != device ||
       (sh_in && (sh_in->device() != device || sh_out->device() != device)) || any_grad(x_in, topk_w))
     return {};
+  refuse_forward_mode_of("int4_experts", x_in, topk_w);
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard on(device);
   const Tensor x = rows8(x_in), w = topk_w.contiguous(), idx = topk_idx.contiguous();
@@ -973,10 +979,9 @@ struct DropoutAddBackward : public torch::autograd::Node {
 
 // keep_state: rng may change before the backward, which gets a copy that the kernel makes.
 Tensor dropout_call(const Tensor& x_in, const Tensor& res_in, double p, const Tensor& rng, bool keep_state) {
+  refuse_forward_mode_of("dropout_add", x_in, res_in);
   std::shared_ptr<DropoutAddBackward> node;
   if (any_grad(x_in, res_in)) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!x_in._fw_grad(0).defined() && !(res_in.defined() && res_in._fw_grad(0).defined()),
-                                "dropout_add does not support forward mode AD");
     node = new_node<DropoutAddBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(x_in, res_in));
   }

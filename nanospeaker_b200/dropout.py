@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import kernels as K
-from .moe_kernel import native_ok
+from .moe_kernel import native_ok, refuse_forward_mode
 
 DROPOUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -83,6 +83,7 @@ def dropout_add(x: torch.Tensor, residual: Optional[torch.Tensor], p: float,
         out = K.shim().dropout_add(x, residual, p, rng)
         if out is not None:
             return out
+    refuse_forward_mode("dropout_add", x, residual)
     if x.dtype not in DROPOUT_DTYPES:
         raise ValueError(f"dropout computes in bf16, fp16 or fp32, got {x.dtype}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):

@@ -10,7 +10,7 @@ csrc/grouped.cu.
 import torch
 
 from . import kernels as K
-from .moe_kernel import native_ok
+from .moe_kernel import native_ok, refuse_forward_mode
 
 MAX_GROUPS = 1024
 MAX_WIDTH = 2 ** 31 - 257
@@ -98,5 +98,6 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch
         y = K.shim().grouped_mm(x, w, offsets, MAX_GROUPS)
         if y is not None:
             return y
+    refuse_forward_mode("grouped_mm", x, w)
     _check(x, w, offsets)
     return _grouped_mm(x, w, offsets)

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import kernels as K
-from .moe_kernel import _act_id, native_ok
+from .moe_kernel import _act_id, native_ok, refuse_forward_mode
 
 INT4_DTYPES = (torch.bfloat16, torch.float16)
 GROUPS = (32, 64, 128)      # inputs that share a scale
@@ -213,6 +213,7 @@ def int4_mm(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
         out = K.shim().int4_mm(x, weight.data, weight.dtype, weight.shape, weight.group)
         if out is not None:
             return out
+    refuse_forward_mode("int4_mm", x)
     _check_types(x, weight)
     if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
         raise ValueError(f"int4_mm takes x [..., K] and one matrix [K, N], got {tuple(x.shape)} and "
@@ -257,6 +258,7 @@ def int4_experts(x: torch.Tensor, topk_w: torch.Tensor, topk_idx: torch.Tensor, 
             out = K.shim().int4_experts(x, topk_w, topk_idx, *plain, act)
             if out is not None:
                 return out
+    refuse_forward_mode("int4_experts", x, topk_w)
     shared = () if shared_in is None and shared_out is None else (shared_in, shared_out)
     weights = (w_in, w_out, *shared)
     _check_types(x, *weights)

@@ -15,6 +15,7 @@ stays in a 1-element device tensor that the kernels read.
 from typing import List, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import kernels as K
 from .kernels import ALIGN_M, KERNEL_ACTIVATIONS, l_cap as _l_cap  # noqa: F401  (re-exported)
@@ -851,6 +852,14 @@ def native_ok(x: torch.Tensor) -> bool:
             and torch._C._functorch.peek_interpreter_stack() is None)
 
 
+def refuse_forward_mode(whose: str, *tensors) -> None:
+    """The registered ops have no forward-mode derivative and would drop an operand's without a word."""
+    if torch.compiler.is_compiling():
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{whose} does not support forward mode AD")
+
+
 def fused_moe_block(x, router, w_in, w_out, w_sh_in, w_sh_out, activation, full_softmax,
                     combine: Optional[str] = None, noise: Optional[torch.Tensor] = None):
     """(out, aux_loss (fp32; zero in eager calls' x.dtype without the loss), counts int32 [E]) for a TopKRouter-like `router` (attributes W,
@@ -864,6 +873,7 @@ def fused_moe_block(x, router, w_in, w_out, w_sh_in, w_sh_out, activation, full_
             router.aux_loss_coef, act, 0, not _atomic(combine), False, _DEBUG_ONE_STREAM)[:3]
     cast = lambda t: None if t is None else t.to(x.dtype)
     tensors = (x, router.W, w_in, w_out, w_sh_in, w_sh_out)
+    refuse_forward_mode("the MoE block", *tensors)
     save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
     bias = router.logit_bias
     if bias is not None:
@@ -933,6 +943,7 @@ def fused_moe_forward(x, w_in, w_out, topk_w, topk_idx, b_in, b_out, activation,
     the GEMM epilogues and get gradients.
     """
     _act_id(activation)
+    refuse_forward_mode("the MoE block", x, w_in, w_out, topk_w, b_in, b_out, w_sh_in, w_sh_out, b_sh_in, b_sh_out)
     n_experts = w_in.shape[0]
     topk_w = topk_w.to(x.dtype)
     if w_sh_in is not None:

@@ -133,3 +133,35 @@ def test_low_level_entries_refuse_operands_that_do_not_fit():
         with pytest.raises((ValueError, RuntimeError), match="do not fit together"):
             call(*args)
     kernels.check_status("cuda")
+
+
+@pytest.mark.parametrize("how", ["dual", "jvp"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(how, grad):
+    """Whether or not an operand requires a gradient, through the eager calls and through the registered ops."""
+    import torch.autograd.forward_ad as fwad
+    from nanospeaker_b200 import MoEBlock, MoEFFNSublayer, dropout_add, int4_mm, quantize_int4
+    half = lambda *s: torch.randn(*s, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    w, off = half(2, 64, 24).requires_grad_(grad), torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda")
+    rng = torch.zeros(2, dtype=torch.int64, device="cuda")
+    x, tw, idx = half(6, 64), half(6, 1), torch.zeros(6, 1, dtype=torch.int64, device="cuda")
+    res = half(6, 64).requires_grad_(grad)
+    one = quantize_int4(half(64, 8))
+    w_in, w_out = quantize_int4(half(2, 64, 32)), quantize_int4(half(2, 16, 64))
+    block = MoEBlock(576, 76, d_ff=192, top_k=6, n_shared=2, capacity_factor=None).to(torch.bfloat16).cuda()
+    block.requires_grad_(grad)
+    sub = MoEFFNSublayer(block).to(torch.bfloat16).cuda().requires_grad_(grad)
+    calls = [(lambda v: grouped_mm(v, w, off), x), (lambda v: dropout_add(v, res, 0.1, rng), x),
+             (lambda v: dropout_add(x, v, 0.1, rng), x)]
+    if how == "dual":   # (the sublayer's traced form is an autograd.Function, which refuses in its own words)
+        calls += [(block, half(5, 576)), (lambda v: sub(v)[0], half(5, 576))]
+    if not grad:
+        calls += [(lambda v: int4_mm(v, one), x), (lambda v: int4_experts(v, tw, idx, w_in, w_out), x),
+                  (lambda v: int4_experts(x, v, idx, w_in, w_out), tw)]
+    for call, at in calls:
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            if how == "jvp":
+                torch.func.jvp(call, (at,), (torch.ones_like(at),))
+            else:
+                with fwad.dual_level():
+                    call(fwad.make_dual(at, torch.ones_like(at)))

@@ -515,3 +515,26 @@ def test_low_level_entries_refuse_operands_that_do_not_fit():
                 call(*args)
             n += 1
     assert n > 30
+
+
+@pytest.mark.parametrize("how", ["dual", "jvp"])
+def test_forward_mode_is_refused(how):
+    """An operand with a tangent requires no gradient as a rule; its tangent would be dropped without a word."""
+    import torch.autograd.forward_ad as fwad
+    from nanospeaker_b200 import dropout_add, fused_moe_forward, grouped_mm, int4_experts, int4_mm, quantize_int4
+    half = lambda *s: torch.randn(*s).bfloat16()  # noqa: E731
+    w, off, one = half(2, 16, 24), torch.tensor([0, 2, 6], dtype=torch.int32), quantize_int4(half(16, 8))
+    w_in, w_out = quantize_int4(half(2, 16, 32)), quantize_int4(half(2, 16, 16))
+    tw, idx, rng = half(6, 1), torch.zeros(6, 1, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)
+    x = half(6, 16)
+    calls = ((lambda v: grouped_mm(v, w, off), x), (lambda v: grouped_mm(x, v, off), w), (lambda v: int4_mm(v, one), x),
+             (lambda v: int4_experts(v, tw, idx, w_in, w_out), x), (lambda v: int4_experts(x, v, idx, w_in, w_out), tw),
+             (lambda v: dropout_add(v, None, 0.1, rng), x), (lambda v: dropout_add(x, v, 0.1, rng), x),
+             (lambda v: fused_moe_forward(v, half(2, 16, 32), half(2, 16, 16), tw, idx, None, None, "silu"), x))
+    for call, at in calls:
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            if how == "jvp":
+                torch.func.jvp(call, (at,), (torch.ones_like(at),))
+            else:
+                with fwad.dual_level():
+                    call(fwad.make_dual(at, torch.ones_like(at)))
