@@ -38,6 +38,27 @@ from .utils import ACTIVATIONS, resolve_activation
 AUTO_CAPACITY = 1.25
 
 
+class _PairRows(torch.autograd.Function):
+    """x[token_idx] [N * k, D] for the N tokens' pairs in a sorted order, `place` [N * k] being where each pair is in
+    it. The gradient of a token is its k pairs' rows summed in fp32 and rounded once (of x[token_idx] alone it would
+    be summed in x's type, with a rounding per pair)."""
+
+    @staticmethod
+    def forward(x, token_idx, place):
+        return x[token_idx]
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(inputs[2])
+        ctx.shape = inputs[0].shape
+
+    @staticmethod
+    def backward(ctx, grad):
+        place, = ctx.saved_tensors
+        n, d = ctx.shape
+        return grad[place].view(n, -1, d).sum(1), None, None
+
+
 class MoEBlock(nn.Module):
     """Sparse MoE feed-forward block with GLU experts (SwiGLU by default).
 
@@ -218,14 +239,15 @@ class MoEBlock(nn.Module):
             kept = torch.empty_like(at, dtype=torch.bool).index_copy_(0, order, at - offsets[experts] < cap)
             self.dropped = (~kept).sum().detach()
         offsets = offsets.to(torch.int32)
-        a = grouped_mm(x[token_idx], self.W_in.to(x.dtype), offsets)
+        place = torch.empty_like(order).index_copy_(0, order, at)
+        a = grouped_mm(_PairRows.apply(x, token_idx, place), self.W_in.to(x.dtype), offsets)
         if self.b_in is not None:
             a = a + self.b_in.float()[experts].to(x.dtype)   # (its gradient is then summed in fp32)
         gate, up = a.chunk(2, dim=-1)
         y = grouped_mm(self.glu(gate, up), self.W_out.to(x.dtype), offsets)
         if self.b_out is not None:
             y = y + self.b_out.float()[experts].to(x.dtype)
-        rows = y[torch.empty_like(order).index_copy_(0, order, at)].view(*topk_idx.shape, self.d_model)
+        rows = y[place].view(*topk_idx.shape, self.d_model)
         rows = rows.float() * topk_w[..., None].float()
         if kept is not None:
             rows = torch.where(kept.view(*topk_idx.shape, 1), rows, 0.0)

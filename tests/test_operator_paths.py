@@ -34,6 +34,33 @@ def test_grouped_setting_changes_nothing_off_the_gpu():
     assert m.capacity_factor == cap and torch.equal(m(x), want)
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_of_gathered_rows_is_rounded_once(device, dtype):
+    """A token's rows of the gradient, of which there are k: their fp32 sum (off by k 2^-24 of the magnitude) and one
+    rounding. Summed in the type, one rounding a row, they are not within that."""
+    from nanospeaker_b200.moe import _PairRows
+    gen = torch.Generator().manual_seed(0)
+    n, k, d = 50, 8, 40
+    order = torch.randperm(n * k, generator=gen)
+    place = torch.empty_like(order).index_copy_(0, order, torch.arange(n * k))
+    x, g = torch.randn(n, d, generator=gen), torch.randn(n * k, d, generator=gen)
+    x, g = (t.to(device, dtype) for t in (x, g))
+    order, place = order.to(device), place.to(device)
+    x.requires_grad_()
+    out = _PairRows.apply(x, order // k, place)
+    assert torch.equal(out, x[order // k])
+    got, = torch.autograd.grad(out, x, g)
+    rows = g[place].view(n, k, d).double()
+    a = k * 2.0 ** -24 * rows.abs().sum(1)
+    bound = torch.finfo(dtype).eps / 2 * (rows.sum(1).abs() + a) + a
+    assert got.dtype == dtype and bool(((got.double() - rows.sum(1)).abs() <= bound).all())
+    in_type = torch.zeros_like(x)
+    for j in range(k):
+        in_type = in_type + g[place].view(n, k, d)[:, j]
+    assert not bool(((in_type.detach().double() - rows.sum(1)).abs() <= bound).all())
+
+
 def test_sublayer_dropout_on_the_cpu():
     sub = MoEFFNSublayer(block(64, 6, 96, 2), dropout=0.25)
     x = torch.randn(200, 64)
@@ -103,6 +130,33 @@ def test_block_of_any_width_matches_the_torch_loop(kw, dtype):
     for a, b in zip(got, want):
         assert rel_l2(a, b) < TOL[dtype]
     assert all(torch.equal(a, b) for a, b in zip(both(m, x, dout)[:1], got[:1]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_grouped_blocks_input_gradient_is_rounded_once(dtype):
+    """Every token through all eight experts, whole numbers throughout (weights are signed permutations, so that a
+    pair's gradient stays below 256, exact in either type): the token's gradient is the exact sum, rounded once."""
+    gen = torch.Generator().manual_seed(1)
+    d, e, n = 16, 8, 60
+    m = block(d, e, 24, e, dtype=torch.float64, activation="relu")
+    assert m.d_hidden == d
+    sign = lambda *s: torch.randint(0, 2, s, generator=gen).double() * 2 - 1  # noqa: E731
+    perm = lambda: torch.eye(d, dtype=torch.float64)[torch.randperm(d, generator=gen)] * sign(d, 1)  # noqa: E731
+    with torch.no_grad():
+        for i in range(e):
+            m.W_in[i] = torch.cat([perm(), perm()], 1)
+            m.W_out[i] = perm()
+    x = torch.randint(-2, 3, (n, d), generator=gen).double().requires_grad_()
+    dout = torch.randint(-63, 64, (n, d), generator=gen).double()
+    idx, tw = torch.arange(e).expand(n, e).contiguous(), torch.ones(n, e, dtype=torch.float64)
+    want, = torch.autograd.grad(m._torch_experts(x, tw, idx, 0)[0], x, dout)
+    assert float(want.abs().max()) > 256
+    m = m.to(dtype).cuda()
+    xc = x.detach().to("cuda", dtype).requires_grad_()
+    out, _ = m._grouped_experts(xc, tw.to("cuda", dtype), idx.cuda(), 0)
+    got, = torch.autograd.grad(out, xc, dout.to("cuda", dtype))
+    assert torch.equal(got.cpu(), want.to(dtype))
 
 
 @gpu
