@@ -228,16 +228,21 @@ class MoEBlock(nn.Module):
         return out, counts
 
     def _grouped_experts(self, x, topk_w, topk_idx, cap: int):
-        """The routed experts as two grouped products over the sorted pairs. Pairs over a capacity are
-        multiplied with the rest and left out of the sum. A token's rows are summed in fp32
-        in pair order: reproducible bit for bit."""
+        """The routed experts as two grouped products over the sorted pairs. Pairs over a capacity lie behind the
+        last run, where the products do not look: neither values nor gradients of theirs, finite or not, reach
+        anything. A token's rows are summed in fp32 in pair order: reproducible bit for bit."""
         experts, order, token_idx, counts = self._plan(topk_idx)
         offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
         at = torch.arange(order.numel(), device=x.device)
         kept = None
         if cap:
-            kept = torch.empty_like(at, dtype=torch.bool).index_copy_(0, order, at - offsets[experts] < cap)
-            self.dropped = (~kept).sum().detach()
+            fits = at - offsets[experts] < cap
+            self.dropped = (~fits).sum().detach()
+            offsets = torch.cat([counts.new_zeros(1), counts.clamp(max=cap).cumsum(0)])
+            to = torch.where(fits, fits.cumsum(0) - 1, offsets[-1] + (~fits).cumsum(0) - 1)
+            experts, order, token_idx = (torch.empty_like(t).index_copy_(0, to, t)
+                                         for t in (experts, order, token_idx))
+            kept = torch.empty_like(fits).index_copy_(0, order, at < offsets[-1]).view(topk_idx.shape)
         offsets = offsets.to(torch.int32)
         place = torch.empty_like(order).index_copy_(0, order, at)
         a = grouped_mm(_PairRows.apply(x, token_idx, place), self.W_in.to(x.dtype), offsets)
@@ -248,9 +253,9 @@ class MoEBlock(nn.Module):
         if self.b_out is not None:
             y = y + self.b_out.float()[experts].to(x.dtype)
         rows = y[place].view(*topk_idx.shape, self.d_model)
-        rows = rows.float() * topk_w[..., None].float()
         if kept is not None:
-            rows = torch.where(kept.view(*topk_idx.shape, 1), rows, 0.0)
+            rows, topk_w = torch.where(kept[..., None], rows, 0.0), torch.where(kept, topk_w, 0.0)
+        rows = rows.float() * topk_w[..., None].float()
         return rows.sum(1).to(x.dtype), counts
 
     # ------------------------------------------------------------------------------ forward

@@ -160,6 +160,44 @@ def test_grouped_blocks_input_gradient_is_rounded_once(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_what_dropped_pairs_hold_reaches_nothing(dtype, bias):
+    """Tokens whose pairs are all over the capacity hold infinities and NaN: results, gradients of the weights, of the
+    router's weights and of the other tokens as the torch loop gives them, which never looks at those pairs."""
+    m = block(64, 4, 96, 2, dtype=dtype, bias=bias).cuda()
+    gen = torch.Generator().manual_seed(2)
+    n, cap = 40, 12
+    idx = torch.stack([torch.zeros(n, dtype=torch.long), torch.arange(n) % 3 + 1], 1)   # expert 0: every token
+    idx[20:] = torch.tensor([0, 1])
+    counts = [0] * 4                       # pairs in expert order, ties in pair order: the first 12 of each are kept
+    kept = torch.zeros(n, 2, dtype=torch.bool)
+    for t in range(n):
+        for j in range(2):
+            kept[t, j] = counts[idx[t, j]] < cap
+            counts[idx[t, j]] += 1
+    lost = ~kept.any(1)
+    assert 5 < int(lost.sum()) < n
+    x, dout = torch.randn(n, 64, generator=gen), torch.randn(n, 64, generator=gen)
+    x[lost] = torch.tensor([float("inf"), float("nan"), float("-inf"), 3e38]).repeat(16)
+    tw = torch.rand(n, 2, generator=gen)
+    results = []
+    for path in (m._torch_experts, m._grouped_experts):
+        xc, tc = x.to("cuda", dtype).requires_grad_(), tw.to("cuda", dtype).requires_grad_()
+        out, c = path(xc, tc, idx.cuda(), cap)
+        params = [p for p in (m.W_in, m.W_out, m.b_in, m.b_out) if p is not None]
+        grads = torch.autograd.grad(out, (xc, tc, *params), dout.to("cuda", dtype))
+        assert c.tolist() == counts and int(m.dropped) == int((~kept).sum())
+        results.append([out.detach(), *grads])
+    for a, b in zip(*results):
+        assert bool(torch.isfinite(a).all()) and bool(torch.isfinite(b).all())
+        assert rel_l2(b, a) < TOL[dtype]
+    gone = lost.cuda()
+    assert not results[1][0][gone].any() and not results[1][1][gone].any()
+    assert not results[1][2][~kept.cuda()].any()
+
+
+@gpu
 def test_wide_block_with_fp32_weights_takes_16_bit_rows():
     """Weights in fp32, cast where they are used: the result of the 16-bit block with the same values, and fp32
     gradients."""
