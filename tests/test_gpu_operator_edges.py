@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from nanospeaker_b200 import Int4Weight, grouped_mm, int4_experts, kernels
+from test_operators import host  # noqa: F401  (the schedule's arithmetic, compiled for the host)
 
 pytestmark = pytest.mark.gpu
 
@@ -83,6 +84,43 @@ def test_int4_experts_what_is_not_finite_stays_with_its_token():
     keep = [i for i in range(40) if i not in (7, 20)]
     assert torch.equal(out[keep], want[keep])
     assert not torch.isfinite(out[7]).all() and torch.isnan(out[20]).any()
+
+
+# --------------------------------------------------------------------------- grouped products, bit for bit
+@pytest.mark.parametrize("k,n,rows,groups", [(64, 40, 40000, 14), (72, 264, 40000, 14), (264, 72, 40000, 14),
+                                             (304, 520, 100000, 8), (64, 64, 3000, 3)])
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+def test_grouped_whole_numbers_are_exact(k, n, rows, groups, dtype, layout, host):
+    """Rows of -1, 0 and 1: every fp32 sum is exact in any order, so results are those of 64 bits, rounded once, bit
+    for bit. Runs around one, two and three chunks of the weight gradient, around its 64-row stages and its 16-row
+    steps; NaN behind the last run."""
+    a, b = (k, n) if layout == "kn" else (n, k)       # (dw of a transposed weight is the product's transpose)
+    tiles = -(-a // 256) * -(-b // (256 if b > 128 else 128))
+    ks = host.chunk_rows(rows, groups, tiles, 74)
+    counts = [ks - 1, ks, ks + 1, 2 * ks - 17, 2 * ks + 63, 3 * ks + 16, 2 * ks, 65, 64, 63, 0, 15, 17, 1]
+    counts = counts[:groups] if groups > 3 else [ks + 1, 63, ks - 65]
+    cut = [0]
+    for c in counts:
+        cut.append(cut[-1] + c)
+    assert cut[-1] <= rows and max(counts) > ks
+    x, w = whole(-1, 1, rows, k).to(dtype), whole(-1, 1, groups, k, n, seed=1).to(dtype)
+    dy = whole(-1, 1, rows, n, seed=2).to(dtype)
+    if layout == "nk":
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    x[cut[-1]:], dy[cut[-1]:] = float("nan"), float("nan")
+    x.requires_grad_(), w.requires_grad_()
+    y = grouped_mm(x, w, torch.tensor(cut, dtype=torch.int32, device="cuda"))
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    kernels.check_status("cuda")
+    for g, (lo, hi) in enumerate(zip(cut, cut[1:])):
+        xg, wg, dg = x.detach()[lo:hi].double(), w.detach()[g].double(), dy[lo:hi].double()
+        assert torch.equal(y.detach()[lo:hi], (xg @ wg).to(dtype))
+        assert torch.equal(dx[lo:hi], (dg @ wg.T).to(dtype))
+        assert torch.equal(dw[g], (xg.T @ dg).to(dtype))
+        if hi - lo > 1:      # a run that is a row short is seen
+            assert not torch.equal(dw[g], (xg[:-1].T @ dg[:-1]).to(dtype))
+    assert not y.detach()[cut[-1]:].any() and not dx[cut[-1]:].any()
 
 
 # --------------------------------------------------------------------------- behind a reported input
