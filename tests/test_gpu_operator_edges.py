@@ -3,7 +3,7 @@ sums but the one under test are exact, calls behind a reported one, and what is 
 import pytest
 import torch
 
-from nanospeaker_b200 import Int4Weight, grouped_mm, int4_experts, kernels
+from nanospeaker_b200 import Int4Weight, grouped_mm, int4_experts, int4_mm, kernels
 from test_operators import host  # noqa: F401  (the schedule's arithmetic, compiled for the host)
 
 pytestmark = pytest.mark.gpu
@@ -14,6 +14,21 @@ HALF = (torch.bfloat16, torch.float16)
 def whole(lo, hi, *shape, seed=0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     return torch.randint(lo, hi + 1, shape, generator=g, device="cuda")
+
+
+# --------------------------------------------------------------------------- 4-bit products, bit for bit
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 16, 17, 32, 33, 64, 100])
+@pytest.mark.parametrize("k,n,group", [(8, 1, 32), (72, 40, 32), (576, 100, 64), (1000, 1537, 32), (4096, 48, 128),
+                                       (4104, 272, 64), (8192, 17, 128)])
+@pytest.mark.parametrize("dtype", HALF)
+def test_int4_mm_whole_numbers_are_exact(rows, k, n, group, dtype):
+    """Rows of -2 .. 2 and scales of 1, 1/2, 1/4 and 1/8: every fp32 sum is exact (below 2^17, in steps of 2^-3), so
+    the result is that of 64 bits, rounded once, bit for bit."""
+    x, q = whole(-2, 2, rows, k), whole(0, 15, k, n, seed=1)
+    s = 0.5 ** whole(0, 3, -(-k // group), n, seed=2).double()
+    w = (q - 8).double() * s.repeat_interleave(group, 0)[:k]
+    got = int4_mm(x.to(dtype), Int4Weight.from_levels(q.to(torch.uint8), s.to(dtype), group))
+    assert torch.equal(got, (x.double() @ w).to(dtype))
 
 
 # --------------------------------------------------------------------------- 4-bit experts: the hidden values
