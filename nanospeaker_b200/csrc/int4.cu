@@ -156,9 +156,11 @@ __device__ __forceinline__ void levels_of(uint32_t word, uint32_t* a) {
 }
 
 // Four at a time, side by side: one after another they were a tenth of a CTA's time. (Called, not copied to every
-// place: these kernels are over before much code has been fetched.)
+// place: these kernels are over before much code has been fetched.) tanh is CUDA's own: the block's 2 / (1 + exp(-2 g))
+// - 1 is off by 2^-24 however small g is, more than fp16's rounding below |g| = 2^-13.
 template <int ACT>
 __device__ __forceinline__ float4 act4(const float4& g) {
+  if constexpr (ACT == ACT_TANH) return make_float4(tanhf(g.x), tanhf(g.y), tanhf(g.z), tanhf(g.w));
   return make_float4(act_f<ACT>(g.x), act_f<ACT>(g.y), act_f<ACT>(g.z), act_f<ACT>(g.w));
 }
 __device__ __noinline__ float4 activation(int act, float4 g) {

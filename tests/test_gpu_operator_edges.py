@@ -90,6 +90,32 @@ def test_int4_experts_hidden_values_past_the_types_range(t, h, dtype):
     assert float(exact.abs().max()) < 65504 and bool((off <= bound).all())
 
 
+@pytest.mark.parametrize("t", [1, 12, 40])
+def test_int4_experts_small_gates_of_tanh(t):
+    """Gates of some 1e-5: tanh is right relative to its value (2 units of 2^-23 and fp32's rounding of the product:
+    2^-21), not to one. tanh by an exponential in fp32 does not hold the bound."""
+    d, h, e, dtype = 64, 16, 2, torch.bfloat16
+    x, q_in, q_out = whole(-2, 2, t, d), whole(0, 15, e, d, 2 * h, seed=1), whole(0, 15, e, h, d, seed=2)
+    s_in = torch.ones(e, 1, 2 * h, device="cuda", dtype=torch.float64)
+    s_in[..., :h] = 45 * 2.0 ** -28
+    idx = whole(0, e - 1, t, 1, seed=3)
+    pack = lambda q, s: Int4Weight.from_levels(q.to(torch.uint8), s.to(dtype), 64)  # noqa: E731
+    out = int4_experts(x.to(dtype), torch.ones(t, 1, dtype=dtype, device="cuda"), idx, pack(q_in, s_in),
+                       pack(q_out, torch.ones(e, 1, d, device="cuda")), "tanh").double()
+    a = torch.einsum("td,tdh->th", x.double(), (q_in - 8).double()[idx[:, 0]]) * s_in[0]
+    gate, up = a.chunk(2, 1)
+    down = (q_out - 8).double()[idx[:, 0]]
+    exact = torch.einsum("th,thd->td", torch.tanh(gate) * up, down)
+    magnitude = torch.einsum("th,thd->td", (torch.tanh(gate) * up).abs(), down.abs())
+    err = (4 * h * 2.0 ** -23 + 2.0 ** -15 + 2.0 ** -21) * magnitude
+    f = torch.finfo(dtype)
+    bound = f.eps / 2 * (exact.abs() + err) + err + f.smallest_normal * f.eps
+    assert bool(((out - exact).abs() <= bound).all())
+    one = 2 / (1 + torch.exp(-2 * gate.float())) - 1
+    loose = torch.einsum("th,thd->td", one.double() * up, down)
+    assert t < 40 or not bool(((loose.to(dtype).double() - exact).abs() <= bound).all())
+
+
 def test_int4_experts_what_is_not_finite_stays_with_its_token():
     args, _, _ = whole_experts(40, 64, 128, 3, 64, torch.float16)
     want = int4_experts(*args, "relu")
