@@ -70,11 +70,6 @@ class MoEBlock(nn.Module):
         fused into the GEMM epilogue on the kernel path), kernel, std.
     """
 
-    # Blocks that the kernels decline for their width or dtype run their experts' products as grouped_mm where this
-    # is set (off: the torch loop). A default of the class: a block that was saved whole before there was a choice has
-    # none of its own.
-    grouped = False
-
     def __init__(self, d_model, n_experts, d_ff=None, top_k=2, n_shared=0,
                  capacity_factor="auto", activation="silu", bias=False, normalize_weights=True,
                  aux_loss_coef=1e-2, noise_std=0.0, fused=True, kernel=True, std=0.02):
@@ -100,6 +95,9 @@ class MoEBlock(nn.Module):
         # how the kernel path sums a token's per-pair rows: None = the library default
         # (moe_kernel.get_combine_mode()), or "atomic" / "store" for this block
         self.combine_mode = None
+        # Blocks that the kernels decline for their width or dtype run their experts' products as
+        # grouped_mm where this is set (off: the torch loop, as before it existed).
+        self.grouped = False
         # a registered name bound to its registered function, and known to the epilogues
         named = ACTIVATIONS.get(self.activation) is act_fn and self.activation in KERNEL_ACTIVATIONS
         self._kernel_act = self.activation if named else None

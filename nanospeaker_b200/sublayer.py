@@ -79,8 +79,6 @@ class MoEFFNSublayer(nn.Module):
     device at every forward, so torch.manual_seed, activation checkpointing and graph replays treat it as
     they treat torch's own dropout. (0, the default, keeps the fused node.)"""
 
-    dropout = 0.0   # (of a sublayer that was saved whole before there was one, too)
-
     def __init__(self, ffn: MoEBlock, epsilon: float = 1e-6, dropout: float = 0.0):
         super().__init__()
         if not 0 <= dropout < 1:

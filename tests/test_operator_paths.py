@@ -34,21 +34,6 @@ def test_grouped_setting_changes_nothing_off_the_gpu():
     assert m.capacity_factor == cap and torch.equal(m(x), want)
 
 
-def test_modules_saved_before_the_settings_existed_still_run(tmp_path):
-    """Whole modules, as torch.save leaves them, without the newer attributes."""
-    sub = MoEFFNSublayer(block(64, 6, 96, 2))
-    x = torch.randn(20, 64)
-    want, _ = sub(x)
-    sub.__dict__.pop("dropout"), sub.ffn.__dict__.pop("grouped", None)
-    torch.save(sub, tmp_path / "m.pt")
-    old = torch.load(tmp_path / "m.pt", weights_only=False)
-    assert "dropout" not in vars(old) and "grouped" not in vars(old.ffn)
-    old.train()
-    assert torch.equal(old(x)[0], want) and old.ffn.capacity_factor == sub.ffn.capacity_factor
-    old.ffn.grouped = True
-    assert not block(64, 6, 96, 2).grouped
-
-
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_gradient_of_gathered_rows_is_rounded_once(device, dtype):
