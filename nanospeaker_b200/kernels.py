@@ -71,7 +71,8 @@ def status_word(device) -> torch.Tensor:
     key = (dev.type, dev.index if dev.index is not None else torch.cuda.current_device())
     w = _status_words.get(key)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=dev)
+        with torch.inference_mode(False):   # (one made by a call in inference mode could not be set back outside)
+            w = torch.zeros(1, dtype=torch.int32, device=dev)
         _status_words[key] = w
     return w
 

@@ -469,6 +469,22 @@ def test_widths_whose_last_tile_leaves_31_bits_are_refused(lib):
     _refused(Int4Weight, "outputs", torch.empty(1, 64, device="meta", dtype=torch.uint8), (8, odd), 64, torch.bfloat16)
 
 
+def test_status_word_of_a_call_in_inference_mode():
+    """A word that a serving call makes first is read and set back outside inference mode as well."""
+    from nanospeaker_b200 import kernels
+    dev = torch.device("cpu", 7)
+    with torch.inference_mode():
+        word = kernels.status_word(dev)
+    word.fill_(2)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="expert id"):
+            kernels.check_status(dev)
+        kernels.check_status(dev)
+        with torch.inference_mode():
+            kernels.status_word(dev).fill_(2)
+    kernels._status_words.pop(("cpu", 7))
+
+
 def low_level_calls(device):
     """Every low-level entry, by its function or its registered op, with one operand that does not have the length
     that another gives it."""
