@@ -159,6 +159,9 @@ class StackedMoEDecoder:
     @torch.no_grad()
     def _capture(self, x: torch.Tensor):
         static_x = x.clone()
+        if self.weights == "int4":   # on the caller's stream, which the graph is replayed on, not the warm-up's
+            for b in self.blocks:
+                self._int4_args(b, static_x)
         side = torch.cuda.Stream(device=x.device)
         side.wait_stream(torch.cuda.current_stream(x.device))
         with torch.cuda.stream(side):           # warm-up outside the capture (lazy initialisations)

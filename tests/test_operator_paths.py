@@ -355,6 +355,26 @@ def test_decoder_with_4_bit_weights(kw, dtype, t):
 
 
 @gpu
+def test_decoder_packs_its_weights_on_the_callers_stream(monkeypatch):
+    """What a replay reads belongs to the stream that it runs on: weights packed during the warm-up were the warm-up
+    stream's, and could be handed out again on it while a replay still read them."""
+    from nanospeaker_b200 import int4
+    seen = []
+    pack = int4.quantize_int4
+    monkeypatch.setattr(int4, "quantize_int4", lambda *a: (seen.append(torch.cuda.current_stream()), pack(*a))[1])
+    dec = StackedMoEDecoder([block(64, 8, 96, 2, 1, torch.bfloat16).cuda() for _ in range(2)], weights="int4")
+    x = torch.randn(5, 64, device="cuda").bfloat16()
+    mine = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), mine):
+        seen.clear()
+        dec.requantize()
+        with torch.cuda.stream(stream):
+            dec.step(x)
+        assert len(seen) == 8 and all(s == stream for s in seen)
+    torch.cuda.synchronize()
+
+
+@gpu
 def test_trained_with_dropout_on_grouped_products_then_served_in_4_bits():
     """The set as it is used: a wide block trained for a few steps inside the sublayer with dropout, its
     experts rounded to 4 bits, and the decode stack run on them."""
