@@ -156,6 +156,7 @@ class StackedMoEDecoder:
                                                                       combine=b.combine_mode or self.combine)
         return x
 
+    @torch.inference_mode(False)   # (the graph's input, made in inference mode, could not be written outside it)
     @torch.no_grad()
     def _capture(self, x: torch.Tensor):
         static_x = x.clone()

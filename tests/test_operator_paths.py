@@ -355,6 +355,20 @@ def test_decoder_with_4_bit_weights(kw, dtype, t):
 
 
 @gpu
+@pytest.mark.parametrize("weights", ["16bit", "int4"])
+def test_decoder_first_stepped_in_inference_mode(weights):
+    blocks = [block(576, 76, 192, 6, 2, torch.bfloat16).cuda() for _ in range(2)]
+    dec = StackedMoEDecoder(blocks, weights=weights)
+    x = torch.randn(5, 576, device="cuda").bfloat16()
+    with torch.inference_mode():
+        want = dec.step(x).clone()
+        held = x.clone()
+    assert torch.equal(dec.step(x), want) and torch.equal(dec.step(held), want)
+    with torch.inference_mode():
+        assert torch.equal(dec.step(x), want)
+
+
+@gpu
 def test_decoder_packs_its_weights_on_the_callers_stream(monkeypatch):
     """What a replay reads belongs to the stream that it runs on: weights packed during the warm-up were the warm-up
     stream's, and could be handed out again on it while a replay still read them."""
