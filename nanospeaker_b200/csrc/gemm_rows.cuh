@@ -477,6 +477,8 @@ __global__ void __launch_bounds__(rows_threads(EPI, GATHER), 1)
         }
         umma_commit(tfull_bar + b);
       }
+      // (whoever gave up, nobody reads on from here)
+      if (*abort_flag) mbar_drain(full_bar, it, STAGES);
     }
   } else if (epi_reduces(EPI) && warp >= 2 + EPI_WARPS) {
     // ------------------------------------------------------------------------ reducers

@@ -276,6 +276,9 @@ __global__ void __launch_bounds__(rows2_bound(EPI), 1)
         }
         umma_commit_2cta(tfull_bar + b, 3);     // the accumulators are ready in both CTAs
       }
+      // (whoever gave up, nobody reads on from here; the leader's barriers count both CTAs' bytes, and the pair leaves
+      // together)
+      if (*abort_flag) mbar_drain(full_bar, it, STAGES);
     }
   } else if (epi_reduces(EPI) && warp >= 2 + EPI_WARPS) {
     // ------------------------------------------------------------------------ reducers

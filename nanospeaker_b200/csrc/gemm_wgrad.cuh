@@ -412,6 +412,8 @@ __global__ void __launch_bounds__(GATHER ? WGRAD_THREADS_GATHER : WGRAD_THREADS,
         }
         umma_commit(tfull_bar + b);
       }
+      // (whoever gave up, nobody reads on from here)
+      if (*abort_flag) mbar_drain(full_bar, it, STAGES);
     }
   } else if (warp < 2 + EPI_WARPS) {
     const int ew = warp - 2;

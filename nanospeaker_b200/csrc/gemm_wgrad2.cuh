@@ -155,6 +155,9 @@ __global__ void __launch_bounds__(WGRAD_THREADS, 1)
         }
         umma_commit_2cta(tfull_bar + b, 3);
       }
+      // (whoever gave up, nobody reads on from here; the leader's barriers count both CTAs' bytes, and the pair leaves
+      // together)
+      if (*abort_flag) mbar_drain(full_bar, it, STAGES);
     }
   } else if (warp < 2 + EPI_WARPS) {
     const int ew = warp - 2;
