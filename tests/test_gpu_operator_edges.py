@@ -80,6 +80,15 @@ def test_int4_experts_hidden_values_are_not_held_in_the_type(t, e, d, h, group, 
         assert not bool(((held - exact).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("t,d,h,e,group", [(1, 8, 16, 1, 32), (7, 8, 48, 3, 128), (33, 24, 16, 2, 64),
+                                           (5000, 40, 80, 3, 64), (70, 584, 48, 300, 32), (20, 64, 1040, 2, 128),
+                                           (9, 1096, 64, 3, 64), (2500, 64, 336, 40, 32)])
+def test_int4_experts_smallest_widths_and_prompts(t, d, h, e, group):
+    args, hid, down = whole_experts(t, d, h, e, group, torch.bfloat16)
+    off, bound, _ = hidden_bound(args, hid, down)
+    assert bool((off <= bound).all())
+
+
 @pytest.mark.parametrize("t,h", [(5, 128), (60, 528), (300, 64)])
 @pytest.mark.parametrize("dtype", HALF)
 def test_int4_experts_hidden_values_past_the_types_range(t, h, dtype):
