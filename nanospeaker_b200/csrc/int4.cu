@@ -135,7 +135,9 @@ struct Mma<__half> {
   }
 };
 
-// A packed word's eight levels as the four registers of an A fragment, values -8 .. 7. (fp16 has the bits for a
+// A packed word's eight levels as the four registers of an A fragment, values -8 .. 7: a level is laid into the lowest
+// bits of a power of two, which is then subtracted (as Kim, Henry, Fahim, Awadalla describe for quantised weights, "Who
+// Says Elephants Can't Run: Bringing Large Scale MoE Models into Cloud Scale Production", 2022). (fp16 has the bits for a
 // level where it lies, times 16: of three shifts one is left. 200 tokens of the wide block 55.4 -> 54.3 us.)
 template <typename T>
 __device__ __forceinline__ void levels_of(uint32_t word, uint32_t* a) {
