@@ -16,6 +16,10 @@
 // the activations' type it cost as much again as the rounding of the result (relative error against 64 bits: bf16
 // 0.0024 to 0.0027 in place of 0.0017, fp16 0.00029 in place of 0.00021).
 //
+// In a graph, us: one row of 4096 x 16384 12.9, 64 of 4096 x 4096 12.1; the experts of one token 8.8, of 64 14.9, of 200
+// tokens of the wide block (32 experts of 1024 x 768, four a token) 57.6. Figures further down compare the two sides of
+// one choice when it was made; the experts' are up to 5 us lower there, before hidden values had a second part.
+//
 // A chunk of 512 inputs of neighbouring strips (16 outputs each), levels and scales together, is one contiguous
 // piece: it comes to shared memory by one bulk copy (which costs the SM's copy engine some 50 cycles however
 // small it is). The rows of x, few, in any place and read by every CTA, come by 16-byte asynchronous copies.

@@ -20,9 +20,14 @@ class StackedMoEDecoder:
     size.
 
     weights="int4" holds the experts' weights (not the router's) in 4 bits with a scale per `group`
-    inputs, a quarter of the bytes; they are rounded once, on the first step (`requantize` after the
-    blocks' weights have changed). Then blocks of any width that is a multiple of 16 and bf16 or fp16
-    activations are taken, without biases or a capacity, four launches a layer (`int4_experts`).
+    inputs: a step reads a quarter of the bytes. They are rounded once, on the first step (`requantize` after
+    the blocks' weights have changed), and held beside the blocks' own, which stay. Then blocks of any width
+    that is a multiple of 16 and bf16 or fp16 activations are taken, without biases or a capacity, block by
+    block: nine launches a layer, three of them `int4_experts`, the others the router's (a library product,
+    top-k, casts) and the residual's; ten with fp32 parameters. Blocks that the one-kernel stack takes are
+    faster on it at any batch measured (d_model 576, 76 experts, 1 / 16 / 64 tokens: 15.8 / 16.6 / 21.3 us a
+    layer, in 4 bits 20.8 / 29.6 / 43.3); blocks that it does not take are faster in 4 bits than on grouped
+    products (1024 wide, 32 experts: 25.7 / 36.8 / 45.5 us against 98.9 / 125.6 / 149.4).
 
     step(x) runs the stack on x [T, d_model] and returns the result (a tensor owned by the runner:
     it is overwritten by the next step with the same T). The first call for a given T captures the
