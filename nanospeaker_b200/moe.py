@@ -232,20 +232,24 @@ class MoEBlock(nn.Module):
         last run, where the products do not look: neither values nor gradients of theirs, finite or not, reach
         anything. A token's rows are summed in fp32 in pair order: reproducible bit for bit."""
         experts, order, token_idx, counts = self._plan(topk_idx)
-        offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
-        at = torch.arange(order.numel(), device=x.device)
+        runs = counts.clamp(max=cap) if cap else counts
+        offsets = torch.cat([counts.new_zeros(1), runs.cumsum(0)])
+        row = torch.arange(order.numel(), device=x.device)     # of the sorted pairs
         kept = None
         if cap:
-            fits = at - offsets[experts] < cap
-            self.dropped = (~fits).sum().detach()
-            offsets = torch.cat([counts.new_zeros(1), counts.clamp(max=cap).cumsum(0)])
-            to = torch.where(fits, fits.cumsum(0) - 1, offsets[-1] + (~fits).cumsum(0) - 1)
-            experts, order, token_idx = (torch.empty_like(t).index_copy_(0, to, t)
-                                         for t in (experts, order, token_idx))
-            kept = torch.empty_like(fits).index_copy_(0, order, at < offsets[-1]).view(topk_idx.shape)
+            self.dropped = order.numel() - offsets[-1]
+            at = row - (counts.cumsum(0) - counts)[experts]
+            fits = at < cap
+            # (a row each for the dropped pairs, too: one for all of them would be a single long sum in the backward)
+            row = torch.where(fits, at + offsets[experts], (~fits).cumsum(0) + (offsets[-1] - 1))
+            token_idx = torch.empty_like(token_idx).index_copy_(0, row, token_idx)
+            if self.b_in is not None:
+                experts = torch.empty_like(experts).index_copy_(0, row, experts)
+            kept = torch.empty_like(fits).index_copy_(0, order, fits).view(*topk_idx.shape, 1)
         offsets = offsets.to(torch.int32)
-        place = torch.empty_like(order).index_copy_(0, order, at)
-        a = grouped_mm(_PairRows.apply(x, token_idx, place), self.W_in.to(x.dtype), offsets)
+        place = torch.empty_like(order).index_copy_(0, order, row)
+        rows = _PairRows.apply(x, token_idx, place) if torch.is_grad_enabled() else x[token_idx]
+        a = grouped_mm(rows, self.W_in.to(x.dtype), offsets)
         if self.b_in is not None:
             a = a + self.b_in.float()[experts].to(x.dtype)   # (its gradient is then summed in fp32)
         gate, up = a.chunk(2, dim=-1)
@@ -253,9 +257,9 @@ class MoEBlock(nn.Module):
         if self.b_out is not None:
             y = y + self.b_out.float()[experts].to(x.dtype)
         rows = y[place].view(*topk_idx.shape, self.d_model)
-        if kept is not None:
-            rows, topk_w = torch.where(kept[..., None], rows, 0.0), torch.where(kept, topk_w, 0.0)
         rows = rows.float() * topk_w[..., None].float()
+        if kept is not None:
+            rows = torch.where(kept, rows, 0.0)
         return rows.sum(1).to(x.dtype), counts
 
     # ------------------------------------------------------------------------------ forward
